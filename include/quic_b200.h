@@ -300,6 +300,131 @@ int32_t quic_attn_decode_streams(int32_t b, int32_t s_max);
 int64_t quic_attn_scratch_bytes(int32_t b, int32_t splits);
 
 /* ------------------------------------------------------------------------
+ * Several tokens per forward: trees of drafted tokens over blocks of KV memory.
+ * No counterpart in the reference, whose cache grows by torch.cat and whose
+ * decode takes one token at a time (src/model.py:160, src/engine.py:78-107).
+ *
+ * Rows of all requests lie one after the other: request b has rows row_start[b]
+ * .. row_start[b + 1] - 1, row i of it is node i of its tree (or token i of a
+ * chain).  Position p of request b is cached in block tables[b][p / block_size]
+ * at offset p % block_size of planes [n_blocks, kv heads, block_size, dim], so
+ * the slots of a slotted cache are blocks of s_max tokens.  Node i has its K and
+ * V at position lengths[b] + i, behind the request's lengths[b] cached tokens.
+ * The parent of node i is a node before it; node 0 has none (-1).  A mask row
+ * has a bit per node, 32 to a word, set for the nodes that the row sees.
+ * ---------------------------------------------------------------------- */
+#define QUIC_DTYPE_F16 0
+#define QUIC_DTYPE_BF16 1
+
+typedef struct {
+  /* Strides in elements; the innermost dimension is contiguous.  Bases are
+   * 16-byte aligned, strides of q, k and v multiples of 8. */
+  const void *q;  /* [rows, heads, dim] */
+  const void *k;  /* [n_blocks, kv_heads, block_size, dim] */
+  const void *v;
+  void *out;      /* [rows, heads, dim] contiguous */
+  int64_t q_row, q_head, k_block, k_head, k_tok, v_block, v_head, v_tok;
+  const int32_t *tables; /* [requests, max_blocks], rows table_row apart */
+  int64_t table_row;
+  const int32_t *lengths;   /* [requests] cached tokens before the rows */
+  const int32_t *row_start; /* [requests + 1] */
+  const int32_t *mask;      /* [rows, mask_words], rows mask_row apart, or NULL:
+                               row i sees rows 0 .. i of its request */
+  int64_t mask_row;
+  int32_t mask_words;
+  int32_t rows, requests, heads, kv_heads, dim; /* dim 64 or 128 */
+  int32_t n_blocks, block_size, max_blocks;
+  int32_t dtype;   /* QUIC_DTYPE_* of q, k, v and out */
+  int32_t max_new; /* rows of one request at most; what is beyond stays unwritten */
+  int64_t max_len; /* lengths[] at most, for the plan; longer requests are still
+                      read to their end, by fewer CTAs than would be best */
+  float scale;     /* <= 0: dim^-0.5 */
+} quic_tree_attn_t;
+
+/* Attention of every row over its request's cached tokens and the nodes that it
+ * sees.  fp32 scores, softmax and sums; the weights multiply V rounded to the
+ * tensors' type.  A row that sees nothing yields zeros; a position whose block
+ * is outside 0 .. n_blocks - 1 is seen by nobody; rows before row_start[0] and
+ * from row_start[requests] on are left as they were.  K and V of positions that
+ * a row does not see do not reach it, whatever they hold.  `scratch` (16-byte
+ * aligned, need not be initialised) is used when several CTAs share a request's
+ * keys: quic_tree_attn_scratch_bytes of the call's numbers. */
+int quic_tree_attn(const quic_tree_attn_t *t, void *scratch, void *stream);
+int64_t quic_tree_attn_scratch_bytes(int32_t rows, int32_t requests,
+                                     int32_t heads, int32_t kv_heads,
+                                     int32_t dim, int32_t max_new,
+                                     int64_t max_len);
+
+/* What a step needs to know of its requests, built on the device from their
+ * lengths.  n_new[b] > 0: request b gets that many rows behind lengths[b] cached
+ * tokens, and from the pool the blocks that it needs for them beyond its held[b]
+ * (in table order).  0: it is left alone.  < 0: it has ended, its blocks go back.
+ * pool int32 [4 + n_blocks]: head, count, 0, status, and a ring of block ids of
+ * which `count` from `head` on are free.  Blocks come from the ring's head in
+ * the order of the requests and go back behind its tail, where this call does
+ * not yet take them.  Updates tables, held and pool in place; writes
+ *   row_start int32 [requests + 1], the exclusive sum of the rows;
+ *   slot_map int64 [max_rows], block * block_size + offset of every row, -1
+ *     behind the last one;
+ *   positions int32 [max_rows], lengths[b] + depth of the row's node in its tree
+ *     (parents NULL: its number), 0 behind the last one;
+ *   mask int32 [max_rows, mask_words] (with parents), the node's ancestors and
+ *     itself, 0 behind the last one.
+ * parents int32 [max_rows] or NULL; an entry that is no earlier node counts as
+ * -1.  All or nothing: where the pool lacks blocks (status: how many), a request
+ * needs more than max_blocks (status -1), or there are more rows than max_rows or,
+ * with parents, than 32 * mask_words in a request (status -2), no request gets
+ * rows or blocks: row_start is all 0.  Ended requests give theirs back all the
+ * same.  Status 0: done.  A pool serves one stream at a time.  At most 4096
+ * requests and 65535 * 256 rows.  Positions reach 2^29 at most. */
+int quic_block_tables(int32_t *tables, int64_t table_row, int32_t max_blocks,
+                      int32_t *held, int32_t *pool, int32_t n_blocks,
+                      const int32_t *lengths, const int32_t *n_new,
+                      int32_t requests, int32_t block_size,
+                      const int32_t *parents, int32_t *row_start,
+                      int64_t *slot_map, int32_t *positions, int32_t *mask,
+                      int32_t mask_words, int32_t max_rows, void *stream);
+
+typedef struct {
+  /* [layers, 2 (K, V), n_blocks, kv_heads, block_size, dim] of 2-byte elements,
+   * strides in elements and multiples of 8, base 16-byte aligned */
+  void *kv;
+  int64_t kv_layer, kv_kind, kv_block, kv_head, kv_tok;
+  const int32_t *tables;
+  int64_t table_row;
+  const int32_t *lengths, *row_start, *parents; /* [requests], [requests + 1], [rows] */
+  const void *tokens;  /* [rows] the drafted tokens: int32, or int64 with token_bytes 8 */
+  const void *targets; /* [rows] the target's choice after each, same type */
+  int32_t token_bytes;
+  int32_t layers, n_blocks, kv_heads, block_size, dim, max_blocks;
+  int32_t rows, requests;
+  int32_t max_new;      /* rows of one request at most, 1024; larger ones are left alone */
+  int32_t *path;        /* [requests, max_new] accepted nodes, -1 behind them */
+  int32_t *accepted;    /* [requests] how many */
+  void *next_token;     /* [requests], as tokens: the target's choice after the last; -1 without rows */
+  int32_t *new_lengths; /* [requests] lengths + accepted; not lengths itself */
+} quic_tree_commit_t;
+
+/* Keeps the branch of each tree that the target agrees with.  Node 0 is right by
+ * definition; of the children of an accepted node the first whose token is the
+ * target's choice at that node is accepted, and so on.  K and V of accepted node
+ * number j move from position lengths[b] + path[j] to lengths[b] + j, in every
+ * layer.  Positions whose block is outside 0 .. n_blocks - 1 are not moved. */
+int quic_tree_commit(const quic_tree_commit_t *t, void *stream);
+
+/* quic_qkv_rope_append with the place in the cache apart from the position of
+ * the rotation: row r is rotated as position positions[r] and appended at block
+ * slot_map[r] / block_size, offset slot_map[r] % block_size of planes [n_blocks,
+ * 2, block_size, 64]; nothing is appended where slot_map[r] is outside 0 ..
+ * n_blocks * block_size - 1. */
+int quic_qkv_rope_append_at(const void *qkv_f16, const int64_t *slot_map,
+                            const int32_t *positions, const void *cos_f16,
+                            const void *sin_f16, int32_t max_pos,
+                            void *q_out_f16, void *kcache_f16,
+                            void *vcache_f16, int32_t block_size,
+                            int32_t n_blocks, int32_t rows, void *stream);
+
+/* ------------------------------------------------------------------------
  * The fused decode step (one token for every active row).
  * Replaces Engine.step + QUICForCausalLM.forward with seq_len == 1
  * (src/engine.py:78-107, src/model.py:272-303): embedding gather, 24 decoder

@@ -243,11 +243,13 @@ __global__ void embed_rows_kernel(const half* __restrict__ embed, const int32_t*
 // already added) of a prefill: every row brings its own slot and position, q is written
 // head-major.  One thread per (row, head, 8 of the 64 dims), which reads the 8 stored pairs
 // its dims come from (32 bytes) with their cos / sin (16 bytes each) and writes 16 bytes.
+// kAt: row b goes to place at[b] of the cache, slot x s_max + position, instead of (slots[b], row_pos[b]).
+template <bool kAt>
 __global__ void __launch_bounds__(256) qkv_rope_rows_kernel(
     const half* __restrict__ qkv, const int32_t* __restrict__ slots, const int32_t* __restrict__ row_pos,
     const half* __restrict__ cos_t, const half* __restrict__ sin_t, int max_pos, half* __restrict__ qbuf,
     half* __restrict__ kcache, half* __restrict__ vcache, int s_max, int rows, int n_slots,
-    const float* __restrict__ part, int splits, const half* __restrict__ bias) {
+    const float* __restrict__ part, int splits, const half* __restrict__ bias, const int64_t* __restrict__ at) {
   constexpr int kPerRow = (kHeads + 2 * kKvHeads) * 8;  // 144 threads per row
   const size_t idx = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
   pdl_launch_dependents();
@@ -257,7 +259,7 @@ __global__ void __launch_bounds__(256) qkv_rope_rows_kernel(
   const int head = rem >> 3, piece = rem & 7;   // piece: dims 8 piece .. 8 piece + 7
   const int pair0 = (piece & 3) * 8;            // their pairs: dims d and d + 32 are stored side by side
   const bool high = piece >= 4;                 // dims 32..63: the second element of the rotated pair
-  const int slot = slots[b], p = row_pos[b];
+  const int p = row_pos[b];
   const size_t col = (size_t)head * kHeadDim + 2 * pair0;
   uint4 in0, in1;
   if (part != nullptr) {  // the linear's K splits, summed, rounded and biased as its own finish would
@@ -316,10 +318,19 @@ __global__ void __launch_bounds__(256) qkv_rope_rows_kernel(
   if (head < kHeads) {
     dst = qbuf + ((size_t)head * rows + b) * kHeadDim;
   } else {
-    if (p >= s_max || p < 0 || slot < 0 || slot >= n_slots) return;  // nothing is appended for such a row
+    int slot, place = p;
+    if constexpr (kAt) {
+      const int64_t where = at[b];
+      if (where < 0 || where >= (int64_t)n_slots * s_max) return;  // nothing is appended for such a row
+      slot = (int)(where / s_max);
+      place = (int)(where - (int64_t)slot * s_max);
+    } else {
+      slot = slots[b];
+      if (p >= s_max || p < 0 || slot < 0 || slot >= n_slots) return;
+    }
     const int kvh = (head - kHeads) & 1;
     half* base = (head < kHeads + kKvHeads) ? kcache : vcache;
-    dst = base + (((size_t)slot * kKvHeads + kvh) * s_max + p) * kHeadDim;
+    dst = base + (((size_t)slot * kKvHeads + kvh) * s_max + place) * kHeadDim;
   }
   *reinterpret_cast<uint4*>(dst + piece * 8) = *reinterpret_cast<const uint4*>(out);
 }
@@ -375,8 +386,8 @@ cudaError_t launch_qkv_rope_append(const half* qkv, const int32_t* slots, const 
                                    int n_slots, int rows, cudaStream_t st, bool pdl, const float* part, int splits,
                                    const half* bias) {
   const size_t total = (size_t)rows * (kHeads + 2 * kKvHeads) * 8;
-  return launch(qkv_rope_rows_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, pdl, qkv, slots, positions,
-                cos_t, sin_t, max_pos, q_out, kcache, vcache, s_max, rows, n_slots, part, splits, bias);
+  return launch(qkv_rope_rows_kernel<false>, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, pdl, qkv, slots, positions,
+                cos_t, sin_t, max_pos, q_out, kcache, vcache, s_max, rows, n_slots, part, splits, bias, (const int64_t*)nullptr);
 }
 cudaError_t launch_rmsnorm_part(const float* part, int splits, const half* residual, const half* w, float eps,
                                 half* y, half* sum_out, int rows, cudaStream_t st) {
@@ -464,6 +475,25 @@ extern "C" int quic_qkv_rope_append(const void* qkv, const int32_t* slots, const
   QUIC_CUDA(launch_qkv_rope_append((const half*)qkv, slots, positions, (const half*)cos_t, (const half*)sin_t,
                                    (int)max_pos, (half*)q_out, (half*)kcache, (half*)vcache, (int)s_max, (int)n_slots,
                                    (int)rows, (cudaStream_t)stream, false));
+  return QUIC_OK;
+}
+
+extern "C" int quic_qkv_rope_append_at(const void* qkv, const int64_t* slot_map, const int32_t* positions, const void* cos_t,
+                                       const void* sin_t, int32_t max_pos, void* q_out, void* kcache, void* vcache,
+                                       int32_t block_size, int32_t n_blocks, int32_t rows, void* stream) {
+  QUIC_REQUIRE(rows == 0 || (qkv && slot_map && positions && cos_t && sin_t && q_out && kcache && vcache), QUIC_E_ARG,
+               "qkv_rope_append_at: null tensor");
+  QUIC_REQUIRE(rows >= 0 && rows <= (1 << 20) && block_size >= 1 && max_pos >= 1 && n_blocks >= 1, QUIC_E_SHAPE,
+               "qkv_rope_append_at: bad row count or cache geometry");
+  QUIC_REQUIRE(((uintptr_t)qkv | (uintptr_t)cos_t | (uintptr_t)sin_t | (uintptr_t)q_out | (uintptr_t)kcache |
+                (uintptr_t)vcache) % 16 == 0,
+               QUIC_E_ARG, "qkv_rope_append_at: tensors must be 16-byte aligned");
+  if (rows == 0) return QUIC_OK;
+  const size_t total = (size_t)rows * (kHeads + 2 * kKvHeads) * 8;
+  QUIC_CUDA(launch(qkv_rope_rows_kernel<true>, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (cudaStream_t)stream, false,
+                   (const half*)qkv, (const int32_t*)nullptr, positions, (const half*)cos_t, (const half*)sin_t, (int)max_pos,
+                   (half*)q_out, (half*)kcache, (half*)vcache, (int)block_size, (int)rows, (int)n_blocks, (const float*)nullptr, 0,
+                   (const half*)nullptr, slot_map));
   return QUIC_OK;
 }
 

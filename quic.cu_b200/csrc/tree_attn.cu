@@ -1,0 +1,489 @@
+// Attention of drafted trees over a blocked KV cache.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(scale q_i . k_j)
+//
+// for node i of a request's tree over the request's cached positions 0 .. len - 1 and those of the nodes (position
+// len + a for node a) that it sees: its ancestors and itself by bit mask, or without masks nodes 0 .. i.  A chain, the next
+// chunk of a prompt and a single decode token are trees too.  The R = nodes x (query heads per KV head) rows of a
+// request and KV head share their keys; K and V are read once per tile of those rows.
+//
+// This file: the form for few rows (mma.sync), which takes every call, the merge of a request's parts, and the entry point.
+// A CTA has 16 or 32 rows and a part of the keys, which its four warps walk 32 at a time, each through a ring of its own
+// (cp.async, no barrier between warps), one pass with a running maximum and sum per row; the warps' results meet in
+// shared memory at the end, those of several CTAs in the merge kernel.  Bound: the bytes of K and V.
+#include <math.h>
+
+#include "tree_attn.cuh"
+
+namespace quic {
+namespace {
+
+constexpr int kWarps = 4, kKeys = 32;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {  // zeros beyond `bytes`
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int D>
+constexpr int kStages = D == 64 ? 3 : 2;
+template <int D>
+constexpr uint32_t kRowsBytes = kKeys * D * 2;                       // K (or V) of a tile
+template <int D, int MT>
+constexpr uint32_t kSmem = kWarps * kStages<D> * 2 * kRowsBytes<D> > kWarps * MT * 16 * (D + 4) * 4
+                               ? kWarps * kStages<D> * 2 * kRowsBytes<D>
+                               : kWarps * MT * 16 * (D + 4) * 4;
+
+// Tile element (row, 16-byte chunk): chunks swapped by row so that eight rows of a chunk lie in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
+  return row * (D * 2) + ((chunk ^ (row & 7)) << 4);
+}
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ uint32_t valid_s[kWarps][kStages<D>];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int split = blockIdx.x, kvh = blockIdx.y % a.kv_heads, tile = blockIdx.y / a.kv_heads;
+  const TreeRequest r = tree_request(a, blockIdx.z);
+  const int all = min(r.n, a.max_new) * (int)a.group.d, r0 = tile * 16 * MT;  // row = node x group + head of the group
+  if (r0 >= all) return;
+  int per;
+  const int parts = tree_parts(a, r.end, per);
+  if (split >= parts) return;
+  const int t_begin = split * per, t_end = min(t_begin + per, r.end);
+  const int32_t* table = a.tables + (int64_t)blockIdx.z * a.table_row;
+
+  // ---- queries: A fragments of every 16 rows
+  uint32_t qf[MT][D / 16][4];
+  int node[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = r0 + 16 * m + 8 * h + g;
+      node[m][h] = (int)a.group.div(row);
+      const int head = kvh * (int)a.group.d + row - node[m][h] * (int)a.group.d;
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(a.q) + (int64_t)(r.start + node[m][h]) * a.q_row +
+                                                            (int64_t)head * a.q_head);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        qf[m][ks][h] = row < all ? __ldg(q + 8 * ks + c) : 0u;
+        qf[m][ks][2 + h] = row < all ? __ldg(q + 8 * ks + 4 + c) : 0u;
+      }
+      if (row >= all) node[m][h] = 0;
+    }
+
+  // ---- the warp's ring
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * kStages<D> * 2 * kRowsBytes<D>;
+  constexpr int kPer = D / 8, kAtOnce = 32 / kPer;  // chunks of a row, rows of one instruction
+  const int step = kWarps * kKeys;
+  // the block of position t + lane, or -1 where there is none
+  auto fetch = [&](int t) {
+    const int p = t + lane;
+    const int id = p < t_end ? __ldg(table + a.block.div(p)) : -1;
+    return id < a.n_blocks ? id : -1;
+  };
+  auto request = [&](int t, int stage, int id) {
+    const uint32_t ok = __ballot_sync(0xffffffffu, id >= 0);
+    if (lane == 0) valid_s[warp][stage] = ok;
+    const int p = t + lane, off = p - (int)a.block.div(p) * (int)a.block.d;
+    const uint32_t dst = ring + stage * 2 * kRowsBytes<D>;
+    const int chunk = lane % kPer;
+#pragma unroll
+    for (int i = 0; i < kKeys / kAtOnce; ++i) {
+      const int row = i * kAtOnce + lane / kPer;
+      const int bid = __shfl_sync(0xffffffffu, id, row), boff = __shfl_sync(0xffffffffu, off, row);
+      const int64_t at = max(bid, 0);
+      const int64_t o = bid >= 0 ? boff : 0;
+      const uint32_t bytes = bid >= 0 ? 16u : 0u;
+      cp_async16(dst + tile_at<D>(row, chunk), reinterpret_cast<const T*>(a.k) + at * a.k_block + kvh * a.k_head + o * a.k_tok + chunk * 8,
+                 bytes);
+      cp_async16(dst + kRowsBytes<D> + tile_at<D>(row, chunk),
+                 reinterpret_cast<const T*>(a.v) + at * a.v_block + kvh * a.v_head + o * a.v_tok + chunk * 8, bytes);
+    }
+  };
+
+  float o[MT][D / 8][4], m_run[MT][2], l_run[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
+    m_run[m][0] = m_run[m][1] = -INFINITY;
+    l_run[m][0] = l_run[m][1] = 0.f;
+  }
+
+  const int t_warp = t_begin + warp * kKeys;
+  int id = fetch(t_warp);
+#pragma unroll
+  for (int s = 0; s < kStages<D> - 1; ++s) {
+    if (t_warp + s * step < t_end) request(t_warp + s * step, s, id);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    id = fetch(t_warp + (s + 1) * step);
+  }
+  int stage = 0;
+  for (int t = t_warp; t < t_end; t += step) {
+    {
+      const int ahead = t + (kStages<D> - 1) * step;
+      const int to = stage == 0 ? kStages<D> - 1 : stage - 1;
+      if (ahead < t_end) request(ahead, to, id);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      id = fetch(ahead + step);
+    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages<D> - 1) : "memory");
+    __syncwarp();
+    const uint32_t k_at = ring + stage * 2 * kRowsBytes<D>, v_at = k_at + kRowsBytes<D>;
+    const uint32_t valid = valid_s[warp][stage];
+
+    // S = Q K^T
+    float s[MT][kKeys / 8][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < kKeys / 8; ++n) s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk)
+#pragma unroll
+      for (int n = 0; n < kKeys / 8; ++n) {
+        uint32_t b[4];
+        ldsm4(b, k_at + tile_at<D>(n * 8 + (lane & 7), kk * 4 + (lane >> 3)));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma<T>(s[m][n], qf[m][2 * kk], b[0], b[1]);
+          mma<T>(s[m][n], qf[m][2 * kk + 1], b[2], b[3]);
+        }
+      }
+
+    // what each row sees
+    const bool tree = t + kKeys > r.len, masked = tree || valid != 0xffffffffu;
+    uint32_t seen[MT][2];
+    if (masked) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          seen[m][h] = valid & tree_visible32(a, r, node[m][h], t);
+#pragma unroll
+          for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (!(seen[m][h] >> (8 * n + 2 * c + e) & 1u)) s[m][n][2 * h + e] = -INFINITY;
+        }
+    }
+
+    // running maximum and sum
+    uint32_t p[MT][kKeys / 16][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < kKeys / 8; ++n) mx = fmaxf(mx, fmaxf(s[m][n][2 * h], s[m][n][2 * h + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(m_run[m][h], mx * a.scale_log2);  // (the scale is positive)
+        const float ref = m_new == -INFINITY ? 0.f : m_new, shifted = kTreeShift<T> - ref;
+        const float alpha = tree_ex2(m_run[m][h] - ref);
+        m_run[m][h] = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < kKeys / 8; ++n) {
+          const uint32_t w = tree_pack<T>(tree_ex2(fmaf(s[m][n][2 * h], a.scale_log2, shifted)),
+                                          tree_ex2(fmaf(s[m][n][2 * h + 1], a.scale_log2, shifted)));
+          p[m][n >> 1][2 * (n & 1) + h] = w;
+          const float2 f = tree_unpack<T>(w);  // what the product will see: the weights sum to one
+          sum += f.x + f.y;
+        }
+        l_run[m][h] = l_run[m][h] * alpha + sum;
+        if (alpha != 1.f) {
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            o[m][n][2 * h] *= alpha;
+            o[m][n][2 * h + 1] *= alpha;
+          }
+        }
+      }
+
+    // A node's infinity or NaN reaches the rows that see the node only: weight zero times it would be NaN in all others.
+    if (tree) {
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < kKeys / kAtOnce; ++i) {
+        const uint4 w = *reinterpret_cast<const uint4*>(smem + (v_at - (uint32_t)__cvta_generic_to_shared(smem)) +
+                                                        tile_at<D>(i * kAtOnce + lane / kPer, lane % kPer));
+        odd |= tree_not_finite<T>(w.x) || tree_not_finite<T>(w.y) || tree_not_finite<T>(w.z) || tree_not_finite<T>(w.w);
+      }
+      if (__any_sync(0xffffffffu, odd)) {
+        unsigned char* v_tile = smem + (v_at - (uint32_t)__cvta_generic_to_shared(smem));
+        for (int key = 0; key < kKeys; ++key) {
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(v_tile + tile_at<D>(key, n) + 4 * c);
+            if (tree_not_finite<T>(w)) {
+              const float2 f = tree_unpack<T>(w), z = tree_unpack<T>(tree_finite<T>(w));
+#pragma unroll
+              for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  if (seen[m][h] >> key & 1u) {
+                    o[m][n][2 * h] += f.x - z.x;  // (x - x = 0 for what is finite)
+                    o[m][n][2 * h + 1] += f.y - z.y;
+                  }
+            }
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kKeys / kAtOnce; ++i) {
+          uint4* const at = reinterpret_cast<uint4*>(v_tile + tile_at<D>(i * kAtOnce + lane / kPer, lane % kPer));
+          uint4 w = *at;
+          w.x = tree_finite<T>(w.x), w.y = tree_finite<T>(w.y), w.z = tree_finite<T>(w.z), w.w = tree_finite<T>(w.w);
+          *at = w;
+        }
+        __syncwarp();
+      }
+    }
+
+    // O += P V
+#pragma unroll
+    for (int jk = 0; jk < kKeys / 16; ++jk)
+#pragma unroll
+      for (int cc = 0; cc < D / 16; ++cc) {
+        uint32_t b[4];
+        ldsm4_t(b, v_at + tile_at<D>(jk * 16 + (lane >> 3 & 1) * 8 + (lane & 7), 2 * cc + (lane >> 4)));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma<T>(o[m][2 * cc], p[m][jk], b[0], b[1]);
+          mma<T>(o[m][2 * cc + 1], p[m][jk], b[2], b[3]);
+        }
+      }
+    __syncwarp();  // (the stage is requested anew in the next round)
+    stage = stage == kStages<D> - 1 ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  pdl_launch_dependents();
+
+  // ---- the four warps' parts
+  constexpr int kRows = MT * 16, kLine = D + 4;  // a row: D values, maximum, sum
+  float* const mine = reinterpret_cast<float*>(smem) + warp * kRows * kLine;
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float* line = mine + (16 * m + 8 * h + g) * kLine;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(line + 8 * n + 2 * c) = make_float2(o[m][n][2 * h], o[m][n][2 * h + 1]);
+      float l = l_run[m][h];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (c == 0) line[D] = l != l ? INFINITY : m_run[m][h], line[D + 1] = l;  // (a maximum passes over NaN)
+    }
+  __syncthreads();
+  for (int i = tid; i < kRows * (D / 2); i += kWarps * 32) {
+    const int row = i / (D / 2), d = 2 * (i % (D / 2));
+    if (r0 + row >= all) break;
+    const float* line = reinterpret_cast<const float*>(smem) + row * kLine;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, line[w * kRows * kLine + D]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float x = 0.f, y = 0.f, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float* at = line + w * kRows * kLine;
+      const float f = tree_ex2(at[D] - ref);
+      if (f != 0.f) {
+        x += f * at[d];
+        y += f * at[d + 1];
+        l += f * at[D + 1];
+      }
+    }
+    const int nd = (int)a.group.div(r0 + row), head = kvh * (int)a.group.d + (r0 + row) - nd * (int)a.group.d;
+    const int64_t line_out = (int64_t)(r.start + nd) * a.heads + head;
+    if (parts == 1) {
+      const float inv = l != 0.f ? 1.f / l : 0.f;  // (NaN stays)
+      *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + line_out * D + d) = tree_pack<T>(x * inv, y * inv);
+    } else {
+      *reinterpret_cast<float2*>(a.part_o + (line_out * a.splits + split) * D + d) = make_float2(x, y);
+      if (d == 0) a.part_ml[line_out * a.splits + split] = make_float2(top, l);
+    }
+  }
+}
+
+// A row and head whose keys several CTAs shared: sum of the parts, each by 2^(its maximum - the largest).  One warp each.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a) {
+  const int lane = threadIdx.x & 31;
+  const TreeRequest r = tree_request(a, blockIdx.y);
+  int per;
+  const int parts = tree_parts(a, r.end, per);
+  pdl_wait();
+  if (parts == 1) return;
+  const int rows = min(r.n, a.max_new) * a.heads;
+  for (int i = blockIdx.x * 4 + (threadIdx.x >> 5); i < rows; i += gridDim.x * 4) {
+    const int64_t line = (int64_t)r.start * a.heads + i;
+    const float2* ml = a.part_ml + line * a.splits;
+    float top = -INFINITY;
+    for (int s = lane; s < parts; s += 32) top = fmaxf(top, ml[s].x);
+    top = warp_max(top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float l = 0.f, o[D / 32] = {};
+    for (int s0 = 0; s0 < parts; s0 += 32) {
+      float f = 0.f;
+      if (s0 + lane < parts) {
+        const float2 x = ml[s0 + lane];
+        f = tree_ex2(x.x - ref);
+        if (f != 0.f) l += f * x.y;
+      }
+#pragma unroll 8
+      for (int s = 0; s < min(32, parts - s0); ++s) {
+        const float w = __shfl_sync(0xffffffffu, f, s);
+        const float* at = a.part_o + (line * a.splits + s0 + s) * D + lane * (D / 32);
+        float x[D / 32];
+        if constexpr (D == 64) {
+          const float2 u = *reinterpret_cast<const float2*>(at);
+          x[0] = u.x, x[1] = u.y;
+        } else {
+          const float4 u = *reinterpret_cast<const float4*>(at);
+          x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+        }
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+          if (w != 0.f) o[d] += w * x[d];
+      }
+    }
+    l = warp_sum(l);
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + line * D) + lane * (D / 64);
+#pragma unroll
+    for (int d = 0; d < D / 64; ++d) out[d] = tree_pack<T>(o[2 * d] * inv, o[2 * d + 1] * inv);
+  }
+}
+
+template <typename T, int D, int MT>
+int launch_few(const TreeArgs& a, cudaStream_t st) {
+  const int tiles = (int)(((int64_t)a.max_new * a.group.d + 16 * MT - 1) / (16 * MT));
+  QUIC_CUDA((allow_smem<tree_attn_kernel<T, D, MT>>(kSmem<D, MT>)));
+  QUIC_CUDA(launch(tree_attn_kernel<T, D, MT>, dim3(a.splits, a.kv_heads * tiles, a.requests), dim3(kWarps * 32), kSmem<D, MT>, st,
+                   false, a));
+  return QUIC_OK;
+}
+template <typename T, int D>
+int launch_typed(const TreeArgs& a, cudaStream_t st) {
+  const int rc = (int64_t)a.max_new * a.group.d <= 16 ? launch_few<T, D, 1>(a, st) : launch_few<T, D, 2>(a, st);
+  if (rc != QUIC_OK || a.splits == 1) return rc;
+  const int64_t warps = (int64_t)a.max_new * a.heads;
+  QUIC_CUDA(launch(tree_merge_kernel<T, D>, dim3((unsigned)((warps + 3) / 4), a.requests), dim3(128), 0, st, true, a));
+  return QUIC_OK;
+}
+
+constexpr int64_t kMostTokens = 1 << 29;  // of a request: sums of two counts stay within an int
+
+// CTAs that share a request's keys, and the tokens of one.  `bound` keys per request at most.
+void plan(int requests, int kv_heads, int heads, int max_new, int64_t bound, int dim, int& splits, int& chunk) {
+  const int64_t rows = (int64_t)max_new * (heads / kv_heads);
+  const int64_t units = (int64_t)requests * kv_heads * (rows <= 16 ? 1 : (rows + 31) / 32);
+  const int64_t ctas = 148 * (dim == 64 ? 2 : 1);
+  int64_t parts = units >= ctas ? 1 : ctas / units;
+  const int64_t most = (bound + 255) / 256;  // at least two tiles a warp
+  if (parts > most) parts = most;
+  if (parts < 1) parts = 1;
+  chunk = (int)(((bound + parts - 1) / parts + 63) / 64 * 64);
+  if (chunk < 64) chunk = 64;
+  splits = (int)((bound + chunk - 1) / chunk);
+  if (splits < 1) splits = 1;
+}
+
+bool plan_of(int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim, int32_t max_new, int64_t max_len, int& splits, int& chunk) {
+  if (requests < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || (dim != 64 && dim != 128) || max_new < 1 || max_len < 0)
+    return false;
+  const int64_t bound = max_len + max_new;
+  plan(requests, kv_heads, heads, max_new, bound < kMostTokens ? bound : kMostTokens, dim, splits, chunk);
+  return true;
+}
+
+}  // namespace
+}  // namespace quic
+
+using namespace quic;
+
+extern "C" int64_t quic_tree_attn_scratch_bytes(int32_t rows, int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim,
+                                                int32_t max_new, int64_t max_len) {
+  int splits, chunk;
+  if (rows < 0 || !plan_of(requests, heads, kv_heads, dim, max_new, max_len, splits, chunk)) return 0;
+  return splits == 1 ? 0 : (int64_t)rows * heads * splits * (dim + 2) * 4;
+}
+
+extern "C" int quic_tree_attn(const quic_tree_attn_t* t, void* scratch, void* stream) {
+  QUIC_REQUIRE(t != nullptr, QUIC_E_ARG, "tree_attn: null arguments");
+  QUIC_REQUIRE(t->dtype == QUIC_DTYPE_F16 || t->dtype == QUIC_DTYPE_BF16, QUIC_E_SHAPE, "tree_attn: unknown element type");
+  QUIC_REQUIRE(t->dim == 64 || t->dim == 128, QUIC_E_SHAPE, "tree_attn: the head dimension is 64 or 128");
+  QUIC_REQUIRE(t->rows >= 0 && t->requests >= 0 && t->heads >= 1 && t->kv_heads >= 1 && t->heads % t->kv_heads == 0, QUIC_E_SHAPE,
+               "tree_attn: bad row, request or head count");
+  QUIC_REQUIRE(t->n_blocks >= 1 && t->block_size >= 1 && t->max_blocks >= 1 && (int64_t)t->block_size * t->max_blocks <= kMostTokens,
+               QUIC_E_SHAPE, "tree_attn: bad block geometry");
+  QUIC_REQUIRE(t->max_new >= 1 && t->max_len >= 0, QUIC_E_SHAPE, "tree_attn: bad bounds of a request's rows or tokens");
+  if (t->rows == 0 || t->requests == 0) return QUIC_OK;
+  QUIC_REQUIRE(t->q && t->k && t->v && t->out && t->tables && t->lengths && t->row_start, QUIC_E_ARG, "tree_attn: null tensor");
+  QUIC_REQUIRE(t->mask == nullptr || t->mask_words >= 1, QUIC_E_SHAPE, "tree_attn: a mask has at least one word a row");
+  QUIC_REQUIRE(((uintptr_t)t->q | (uintptr_t)t->k | (uintptr_t)t->v | (uintptr_t)t->out) % 16 == 0, QUIC_E_ARG,
+               "tree_attn: tensors must be 16-byte aligned");
+  QUIC_REQUIRE(((t->q_row | t->q_head | t->k_block | t->k_head | t->k_tok | t->v_block | t->v_head | t->v_tok) & 7) == 0, QUIC_E_ARG,
+               "tree_attn: strides must be multiples of 8 elements");
+  QUIC_REQUIRE((int64_t)t->rows * t->heads < (1ll << 31), QUIC_E_LIMIT, "tree_attn: rows times heads reach 2^31");
+  const int max_new = t->max_new < t->rows ? t->max_new : t->rows;
+  const int64_t room = (int64_t)t->max_blocks * t->block_size, max_len = t->max_len < room ? t->max_len : room;
+  TreeArgs a = {};
+  QUIC_REQUIRE(plan_of(t->requests, t->heads, t->kv_heads, t->dim, max_new, max_len, a.splits, a.chunk), QUIC_E_SHAPE,
+               "tree_attn: bad shape");
+  const int64_t tiles = (int64_t)t->kv_heads * (((int64_t)max_new * (t->heads / t->kv_heads) + 15) / 16);
+  QUIC_REQUIRE(t->requests <= 65535 && tiles <= 65535, QUIC_E_LIMIT, "tree_attn: more than 65535 requests, or 16-row tiles of one");
+  QUIC_REQUIRE(a.splits == 1 || (scratch != nullptr && (uintptr_t)scratch % 16 == 0), QUIC_E_ARG,
+               "tree_attn: scratch missing or not 16-byte aligned");
+  a.q = t->q, a.k = t->k, a.v = t->v, a.out = t->out;
+  a.q_row = t->q_row, a.q_head = t->q_head;
+  a.k_block = t->k_block, a.k_head = t->k_head, a.k_tok = t->k_tok;
+  a.v_block = t->v_block, a.v_head = t->v_head, a.v_tok = t->v_tok;
+  a.table_row = t->table_row, a.mask_row = t->mask_row;
+  a.tables = t->tables, a.lengths = t->lengths, a.row_start = t->row_start;
+  a.mask = (const uint32_t*)t->mask, a.mask_words = t->mask_words;
+  a.part_o = (float*)scratch;
+  a.part_ml = (float2*)(a.part_o + (int64_t)t->rows * t->heads * a.splits * t->dim);
+  a.block = FastDiv::of((uint32_t)t->block_size);
+  a.group = FastDiv::of((uint32_t)(t->heads / t->kv_heads));
+  a.rows = t->rows, a.requests = t->requests, a.heads = t->heads, a.kv_heads = t->kv_heads;
+  a.n_blocks = t->n_blocks, a.max_blocks = t->max_blocks, a.max_new = max_new;
+  a.scale_log2 = (t->scale > 0.f ? t->scale : 1.f / sqrtf((float)t->dim)) * 1.4426950408889634f;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (t->dtype == QUIC_DTYPE_F16)
+    return t->dim == 64 ? launch_typed<half, 64>(a, st) : launch_typed<half, 128>(a, st);
+  return t->dim == 64 ? launch_typed<__nv_bfloat16, 64>(a, st) : launch_typed<__nv_bfloat16, 128>(a, st);
+}

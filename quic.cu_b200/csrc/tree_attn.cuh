@@ -1,0 +1,130 @@
+// What the two kernels of the tree attention and their merge share: the call's
+// arguments, the place of a position in the blocks, a request's part of the batch and its split into CTAs.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace quic {
+
+// Division of 0 .. 2^31 - 1 by a divisor that the host knows (Granlund and Montgomery 1994): a multiplication and a shift.
+struct FastDiv {
+  uint32_t d, magic, shift;
+  __host__ static FastDiv of(uint32_t d) {
+    uint32_t l = 0;
+    while ((1ull << l) < d) ++l;
+    return {d, (uint32_t)((((1ull << l) - d) << 32) / d + 1), l};
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, magic) + n) >> shift; }
+};
+
+struct TreeArgs {
+  const void* q;                     // [rows][heads][dim] by strides, in elements
+  const void *k, *v;                 // [n_blocks][kv heads][block][dim] by strides, in elements
+  void* out;                         // [rows][heads][dim]
+  int64_t q_row, q_head, k_block, k_head, k_tok, v_block, v_head, v_tok, table_row, mask_row;
+  const int32_t *tables, *lengths, *row_start;
+  const uint32_t* mask;              // [rows][mask_words] by mask_row, or nullptr: node i sees nodes 0 .. i
+  float* part_o;                     // [rows][heads][splits][dim]
+  float2* part_ml;                   // [rows][heads][splits]: maximum (base 2), sum
+  FastDiv block, group;              // tokens per block, query heads per KV head
+  int32_t rows, requests, heads, kv_heads, n_blocks, max_blocks, mask_words, max_new;
+  int32_t splits, chunk;             // CTAs per request, KV head and row tile at most; the tokens of one
+  float scale_log2;
+};
+
+// A request's rows [start, start + n), its cached tokens before them and the end of its keys, all within the tensors
+// whatever the tables hold.
+struct TreeRequest {
+  int start, n, len, end;
+};
+__device__ __forceinline__ TreeRequest tree_request(const TreeArgs& a, int b) {
+  TreeRequest r;
+  const int s = a.row_start[b], e = a.row_start[b + 1];
+  r.start = min(max(s, 0), a.rows);
+  r.n = max(min(e, a.rows) - r.start, 0);
+  const int64_t room = (int64_t)a.max_blocks * a.block.d;
+  r.len = (int)min((int64_t)max(a.lengths[b], 0), room);
+  r.end = (int)min((int64_t)r.len + r.n, room);
+  return r;
+}
+// How many CTAs share a request's keys, and the keys of each: equal parts, whole tiles of 64.
+__device__ __forceinline__ int tree_parts(const TreeArgs& a, int end, int& per) {
+  const int parts = max(1, min(a.splits, (end + a.chunk - 1) / a.chunk));
+  per = ((end + parts - 1) / parts + 63) & ~63;
+  return per > 0 ? (end + per - 1) / per : 1;
+}
+
+// Which of the 32 positions from t on node `node` sees, the positions up to `end` taken for present: bit j for t + j.
+__device__ __forceinline__ uint32_t tree_visible32(const TreeArgs& a, const TreeRequest& r, int node, int t) {
+  const int first = t - r.len;  // number of the node at position t
+  if (first + 32 <= 0) return 0xffffffffu;
+  uint32_t seen;
+  if (a.mask == nullptr) {
+    const int last = node - first;  // the last bit
+    seen = last >= 31 ? 0xffffffffu : (last < 0 ? 0u : (2u << last) - 1u);
+    return first < 0 ? seen | ((1u << -first) - 1u) : seen;
+  }
+  const uint32_t* row = a.mask + (int64_t)(r.start + node) * a.mask_row;
+  const int w = first >> 5;  // (rounds down)
+  const uint32_t lo = w < 0 ? 0xffffffffu : (w < a.mask_words ? row[w] : 0u);
+  const uint32_t hi = w + 1 < a.mask_words ? row[w + 1] : 0u;
+  return __funnelshift_r(lo, hi, first & 31);
+}
+
+__device__ __forceinline__ float tree_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two values in a word of the tensors' type.
+template <typename T>
+__device__ __forceinline__ uint32_t tree_pack(float x, float y);
+template <>
+__device__ __forceinline__ uint32_t tree_pack<half>(float x, float y) {
+  const half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t tree_pack<__nv_bfloat16>(float x, float y) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 tree_unpack(uint32_t w);
+template <>
+__device__ __forceinline__ float2 tree_unpack<half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 tree_unpack<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+// The exponent of an infinity or NaN, and whether one of the two values in a word has it.
+template <typename T>
+constexpr uint32_t kTreeExponent = 0;
+template <>
+constexpr uint32_t kTreeExponent<half> = 0x7c00u;
+template <>
+constexpr uint32_t kTreeExponent<__nv_bfloat16> = 0x7f80u;
+template <typename T>
+__device__ __forceinline__ bool tree_not_finite(uint32_t w) {
+  constexpr uint32_t e = kTreeExponent<T>;
+  return (w & e) == e || ((w >> 16) & e) == e;
+}
+// The word with what is not finite replaced by zero.
+template <typename T>
+__device__ __forceinline__ uint32_t tree_finite(uint32_t w) {
+  constexpr uint32_t e = kTreeExponent<T>;
+  if ((w & e) == e) w &= 0xffff0000u;
+  if (((w >> 16) & e) == e) w &= 0x0000ffffu;
+  return w;
+}
+
+// fp16 weights are P = 2^(score - maximum + 8): probabilities down to 2^-22 stay normal.  bf16 has fp32's range.
+template <typename T>
+constexpr float kTreeShift = 0.f;
+template <>
+constexpr float kTreeShift<half> = 8.f;
+
+}  // namespace quic

@@ -12,9 +12,11 @@ tensors raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import functools
 import os
+import struct
 import threading
 from types import SimpleNamespace
 
@@ -179,6 +181,11 @@ SIGNATURES = {
     "quic_decode_persist": (C.c_int, [C.POINTER(Model), C.POINTER(Decode), _P, _P, _I32, _P]),
     "quic_decode_persist_watch": (C.c_int, [C.POINTER(Model), C.POINTER(Decode), _P, _P, _I32, _P, _P]),
     "quic_decode_persist_status": (C.c_int, [_P, _P, C.POINTER(_I32)]),
+    "quic_tree_attn": (C.c_int, [_P, _P, _P]),
+    "quic_tree_attn_scratch_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32, _I64]),
+    "quic_block_tables": (C.c_int, [_P, _I64, _I32, _P, _P, _I32, _P, _P, _I32, _I32, _P, _P, _P, _P, _P, _I32, _I32, _P]),
+    "quic_tree_commit": (C.c_int, [_P, _P]),
+    "quic_qkv_rope_append_at": (C.c_int, [_P, _P, _P, _P, _P, _I32, _P, _P, _P, _I32, _I32, _I32, _P]),
     "quic_decode_persist_run_host": (C.c_int, [C.POINTER(Model), C.POINTER(Decode), _P, _P, _I32, _P, _P, _P, _I32,
                                                _P, _P, _I32, _P]),
 }
@@ -499,6 +506,33 @@ def qkv_rope_append(qkv: torch.Tensor, slots: torch.Tensor, positions: torch.Ten
     return q
 
 
+def qkv_rope_append_at(qkv: torch.Tensor, slot_map: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor,
+                       sin: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor) -> torch.Tensor:
+    """``qkv_rope_append`` of rows whose place in the cache is not their position (drafted trees, blocked caches):
+    ``positions`` int32 [rows] turn the rows, ``slot_map`` int64 [rows] (of ``block_tables``) says where they go in
+    planes [n_blocks, 2, block size, 64]; rows with an entry outside them append nothing."""
+    _need_cuda(qkv, slot_map, positions, cos, sin, kcache, vcache)
+    _need_half(qkv, cos, sin, kcache, vcache)
+    rows = qkv.shape[0]
+    if qkv.dim() != 2 or qkv.shape[1] != QKV_N or slot_map.shape != (rows,) or positions.shape != (rows,):
+        raise RuntimeError("qkv_rope_append_at: qkv must be [rows, 1152] with one place and position per row")
+    if slot_map.dtype != torch.int64 or positions.dtype != torch.int32:
+        raise RuntimeError("qkv_rope_append_at: slot_map must be int64 and positions int32")
+    if kcache.dim() != 4 or vcache.shape != kcache.shape or kcache.shape[1] != KV_HEADS or kcache.shape[3] != HEAD_DIM or \
+            not (kcache.is_contiguous() and vcache.is_contiguous()):
+        raise RuntimeError("qkv_rope_append_at: cache planes must be contiguous [n_blocks, 2, block size, 64] of equal shape")
+    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != 32 or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise RuntimeError("qkv_rope_append_at: cos/sin must be contiguous [positions, 32] of equal shape")
+    device = _same_device(qkv, slot_map, positions, cos, sin, kcache, vcache)
+    qkv, slot_map, positions = qkv.contiguous(), slot_map.contiguous(), positions.contiguous()
+    q = torch.empty(HEADS, rows, HEAD_DIM, dtype=torch.float16, device=qkv.device)
+    with _on(device):
+        check(lib().quic_qkv_rope_append_at(ptr(qkv), ptr(slot_map), ptr(positions), ptr(cos), ptr(sin), cos.shape[0], ptr(q),
+                                            ptr(kcache), ptr(vcache), kcache.shape[2], kcache.shape[0], rows, _raw_stream(device)),
+              "qkv_rope_append_at")
+    return q
+
+
 def attn_prefill(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, seq_start: torch.Tensor,
                  seq_len: torch.Tensor, seq_slot: torch.Tensor, max_len: int, scale: float = -1.0,
                  seq_off: torch.Tensor | None = None) -> torch.Tensor:
@@ -678,6 +712,216 @@ def _flash_attn_decode_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
     if rc != 0:
         check(rc, "attn_decode")
     return out
+
+
+# ---------------------------------------------------------------------------------
+# Several tokens per forward: trees of drafted tokens over blocks of KV memory
+# ---------------------------------------------------------------------------------
+_stay = contextlib.nullcontext()
+
+
+def _on(device: int):
+    """Makes ``device`` current for a launch on one of its streams."""
+    return _stay if torch.cuda.current_device() == device else torch.cuda.device(device)
+
+
+def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    device = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            raise RuntimeError("quic_b200: CUDA tensors of one device required (no CPU path)")
+    if device < 0:
+        raise RuntimeError("quic_b200: CUDA tensors required (no CPU path)")
+    return device
+
+
+_TREE_TYPES = {torch.float16: 0, torch.bfloat16: 1}
+_TREE_ATTN = struct.Struct("=4Q8qQqQQQq11i4xqf4x")  # quic_tree_attn_t
+_TREE_COMMIT = struct.Struct("=Q5qQq5Q10i4Q")       # quic_tree_commit_t
+
+
+@functools.lru_cache(maxsize=4096)
+def _tree_scratch_bytes(rows: int, requests: int, heads: int, kv_heads: int, dim: int, max_new: int, max_len: int) -> int:
+    return lib().quic_tree_attn_scratch_bytes(rows, requests, heads, kv_heads, dim, max_new, max_len)
+
+
+def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor,
+              row_start: torch.Tensor, mask: torch.Tensor | None = None, softmax_scale: float = -1.0,
+              max_new: int | None = None, max_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted trees (chains, prompt chunks, single tokens) over a blocked or slotted KV cache.
+
+    ``q`` [rows, heads, dim], fp16 or bf16, dim 64 or 128; request b has rows row_start[b] .. row_start[b + 1] - 1, one per
+    node of its tree.  ``kcache`` / ``vcache`` [blocks, KV heads, block size, dim], of any strides that are multiples of 8;
+    position p of request b lies in block tables[b, p // block size]; the request's ``lengths`` [b] cached tokens come first,
+    node i's K and V at position lengths[b] + i.  ``mask`` int32 [rows, words] (``block_tables``): bit j of a row says
+    whether it sees node j of its request; without it row i sees nodes 0 .. i.  Everybody sees the cached tokens.
+
+    ``max_new`` bounds the rows of one request (None: all rows; rows beyond stay unwritten), ``max_len`` the lengths
+    (None: what the tables hold); both only plan the launch, tight bounds make it faster.  Returns [rows, heads, dim]
+    (``out`` if given, contiguous; rows outside row_start[0] .. row_start[-1] - 1 stay as they were): rows that see nothing
+    are zero."""
+    dtype = _TREE_TYPES.get(q.dtype)
+    if dtype is None or kcache.dtype != q.dtype or vcache.dtype != q.dtype:
+        raise RuntimeError("tree_attn: q, kcache and vcache must be of one type, fp16 or bf16")
+    if q.dim() != 3 or kcache.dim() != 4 or kcache.shape != vcache.shape:
+        raise RuntimeError("tree_attn: expected q [rows, heads, dim] and planes [blocks, KV heads, block size, dim]")
+    rows, heads, dim = q.shape
+    blocks, kv_heads, block, kv_dim = kcache.shape
+    if dim not in (64, 128) or kv_dim != dim or kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise RuntimeError("tree_attn: the head dimension is 64 or 128, the query heads a multiple of the KV heads")
+    if tables.dim() != 2 or lengths.dim() != 1 or row_start.dim() != 1:
+        raise RuntimeError("tree_attn: expected tables [requests, blocks], lengths [requests], row_start [requests + 1]")
+    requests, width = tables.shape
+    if lengths.shape[0] != requests or row_start.shape[0] != requests + 1:
+        raise RuntimeError("tree_attn: expected tables [requests, blocks], lengths [requests], row_start [requests + 1]")
+    if not (tables.dtype is lengths.dtype is row_start.dtype is torch.int32) or (mask is not None and mask.dtype is not torch.int32):
+        raise RuntimeError("tree_attn: tables, lengths, row_start and mask must be int32")
+    qs, ks, vs, ts = q.stride(), kcache.stride(), vcache.stride(), tables.stride()
+    if (qs[2] != 1 or ks[3] != 1 or vs[3] != 1 or (ts[1] != 1 and width > 1) or not lengths.is_contiguous() or
+            not row_start.is_contiguous()):
+        raise RuntimeError("tree_attn: the last dimension of every tensor must be contiguous")
+    words = mask_row = mask_ptr = 0
+    if mask is not None:
+        if mask.dim() != 2 or mask.shape[0] != rows or mask.shape[1] < 1 or (mask.stride(1) != 1 and mask.shape[1] > 1):
+            raise RuntimeError("tree_attn: mask must be [rows, words], its words contiguous")
+        words, mask_row, mask_ptr = mask.shape[1], mask.stride(0), mask.data_ptr()
+    device = _same_device(q, kcache, vcache, tables, lengths, row_start, mask, out)
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise RuntimeError("tree_attn: out must be contiguous [rows, heads, dim] of q's type")
+    if rows == 0 or requests == 0:
+        return out
+    if width < 1 or blocks < 1 or block < 1:
+        raise RuntimeError("tree_attn: no blocks")
+    max_new = rows if max_new is None else min(max_new, rows)
+    max_len = width * block if max_len is None else min(max_len, width * block)
+    if max_new < 1 or max_len < 0:
+        raise RuntimeError("tree_attn: max_new must be positive and max_len not negative")
+    need = _tree_scratch_bytes(rows, requests, heads, kv_heads, dim, max_new, max_len)
+    stream = _raw_stream(device)
+    scratch = _thread_scratch(("tree", device, stream), need, 1 << 20, 0).data_ptr() if need > 0 else None
+    call = _TREE_ATTN.pack(q.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), out.data_ptr(), qs[0], qs[1], ks[0], ks[1], ks[2],
+                           vs[0], vs[1], vs[2], tables.data_ptr(), ts[0], lengths.data_ptr(), row_start.data_ptr(), mask_ptr,
+                           mask_row, words, rows, requests, heads, kv_heads, dim, blocks, block, width, dtype, max_new,
+                           max_len, softmax_scale)
+    with _on(device):
+        rc = lib().quic_tree_attn(call, scratch, stream)
+    if rc != 0:
+        check(rc, "tree_attn")
+    return out
+
+
+def block_pool(n_blocks: int, device, block_ids: torch.Tensor | None = None) -> torch.Tensor:
+    """A pool for ``block_tables`` in which the blocks 0 .. n_blocks - 1 (or only ``block_ids``, in their order) are free:
+    int32 [4 + n_blocks] = head, count, 0, status of the last call, ring of block ids."""
+    pool = torch.zeros(4 + n_blocks, dtype=torch.int32, device=device)
+    ids = torch.arange(n_blocks, dtype=torch.int32, device=device) if block_ids is None else block_ids
+    if ids.numel() > n_blocks:
+        raise RuntimeError("block_pool: more free blocks than blocks")
+    pool[1] = ids.numel()
+    pool[4:4 + ids.numel()] = ids
+    return pool
+
+
+def block_tables(tables: torch.Tensor, held: torch.Tensor, pool: torch.Tensor, lengths: torch.Tensor, n_new: torch.Tensor,
+                 block_size: int, max_rows: int, parents: torch.Tensor | None = None, max_new: int | None = None):
+    """The tables of a step, built on the device from the requests' ``lengths`` (cached tokens) and ``n_new`` (rows to come;
+    0: none, < 0: the request has ended).  All int32: ``tables`` [requests, blocks], ``held`` [requests] (blocks of each
+    request, the first entries of its table row) and ``pool`` (``block_pool``) are updated in place: requests get the blocks
+    that their rows need from the pool, ended ones give theirs back.  Returns
+
+    * ``row_start`` int32 [requests + 1], where each request's rows begin;
+    * ``slot_map`` int64 [max_rows], block * block_size + offset per row, -1 behind the last;
+    * ``positions`` int32 [max_rows], lengths + the depth of the row's node (without ``parents``: its number);
+    * ``mask`` int32 [max_rows, words] with ``parents`` (int32 [max_rows], an earlier node of the request's tree or -1):
+      bits of the node's ancestors and itself; words is enough for ``max_new`` (None: max_rows) nodes.  Else None.
+
+    All or nothing: pool[3] is 0, or the number of blocks that the pool lacks, or -1 (a request needs more blocks than
+    its table row has) or -2 (more rows than max_rows, or than the mask has bits): then no request gets rows or blocks and row_start is all zero, which
+    the operators that read it take for no work.  A pool belongs to one stream at a time."""
+    if any(t.dtype is not torch.int32 for t in (tables, held, pool, lengths, n_new)) or (parents is not None and parents.dtype is not torch.int32):
+        raise RuntimeError("block_tables: tables, held, pool, lengths, n_new and parents must be int32")
+    if tables.dim() != 2 or tables.shape[1] < 1 or (tables.stride(1) != 1 and tables.shape[1] > 1) or \
+            (tables.shape[0] > 1 and tables.stride(0) < tables.shape[1]):
+        raise RuntimeError("block_tables: tables must be [requests, blocks], rows contiguous")
+    requests, width = tables.shape
+    if any(t.shape != (requests,) or not t.is_contiguous() for t in (held, lengths, n_new)):
+        raise RuntimeError("block_tables: held, lengths and n_new must be contiguous [requests]")
+    if pool.dim() != 1 or pool.shape[0] < 4 or not pool.is_contiguous():
+        raise RuntimeError("block_tables: pool must be contiguous [4 + blocks]")
+    if max_rows < 0 or (parents is not None and (parents.shape != (max_rows,) or not parents.is_contiguous())):
+        raise RuntimeError("block_tables: max_rows must not be negative, parents contiguous [max_rows]")
+    device = _same_device(tables, held, pool, lengths, n_new, parents)
+    where = tables.device
+    words = 0
+    if parents is not None:
+        words = -(-(max_rows if max_new is None else max_new) // 32) or 1
+        if words < 1:
+            raise RuntimeError("block_tables: max_new must not be negative")
+    # one allocation, the parts at multiples of 8 bytes
+    cut = (requests + 2) // 2 * 2
+    room = torch.empty(2 * max_rows + cut + (max_rows + 1) // 2 * 2 + max_rows * words, dtype=torch.int32, device=where)
+    slot_map = room[:2 * max_rows].view(torch.int64)
+    row_start = room[2 * max_rows:2 * max_rows + requests + 1]
+    at = 2 * max_rows + cut
+    positions = room[at:at + max_rows]
+    at += (max_rows + 1) // 2 * 2
+    mask = room[at:].view(max_rows, words) if parents is not None else None
+    with _on(device):
+        rc = lib().quic_block_tables(tables.data_ptr(), tables.stride(0), width, held.data_ptr(), pool.data_ptr(), pool.shape[0] - 4,
+                                     lengths.data_ptr(), n_new.data_ptr(), requests, block_size, ptr(parents),
+                                     row_start.data_ptr(), slot_map.data_ptr(), positions.data_ptr(), ptr(mask), words, max_rows,
+                                     _raw_stream(device))
+    if rc != 0:
+        check(rc, "block_tables")
+    return row_start, slot_map, positions, mask
+
+
+def tree_commit(kv: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, row_start: torch.Tensor, parents: torch.Tensor,
+                tokens: torch.Tensor, targets: torch.Tensor, max_new: int):
+    """Keeps the branch of each drafted tree that the target model agrees with.  ``tokens`` [rows] are the nodes' tokens and
+    ``targets`` [rows] what the target chose after each, both int32 or both int64; node 0 of a request is right by definition
+    and of an accepted node's children the first whose token is the target's choice.  The accepted nodes' K and V move, in
+    ``kv`` [layers, 2, blocks, KV heads, block size, dim] (2-byte elements), to the positions behind the request's ``lengths``
+    [b] cached tokens.  Returns (path int32 [requests, max_new], the accepted nodes and -1 behind them; accepted int32
+    [requests]; next_token [requests], the target's choice after the last of them, -1 for a request without rows; new_lengths
+    int32 [requests]).  Requests with more than ``max_new`` (at most 1024) rows are left alone."""
+    if kv.dim() != 6 or kv.shape[1] != 2 or kv.element_size() != 2:
+        raise RuntimeError("tree_commit: kv must be [layers, 2, blocks, KV heads, block size, dim] of a 2-byte type")
+    if tables.dim() != 2 or lengths.dim() != 1 or row_start.dim() != 1 or tokens.dim() != 1:
+        raise RuntimeError("tree_commit: expected tables [requests, blocks], lengths [requests], row_start [requests + 1], tokens [rows]")
+    requests, width = tables.shape
+    rows = tokens.shape[0]
+    if lengths.shape[0] != requests or row_start.shape[0] != requests + 1 or targets.shape != (rows,) or parents.shape != (rows,):
+        raise RuntimeError("tree_commit: tables, lengths and row_start, or parents, tokens and targets do not match")
+    if not (tables.dtype is lengths.dtype is row_start.dtype is parents.dtype is torch.int32):
+        raise RuntimeError("tree_commit: tables, lengths, row_start and parents must be int32")
+    if tokens.dtype is not targets.dtype or tokens.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError("tree_commit: tokens and targets must both be int32 or both int64")
+    s = kv.stride()
+    if s[5] != 1 or (tables.stride(1) != 1 and width > 1) or not (lengths.is_contiguous() and row_start.is_contiguous() and
+                                                                 parents.is_contiguous() and tokens.is_contiguous() and
+                                                                 targets.is_contiguous()):
+        raise RuntimeError("tree_commit: the last dimension of every tensor must be contiguous")
+    if kv.numel() == 0 or width < 1:
+        raise RuntimeError("tree_commit: no blocks")
+    device = _same_device(kv, tables, lengths, row_start, parents, tokens, targets)
+    wide = 2 if tokens.dtype is torch.int64 else 1
+    # one allocation: next_token first, where it is aligned
+    room = torch.empty(requests * (wide + 2 + max(max_new, 0)), dtype=torch.int32, device=kv.device)
+    next_token = room[:wide * requests].view(tokens.dtype)
+    accepted, new_lengths = room[wide * requests:(wide + 1) * requests], room[(wide + 1) * requests:(wide + 2) * requests]
+    path = room[(wide + 2) * requests:].view(requests, max(max_new, 0))
+    call = _TREE_COMMIT.pack(kv.data_ptr(), s[0], s[1], s[2], s[3], s[4], tables.data_ptr(), tables.stride(0), lengths.data_ptr(),
+                             row_start.data_ptr(), parents.data_ptr(), tokens.data_ptr(), targets.data_ptr(), 4 * wide, kv.shape[0],
+                             kv.shape[2], kv.shape[3], kv.shape[4], kv.shape[5], width, rows, requests, max_new,
+                             path.data_ptr(), accepted.data_ptr(), next_token.data_ptr(), new_lengths.data_ptr())
+    with _on(device):
+        rc = lib().quic_tree_commit(call, _raw_stream(device))
+    if rc != 0:
+        check(rc, "tree_commit")
+    return path, accepted, next_token, new_lengths
 
 
 @functools.cache
