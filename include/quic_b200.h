@@ -370,18 +370,19 @@ int64_t quic_tree_attn_scratch_bytes(int32_t rows, int32_t requests,
  *     (parents NULL: its number), 0 behind the last one;
  *   mask int32 [max_rows, mask_words] (with parents), the node's ancestors and
  *     itself, 0 behind the last one.
- * parents int32 [max_rows] or NULL; an entry that is no earlier node counts as
- * -1.  All or nothing: where the pool lacks blocks (status: how many), a request
- * needs more than max_blocks (status -1), or there are more rows than max_rows or,
- * with parents, than 32 * mask_words in a request (status -2), no request gets
- * rows or blocks: row_start is all 0.  Ended requests give theirs back all the
+ * parents int32 [parent_rows] or NULL, one per row; an entry that is no earlier
+ * node counts as -1.  All or nothing: where the pool lacks blocks (status: how
+ * many), a request needs more than max_blocks (status -1), or there are more rows
+ * than max_rows or, with parents, than parent_rows or 32 * mask_words in a request
+ * (status -2), no request gets rows or blocks: row_start is all 0.  Ended requests give theirs back all the
  * same.  Status 0: done.  A pool serves one stream at a time.  At most 4096
  * requests and 65535 * 256 rows.  Positions reach 2^29 at most. */
 int quic_block_tables(int32_t *tables, int64_t table_row, int32_t max_blocks,
                       int32_t *held, int32_t *pool, int32_t n_blocks,
                       const int32_t *lengths, const int32_t *n_new,
                       int32_t requests, int32_t block_size,
-                      const int32_t *parents, int32_t *row_start,
+                      const int32_t *parents, int32_t parent_rows,
+                      int32_t *row_start,
                       int64_t *slot_map, int32_t *positions, int32_t *mask,
                       int32_t mask_words, int32_t max_rows, void *stream);
 

@@ -22,7 +22,7 @@ struct TablesArgs {
   int64_t* slot_map;
   const int32_t *lengths, *n_new, *parents;
   int64_t table_row;
-  int32_t max_blocks, n_blocks, requests, block_size, mask_words, max_rows;
+  int32_t max_blocks, n_blocks, requests, block_size, mask_words, max_rows, most_rows;
 };
 
 __device__ __forceinline__ uint32_t warp_exclusive(uint32_t v, uint32_t& total, int lane) {
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kThreads) block_tables_kernel(const TablesArgs
   const int count = min(max(a.pool[1], 0), n_ring), head = n_ring > 0 ? (int)((uint32_t)a.pool[0] % (uint32_t)n_ring) : 0;
   int status = 0;
   if (short_s) status = -1;
-  else if (many_s || rows_s > (unsigned long long)a.max_rows) status = -2;
+  else if (many_s || rows_s > (unsigned long long)a.most_rows) status = -2;
   else if (need_s > (unsigned long long)count) status = (int)min(need_s - count, 0x7fffffffull);
   const bool fine = status == 0;
 #pragma unroll
@@ -195,17 +195,18 @@ using namespace quic;
 
 extern "C" int quic_block_tables(int32_t* tables, int64_t table_row, int32_t max_blocks, int32_t* held, int32_t* pool,
                                  int32_t n_blocks, const int32_t* lengths, const int32_t* n_new, int32_t requests,
-                                 int32_t block_size, const int32_t* parents, int32_t* row_start, int64_t* slot_map,
+                                 int32_t block_size, const int32_t* parents, int32_t parent_rows, int32_t* row_start, int64_t* slot_map,
                                  int32_t* positions, int32_t* mask, int32_t mask_words, int32_t max_rows, void* stream) {
   QUIC_REQUIRE(tables && held && pool && lengths && n_new && row_start, QUIC_E_ARG, "block_tables: null tensor");
   QUIC_REQUIRE(max_rows >= 0 && (max_rows == 0 || (slot_map && positions)), QUIC_E_ARG, "block_tables: null tensor");
-  QUIC_REQUIRE(parents == nullptr || (mask_words >= 1 && (mask || max_rows == 0)), QUIC_E_ARG, "block_tables: parents without a mask");
+  QUIC_REQUIRE(parents == nullptr || (mask_words >= 1 && parent_rows >= 0 && (mask || max_rows == 0)), QUIC_E_ARG, "block_tables: parents without a mask");
   QUIC_REQUIRE(requests >= 1 && max_blocks >= 1 && n_blocks >= 0 && block_size >= 1 && n_blocks < (1 << 30) &&
                    (int64_t)max_blocks * block_size <= kMostPositions,
                QUIC_E_SHAPE, "block_tables: bad request count or block geometry");
   QUIC_REQUIRE(requests <= kMostRequests && max_rows <= 65535 * 256, QUIC_E_LIMIT, "block_tables: more than 4096 requests, or too many rows");
   TablesArgs a = {tables, held, pool, row_start, positions, mask, slot_map, lengths, n_new, parents, table_row,
-                  max_blocks, n_blocks, requests, block_size, mask_words, max_rows};
+                  max_blocks, n_blocks, requests, block_size, mask_words, max_rows,
+                  parents != nullptr && parent_rows < max_rows ? parent_rows : max_rows};
   const int64_t work = (int64_t)max_rows * (parents != nullptr ? mask_words : 1);
   int64_t ctas = (work + 4 * kThreads - 1) / (4 * kThreads);
   ctas = ctas < 1 ? 1 : (ctas > 148 * 4 ? 148 * 4 : ctas);

@@ -183,7 +183,7 @@ SIGNATURES = {
     "quic_decode_persist_status": (C.c_int, [_P, _P, C.POINTER(_I32)]),
     "quic_tree_attn": (C.c_int, [_P, _P, _P]),
     "quic_tree_attn_scratch_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32, _I64]),
-    "quic_block_tables": (C.c_int, [_P, _I64, _I32, _P, _P, _I32, _P, _P, _I32, _I32, _P, _P, _P, _P, _P, _I32, _I32, _P]),
+    "quic_block_tables": (C.c_int, [_P, _I64, _I32, _P, _P, _I32, _P, _P, _I32, _I32, _P, _I32, _P, _P, _P, _P, _I32, _I32, _P]),
     "quic_tree_commit": (C.c_int, [_P, _P]),
     "quic_qkv_rope_append_at": (C.c_int, [_P, _P, _P, _P, _P, _I32, _P, _P, _P, _I32, _I32, _I32, _P]),
     "quic_decode_persist_run_host": (C.c_int, [C.POINTER(Model), C.POINTER(Decode), _P, _P, _I32, _P, _P, _P, _I32,
@@ -834,12 +834,12 @@ def block_tables(tables: torch.Tensor, held: torch.Tensor, pool: torch.Tensor, l
     * ``row_start`` int32 [requests + 1], where each request's rows begin;
     * ``slot_map`` int64 [max_rows], block * block_size + offset per row, -1 behind the last;
     * ``positions`` int32 [max_rows], lengths + the depth of the row's node (without ``parents``: its number);
-    * ``mask`` int32 [max_rows, words] with ``parents`` (int32 [max_rows], an earlier node of the request's tree or -1):
+    * ``mask`` int32 [max_rows, words] with ``parents`` (int32, one per row: an earlier node of the request's tree or -1):
       bits of the node's ancestors and itself; words is enough for ``max_new`` (None: max_rows) nodes.  Else None.
 
     All or nothing: pool[3] is 0, or the number of blocks that the pool lacks, or -1 (a request needs more blocks than
-    its table row has) or -2 (more rows than max_rows, or than the mask has bits): then no request gets rows or blocks and row_start is all zero, which
-    the operators that read it take for no work.  A pool belongs to one stream at a time."""
+    its table row has) or -2 (more rows than max_rows or parents, or than the mask has bits): then no request gets rows or
+    blocks and row_start is all zero, which the operators that read it take for no work.  A pool belongs to one stream at a time."""
     if any(t.dtype is not torch.int32 for t in (tables, held, pool, lengths, n_new)) or (parents is not None and parents.dtype is not torch.int32):
         raise RuntimeError("block_tables: tables, held, pool, lengths, n_new and parents must be int32")
     if tables.dim() != 2 or tables.shape[1] < 1 or (tables.stride(1) != 1 and tables.shape[1] > 1) or \
@@ -850,8 +850,8 @@ def block_tables(tables: torch.Tensor, held: torch.Tensor, pool: torch.Tensor, l
         raise RuntimeError("block_tables: held, lengths and n_new must be contiguous [requests]")
     if pool.dim() != 1 or pool.shape[0] < 4 or not pool.is_contiguous():
         raise RuntimeError("block_tables: pool must be contiguous [4 + blocks]")
-    if max_rows < 0 or (parents is not None and (parents.shape != (max_rows,) or not parents.is_contiguous())):
-        raise RuntimeError("block_tables: max_rows must not be negative, parents contiguous [max_rows]")
+    if max_rows < 0 or (parents is not None and (parents.dim() != 1 or not parents.is_contiguous())):
+        raise RuntimeError("block_tables: max_rows must not be negative, parents contiguous [rows]")
     device = _same_device(tables, held, pool, lengths, n_new, parents)
     where = tables.device
     words = 0
@@ -871,6 +871,7 @@ def block_tables(tables: torch.Tensor, held: torch.Tensor, pool: torch.Tensor, l
     with _on(device):
         rc = lib().quic_block_tables(tables.data_ptr(), tables.stride(0), width, held.data_ptr(), pool.data_ptr(), pool.shape[0] - 4,
                                      lengths.data_ptr(), n_new.data_ptr(), requests, block_size, ptr(parents),
+                                     0 if parents is None else parents.shape[0],
                                      row_start.data_ptr(), slot_map.data_ptr(), positions.data_ptr(), ptr(mask), words, max_rows,
                                      _raw_stream(device))
     if rc != 0:

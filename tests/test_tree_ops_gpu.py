@@ -350,7 +350,7 @@ class Pool:
         status = 0
         if any(n and w > self.width for n, w in zip(take, want)):
             status = -1
-        elif sum(take) > max_rows or (parents is not None and any(n > 32 * words for n in take)):
+        elif sum(take) > max_rows or (parents is not None and (sum(take) > len(parents) or any(n > 32 * words for n in take))):
             status = -2
         elif sum(need) > len(self.free):
             status = sum(need) - len(self.free)
@@ -403,7 +403,7 @@ def test_tables_over_many_steps(requests, block, n_blocks, most, tree):
         max_rows = max(max_rows, 0)
         parents = None
         if tree:
-            parents = [int(x) for x in torch.randint(-1, most, (max_rows,), generator=g)]
+            parents = [int(x) for x in torch.randint(-1, most, (max(max_rows - 3 * (step % 3), 0),), generator=g)]
         i32 = functools.partial(torch.tensor, dtype=torch.int32, device="cuda")
         got = K.block_tables(tables, held, pool, i32(lengths), i32(new), block, max_rows,
                              parents=None if parents is None else i32(parents), max_new=most)

@@ -54,7 +54,7 @@ def _tables(**more):
     ({}, "CUDA tensors"),
     (dict(held=torch.zeros(2).long()), "int32"),
     (dict(parents=torch.zeros(4).long()), "int32"),
-    (dict(parents=torch.zeros(3, **I32)), "parents"),
+    (dict(parents=torch.zeros(3, 1, **I32)), "parents"),
     (dict(tables=torch.zeros(2, 0, **I32)), "tables must be"),
     (dict(tables=torch.zeros(3, **I32)), "tables must be"),
     (dict(tables=torch.zeros(3, **I32).expand(2, 3)), "tables must be"),
@@ -152,7 +152,7 @@ def test_commit_entry_point_refuses():
 def test_tables_entry_point_refuses():
     def call(requests=2, block=16, max_rows=4, n_blocks=5, max_blocks=3, parents=None, words=0, tables=4096):
         p = C.c_void_p(4096)
-        return K.lib().quic_block_tables(tables, 3, max_blocks, p, p, n_blocks, p, p, requests, block, parents, p, p, p, None, words,
+        return K.lib().quic_block_tables(tables, 3, max_blocks, p, p, n_blocks, p, p, requests, block, parents, 4, p, p, p, None, words,
                                          max_rows, None)
     assert call(tables=None) == -1 and call(parents=4096) == -1 and call(parents=4096, words=1) == -1
     assert call(requests=0) == -2 and call(block=0) == -2 and call(max_blocks=0) == -2 and call(n_blocks=-1) == -2
