@@ -7,7 +7,8 @@
 // chunk of a prompt and a single decode token are trees too.  The R = nodes x (query heads per KV head) rows of a
 // request and KV head share their keys; K and V are read once per tile of those rows.
 //
-// This file: the form for few rows (mma.sync), which takes every call, the merge of a request's parts, and the entry point.
+// This file: the form for few rows (mma.sync), the merge of a request's parts, and the entry point; tree_attn_tc.cu has the form
+// for more rows.
 // A CTA has 16 or 32 rows and a part of the keys, which its four warps walk 32 at a time, each through a ring of its own
 // (cp.async, no barrier between warps), one pass with a running maximum and sum per row; the warps' results meet in
 // shared memory at the end, those of several CTAs in the merge kernel.  Bound: the bytes of K and V.
@@ -396,9 +397,15 @@ int launch_few(const TreeArgs& a, cudaStream_t st) {
                    false, a));
   return QUIC_OK;
 }
+// Rows of a request and KV head beyond which the tcgen05 form takes a call.
+constexpr int64_t kFewRows = 32;
+
 template <typename T, int D>
 int launch_typed(const TreeArgs& a, cudaStream_t st) {
-  const int rc = (int64_t)a.max_new * a.group.d <= 16 ? launch_few<T, D, 1>(a, st) : launch_few<T, D, 2>(a, st);
+  const int64_t rows = (int64_t)a.max_new * a.group.d;
+  const int rc = rows <= 16         ? launch_few<T, D, 1>(a, st)
+                 : rows <= kFewRows ? launch_few<T, D, 2>(a, st)
+                                    : tree_attn_tc_launch(a, kTreeExponent<T> == kTreeExponent<__nv_bfloat16>, D, st);
   if (rc != QUIC_OK || a.splits == 1) return rc;
   const int64_t warps = (int64_t)a.max_new * a.heads;
   QUIC_CUDA(launch(tree_merge_kernel<T, D>, dim3((unsigned)((warps + 3) / 4), a.requests), dim3(128), 0, st, true, a));
@@ -410,13 +417,16 @@ constexpr int64_t kMostTokens = 1 << 29;  // of a request: sums of two counts st
 // CTAs that share a request's keys, and the tokens of one.  `bound` keys per request at most.
 void plan(int requests, int kv_heads, int heads, int max_new, int64_t bound, int dim, int& splits, int& chunk) {
   const int64_t rows = (int64_t)max_new * (heads / kv_heads);
-  const int64_t units = (int64_t)requests * kv_heads * (rows <= 16 ? 1 : (rows + 31) / 32);
-  const int64_t ctas = 148 * (dim == 64 ? 2 : 1);
-  int64_t parts = units >= ctas ? 1 : ctas / units;
-  const int64_t most = (bound + 255) / 256;  // at least two tiles a warp
-  if (parts > most) parts = most;
-  if (parts < 1) parts = 1;
-  chunk = (int)(((bound + parts - 1) / parts + 63) / 64 * 64);
+  const bool few = rows <= kFewRows;
+  const int64_t units = (int64_t)requests * kv_heads * (few ? 1 : (rows + 127) / 128);
+  const int64_t slots = 148 * (few ? (dim == 64 ? 2 : 1) : (dim == 64 ? 4 : 2));
+  int64_t best = 1, least = INT64_MAX;
+  for (int64_t s = 1; s <= 128 && (s == 1 || (s - 1) * 256 < bound); ++s) {
+    const int64_t part = ((bound + s - 1) / s + 63) / 64 * 64;
+    const int64_t cost = (units * s + slots - 1) / slots * (part + 256) + (s > 1 ? 256 + 8 * s : 0);
+    if (cost < least) least = cost, best = s;
+  }
+  chunk = (int)(((bound + best - 1) / best + 63) / 64 * 64);
   if (chunk < 64) chunk = 64;
   splits = (int)((bound + chunk - 1) / chunk);
   if (splits < 1) splits = 1;

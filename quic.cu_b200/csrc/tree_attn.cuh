@@ -127,4 +127,7 @@ constexpr float kTreeShift = 0.f;
 template <>
 constexpr float kTreeShift<half> = 8.f;
 
+// The throughput form (tree_attn_tc.cu).
+int tree_attn_tc_launch(const TreeArgs& a, bool bf16, int dim, cudaStream_t stream);
+
 }  // namespace quic
