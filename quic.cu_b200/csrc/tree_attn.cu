@@ -418,8 +418,8 @@ constexpr int64_t kMostTokens = 1 << 29;  // of a request: sums of two counts st
 void plan(int requests, int kv_heads, int heads, int max_new, int64_t bound, int dim, int& splits, int& chunk) {
   const int64_t rows = (int64_t)max_new * (heads / kv_heads);
   const bool few = rows <= kFewRows;
-  const int64_t units = (int64_t)requests * kv_heads * (few ? 1 : (rows + 127) / 128);
-  const int64_t slots = 148 * (few ? (dim == 64 ? 2 : 1) : (dim == 64 ? 4 : 2));
+  const int64_t units = (int64_t)requests * kv_heads * (few ? 1 : (rows + 255) / 256);
+  const int64_t slots = 148 * (few && dim == 64 ? 2 : 1);
   int64_t best = 1, least = INT64_MAX;
   for (int64_t s = 1; s <= 128 && (s == 1 || (s - 1) * 256 < bound); ++s) {
     const int64_t part = ((bound + s - 1) / s + 63) / 64 * 64;
