@@ -348,12 +348,12 @@ typedef struct {
  * from row_start[requests] on are left as they were.  K and V of positions that
  * a row does not see do not reach it, whatever they hold.  `scratch` (16-byte
  * aligned, need not be initialised) is used when several CTAs share a request's
- * keys: quic_tree_attn_scratch_bytes of the call's numbers. */
+ * keys: quic_tree_attn_scratch_bytes of the call's numbers, max_new at most rows and
+ * max_len at most max_blocks * block_size. */
 int quic_tree_attn(const quic_tree_attn_t *t, void *scratch, void *stream);
-int64_t quic_tree_attn_scratch_bytes(int32_t rows, int32_t requests,
-                                     int32_t heads, int32_t kv_heads,
-                                     int32_t dim, int32_t max_new,
-                                     int64_t max_len);
+int64_t quic_tree_attn_scratch_bytes(int32_t requests, int32_t heads,
+                                     int32_t kv_heads, int32_t dim,
+                                     int32_t max_new, int64_t max_len);
 
 /* What a step needs to know of its requests, built on the device from their
  * lengths.  n_new[b] > 0: request b gets that many rows behind lengths[b] cached

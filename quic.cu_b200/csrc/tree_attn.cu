@@ -308,136 +308,132 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
       if (c == 0) line[D] = l != l ? INFINITY : m_run[m][h], line[D + 1] = l;  // (a maximum passes over NaN)
     }
   __syncthreads();
-  for (int i = tid; i < kRows * (D / 2); i += kWarps * 32) {
-    const int row = i / (D / 2), d = 2 * (i % (D / 2));
-    if (r0 + row >= all) break;
+  const int64_t part = tree_part(a, blockIdx.z, kvh, tile, split);
+  for (int i = tid; i < kRows * (D / 4); i += kWarps * 32) {
+    const int row = i % kRows, c4 = i / kRows;
+    if (r0 + row >= all) continue;
     const float* line = reinterpret_cast<const float*>(smem) + row * kLine;
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, line[w * kRows * kLine + D]);
     const float ref = top == -INFINITY ? 0.f : top;
-    float x = 0.f, y = 0.f, l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float* at = line + w * kRows * kLine;
       const float f = tree_ex2(at[D] - ref);
       if (f != 0.f) {
-        x += f * at[d];
-        y += f * at[d + 1];
+        const float4 y = *reinterpret_cast<const float4*>(at + 4 * c4);
+        x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
         l += f * at[D + 1];
       }
     }
-    const int nd = (int)a.group.div(r0 + row), head = kvh * (int)a.group.d + (r0 + row) - nd * (int)a.group.d;
-    const int64_t line_out = (int64_t)(r.start + nd) * a.heads + head;
     if (parts == 1) {
+      const int nd = (int)a.group.div(r0 + row), head = kvh * (int)a.group.d + (r0 + row) - nd * (int)a.group.d;
       const float inv = l != 0.f ? 1.f / l : 0.f;  // (NaN stays)
-      *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + line_out * D + d) = tree_pack<T>(x * inv, y * inv);
+      *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + ((int64_t)(r.start + nd) * a.heads + head) * D + 4 * c4) =
+          make_uint2(tree_pack<T>(x.x * inv, x.y * inv), tree_pack<T>(x.z * inv, x.w * inv));
     } else {
-      *reinterpret_cast<float2*>(a.part_o + (line_out * a.splits + split) * D + d) = make_float2(x, y);
-      if (d == 0) a.part_ml[line_out * a.splits + split] = make_float2(top, l);
+      a.part_o[(part * (D / 4) + c4) * a.tile_rows + row] = x;
+      if (c4 == 0) a.part_ml[part * a.tile_rows + row] = make_float2(top, l);
     }
   }
 }
 
-// A row and head whose keys several CTAs shared: sum of the parts, each by 2^(its maximum - the largest).  One warp each.
+// Rows whose keys several CTAs shared: sum of the parts, each by 2^(its maximum - the largest).  A CTA has 32 rows of a tile,
+// a row a lane, so that parts are read in whole lines; its four warps have a quarter of the head dimensions each.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a) {
-  const int lane = threadIdx.x & 31;
-  const TreeRequest r = tree_request(a, blockIdx.y);
+  constexpr int kMine = D / 16;  // float4 of a thread
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y;
+  const int per_tile = a.tile_rows / 32, tile = blockIdx.x / per_tile, row = blockIdx.x % per_tile * 32 + lane;
+  const TreeRequest r = tree_request(a, blockIdx.z);
   int per;
   const int parts = tree_parts(a, r.end, per);
+  const int all = min(r.n, a.max_new) * (int)a.group.d, number = tile * a.tile_rows + row;
   pdl_wait();
-  if (parts == 1) return;
-  const int rows = min(r.n, a.max_new) * a.heads;
-  for (int i = blockIdx.x * 4 + (threadIdx.x >> 5); i < rows; i += gridDim.x * 4) {
-    const int64_t line = (int64_t)r.start * a.heads + i;
-    const float2* ml = a.part_ml + line * a.splits;
-    float top = -INFINITY;
-    for (int s = lane; s < parts; s += 32) top = fmaxf(top, ml[s].x);
-    top = warp_max(top);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float l = 0.f, o[D / 32] = {};
-    for (int s0 = 0; s0 < parts; s0 += 32) {
-      float f = 0.f;
-      if (s0 + lane < parts) {
-        const float2 x = ml[s0 + lane];
-        f = tree_ex2(x.x - ref);
-        if (f != 0.f) l += f * x.y;
-      }
+  if (parts == 1 || number >= all) return;
+  const int64_t part = tree_part(a, blockIdx.z, kvh, tile, 0);
+  const float2* const ml = a.part_ml + part * a.tile_rows + row;
+  const float4* const po = a.part_o + (part * (D / 4) + warp * kMine) * a.tile_rows + row;
+  float top = -INFINITY;
 #pragma unroll 8
-      for (int s = 0; s < min(32, parts - s0); ++s) {
-        const float w = __shfl_sync(0xffffffffu, f, s);
-        const float* at = a.part_o + (line * a.splits + s0 + s) * D + lane * (D / 32);
-        float x[D / 32];
-        if constexpr (D == 64) {
-          const float2 u = *reinterpret_cast<const float2*>(at);
-          x[0] = u.x, x[1] = u.y;
-        } else {
-          const float4 u = *reinterpret_cast<const float4*>(at);
-          x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-        }
+  for (int s = 0; s < parts; ++s) top = fmaxf(top, ml[(int64_t)s * a.tile_rows].x);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float l = 0.f;
+  float4 o[kMine] = {};
+#pragma unroll 2
+  for (int s = 0; s < parts; ++s) {
+    const float2 x = ml[(int64_t)s * a.tile_rows];
+    float4 y[kMine];
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-          if (w != 0.f) o[d] += w * x[d];
-      }
+    for (int c = 0; c < kMine; ++c) y[c] = po[((int64_t)s * (D / 4) + c) * a.tile_rows];
+    const float f = tree_ex2(x.x - ref);
+    if (f != 0.f) {
+      l += f * x.y;
+#pragma unroll
+      for (int c = 0; c < kMine; ++c) o[c].x += f * y[c].x, o[c].y += f * y[c].y, o[c].z += f * y[c].z, o[c].w += f * y[c].w;
     }
-    l = warp_sum(l);
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + line * D) + lane * (D / 64);
-#pragma unroll
-    for (int d = 0; d < D / 64; ++d) out[d] = tree_pack<T>(o[2 * d] * inv, o[2 * d + 1] * inv);
   }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const int node = (int)a.group.div(number), head = kvh * (int)a.group.d + number - node * (int)a.group.d;
+  uint4* const out = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + ((int64_t)(r.start + node) * a.heads + head) * D + warp * kMine * 4);
+#pragma unroll
+  for (int c = 0; c < kMine; c += 2)
+    out[c / 2] = make_uint4(tree_pack<T>(o[c].x * inv, o[c].y * inv), tree_pack<T>(o[c].z * inv, o[c].w * inv),
+                            tree_pack<T>(o[c + 1].x * inv, o[c + 1].y * inv), tree_pack<T>(o[c + 1].z * inv, o[c + 1].w * inv));
 }
 
 template <typename T, int D, int MT>
 int launch_few(const TreeArgs& a, cudaStream_t st) {
-  const int tiles = (int)(((int64_t)a.max_new * a.group.d + 16 * MT - 1) / (16 * MT));
   QUIC_CUDA((allow_smem<tree_attn_kernel<T, D, MT>>(kSmem<D, MT>)));
-  QUIC_CUDA(launch(tree_attn_kernel<T, D, MT>, dim3(a.splits, a.kv_heads * tiles, a.requests), dim3(kWarps * 32), kSmem<D, MT>, st,
+  QUIC_CUDA(launch(tree_attn_kernel<T, D, MT>, dim3(a.splits, a.kv_heads * a.tiles, a.requests), dim3(kWarps * 32), kSmem<D, MT>, st,
                    false, a));
   return QUIC_OK;
 }
-// Rows of a request and KV head beyond which the tcgen05 form takes a call.
-constexpr int64_t kFewRows = 32;
 
 template <typename T, int D>
-int launch_typed(const TreeArgs& a, cudaStream_t st) {
-  const int64_t rows = (int64_t)a.max_new * a.group.d;
-  const int rc = rows <= 16         ? launch_few<T, D, 1>(a, st)
-                 : rows <= kFewRows ? launch_few<T, D, 2>(a, st)
-                                    : tree_attn_tc_launch(a, kTreeExponent<T> == kTreeExponent<__nv_bfloat16>, D, st);
+int launch_typed(const TreeArgs& a, bool tc, cudaStream_t st) {
+  const int rc = tc                ? tree_attn_tc_launch(a, kTreeExponent<T> == kTreeExponent<__nv_bfloat16>, D, st)
+                 : a.max_new * (int64_t)a.group.d <= 16 ? launch_few<T, D, 1>(a, st)
+                                   : launch_few<T, D, 2>(a, st);
   if (rc != QUIC_OK || a.splits == 1) return rc;
-  const int64_t warps = (int64_t)a.max_new * a.heads;
-  QUIC_CUDA(launch(tree_merge_kernel<T, D>, dim3((unsigned)((warps + 3) / 4), a.requests), dim3(128), 0, st, true, a));
+  QUIC_CUDA(launch(tree_merge_kernel<T, D>, dim3((unsigned)(a.tiles * (a.tile_rows / 32)), a.kv_heads, a.requests), dim3(128), 0, st,
+                   true, a));
   return QUIC_OK;
 }
 
 constexpr int64_t kMostTokens = 1 << 29;  // of a request: sums of two counts stay within an int
+// Rows of a request and KV head beyond which the tcgen05 form takes a call.
+constexpr int64_t kFewRows = 32;
 
-// CTAs that share a request's keys, and the tokens of one.  `bound` keys per request at most.
-void plan(int requests, int kv_heads, int heads, int max_new, int64_t bound, int dim, int& splits, int& chunk) {
+struct Plan {
+  bool tc;
+  int64_t tiles;                       // row tiles of a request and KV head
+  int tile_rows, splits, chunk;        // rows of one (a multiple of 32), CTAs that share its keys, the keys of one
+  int64_t parts(int requests, int kv_heads) const { return (int64_t)requests * kv_heads * tiles * splits * tile_rows; }
+};
+// `bound`: keys of a request at most.
+Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound, int dim, bool tma) {
+  Plan p = {};
   const int64_t rows = (int64_t)max_new * (heads / kv_heads);
-  const bool few = rows <= kFewRows;
-  const int64_t units = (int64_t)requests * kv_heads * (few ? 1 : (rows + 255) / 256);
-  const int64_t slots = 148 * (few && dim == 64 ? 2 : 1);
+  p.tc = tma && rows > kFewRows;
+  p.tile_rows = p.tc ? (int)(rows < kTreeTcRows ? (rows + 31) / 32 * 32 : kTreeTcRows) : 32;
+  p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+  bound = bound < kMostTokens ? bound : kMostTokens;
+  const int64_t units = (int64_t)requests * kv_heads * p.tiles, slots = 148 * (!p.tc && dim == 64 ? 2 : 1);
   int64_t best = 1, least = INT64_MAX;
   for (int64_t s = 1; s <= 128 && (s == 1 || (s - 1) * 256 < bound); ++s) {
     const int64_t part = ((bound + s - 1) / s + 63) / 64 * 64;
     const int64_t cost = (units * s + slots - 1) / slots * (part + 256) + (s > 1 ? 256 + 8 * s : 0);
     if (cost < least) least = cost, best = s;
   }
-  chunk = (int)(((bound + best - 1) / best + 63) / 64 * 64);
-  if (chunk < 64) chunk = 64;
-  splits = (int)((bound + chunk - 1) / chunk);
-  if (splits < 1) splits = 1;
-}
-
-bool plan_of(int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim, int32_t max_new, int64_t max_len, int& splits, int& chunk) {
-  if (requests < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || (dim != 64 && dim != 128) || max_new < 1 || max_len < 0)
-    return false;
-  const int64_t bound = max_len + max_new;
-  plan(requests, kv_heads, heads, max_new, bound < kMostTokens ? bound : kMostTokens, dim, splits, chunk);
-  return true;
+  p.chunk = (int)(((bound + best - 1) / best + 63) / 64 * 64);
+  if (p.chunk < 64) p.chunk = 64;
+  p.splits = (int)((bound + p.chunk - 1) / p.chunk);
+  if (p.splits < 1) p.splits = 1;
+  return p;
 }
 
 }  // namespace
@@ -445,11 +441,16 @@ bool plan_of(int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim, int
 
 using namespace quic;
 
-extern "C" int64_t quic_tree_attn_scratch_bytes(int32_t rows, int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim,
-                                                int32_t max_new, int64_t max_len) {
-  int splits, chunk;
-  if (rows < 0 || !plan_of(requests, heads, kv_heads, dim, max_new, max_len, splits, chunk)) return 0;
-  return splits == 1 ? 0 : (int64_t)rows * heads * splits * (dim + 2) * 4;
+extern "C" int64_t quic_tree_attn_scratch_bytes(int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim, int32_t max_new,
+                                                int64_t max_len) {
+  if (requests < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || (dim != 64 && dim != 128) || max_new < 1 || max_len < 0) return 0;
+  int64_t most = 0;  // (by either form: strides decide)
+  for (int tma = 0; tma < 2; ++tma) {
+    const Plan p = make_plan(requests, kv_heads, heads, max_new, max_len + max_new, dim, tma != 0);
+    const int64_t need = p.splits > 1 ? p.parts(requests, kv_heads) * (dim + 2) * 4 : 0;
+    most = need > most ? need : most;
+  }
+  return most;
 }
 
 extern "C" int quic_tree_attn(const quic_tree_attn_t* t, void* scratch, void* stream) {
@@ -471,11 +472,12 @@ extern "C" int quic_tree_attn(const quic_tree_attn_t* t, void* scratch, void* st
   QUIC_REQUIRE((int64_t)t->rows * t->heads < (1ll << 31), QUIC_E_LIMIT, "tree_attn: rows times heads reach 2^31");
   const int max_new = t->max_new < t->rows ? t->max_new : t->rows;
   const int64_t room = (int64_t)t->max_blocks * t->block_size, max_len = t->max_len < room ? t->max_len : room;
+  const bool tma = tree_attn_tc_takes(t->block_size, t->k_block, t->k_head, t->k_tok, t->v_block, t->v_head, t->v_tok);
+  const Plan p = make_plan(t->requests, t->kv_heads, t->heads, max_new, max_len + max_new, t->dim, tma);
+  QUIC_REQUIRE(t->requests <= 65535 && t->kv_heads * p.tiles <= 65535, QUIC_E_LIMIT,
+               "tree_attn: more than 65535 requests, or row tiles of one");
   TreeArgs a = {};
-  QUIC_REQUIRE(plan_of(t->requests, t->heads, t->kv_heads, t->dim, max_new, max_len, a.splits, a.chunk), QUIC_E_SHAPE,
-               "tree_attn: bad shape");
-  const int64_t tiles = (int64_t)t->kv_heads * (((int64_t)max_new * (t->heads / t->kv_heads) + 15) / 16);
-  QUIC_REQUIRE(t->requests <= 65535 && tiles <= 65535, QUIC_E_LIMIT, "tree_attn: more than 65535 requests, or 16-row tiles of one");
+  a.splits = p.splits, a.chunk = p.chunk, a.tiles = (int)p.tiles, a.tile_rows = p.tile_rows;
   QUIC_REQUIRE(a.splits == 1 || (scratch != nullptr && (uintptr_t)scratch % 16 == 0), QUIC_E_ARG,
                "tree_attn: scratch missing or not 16-byte aligned");
   a.q = t->q, a.k = t->k, a.v = t->v, a.out = t->out;
@@ -485,8 +487,8 @@ extern "C" int quic_tree_attn(const quic_tree_attn_t* t, void* scratch, void* st
   a.table_row = t->table_row, a.mask_row = t->mask_row;
   a.tables = t->tables, a.lengths = t->lengths, a.row_start = t->row_start;
   a.mask = (const uint32_t*)t->mask, a.mask_words = t->mask_words;
-  a.part_o = (float*)scratch;
-  a.part_ml = (float2*)(a.part_o + (int64_t)t->rows * t->heads * a.splits * t->dim);
+  a.part_o = (float4*)scratch;
+  a.part_ml = (float2*)(a.part_o + p.parts(t->requests, t->kv_heads) * (t->dim / 4));
   a.block = FastDiv::of((uint32_t)t->block_size);
   a.group = FastDiv::of((uint32_t)(t->heads / t->kv_heads));
   a.rows = t->rows, a.requests = t->requests, a.heads = t->heads, a.kv_heads = t->kv_heads;
@@ -494,6 +496,6 @@ extern "C" int quic_tree_attn(const quic_tree_attn_t* t, void* scratch, void* st
   a.scale_log2 = (t->scale > 0.f ? t->scale : 1.f / sqrtf((float)t->dim)) * 1.4426950408889634f;
   cudaStream_t st = (cudaStream_t)stream;
   if (t->dtype == QUIC_DTYPE_F16)
-    return t->dim == 64 ? launch_typed<half, 64>(a, st) : launch_typed<half, 128>(a, st);
-  return t->dim == 64 ? launch_typed<__nv_bfloat16, 64>(a, st) : launch_typed<__nv_bfloat16, 128>(a, st);
+    return t->dim == 64 ? launch_typed<half, 64>(a, p.tc, st) : launch_typed<half, 128>(a, p.tc, st);
+  return t->dim == 64 ? launch_typed<__nv_bfloat16, 64>(a, p.tc, st) : launch_typed<__nv_bfloat16, 128>(a, p.tc, st);
 }

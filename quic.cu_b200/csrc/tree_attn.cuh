@@ -25,10 +25,11 @@ struct TreeArgs {
   int64_t q_row, q_head, k_block, k_head, k_tok, v_block, v_head, v_tok, table_row, mask_row;
   const int32_t *tables, *lengths, *row_start;
   const uint32_t* mask;              // [rows][mask_words] by mask_row, or nullptr: node i sees nodes 0 .. i
-  float* part_o;                     // [rows][heads][splits][dim]
-  float2* part_ml;                   // [rows][heads][splits]: maximum (base 2), sum
+  float4* part_o;                    // [requests][kv heads][tiles][splits][dim / 4][tile_rows]
+  float2* part_ml;                   // [requests][kv heads][tiles][splits][tile_rows]: maximum (base 2), sum
   FastDiv block, group;              // tokens per block, query heads per KV head
   int32_t rows, requests, heads, kv_heads, n_blocks, max_blocks, mask_words, max_new;
+  int32_t tiles, tile_rows;          // row tiles of a request and KV head, rows of one
   int32_t splits, chunk;             // CTAs per request, KV head and row tile at most; the tokens of one
   float scale_log2;
 };
@@ -53,6 +54,11 @@ __device__ __forceinline__ int tree_parts(const TreeArgs& a, int end, int& per) 
   const int parts = max(1, min(a.splits, (end + a.chunk - 1) / a.chunk));
   per = ((end + parts - 1) / parts + 63) & ~63;
   return per > 0 ? (end + per - 1) / per : 1;
+}
+
+// A row tile's part number `split` of the partial results.
+__device__ __forceinline__ int64_t tree_part(const TreeArgs& a, int b, int kvh, int tile, int split) {
+  return (((int64_t)b * a.kv_heads + kvh) * a.tiles + tile) * a.splits + split;
 }
 
 // Which of the 32 positions from t on node `node` sees, the positions up to `end` taken for present: bit j for t + j.
@@ -127,7 +133,9 @@ constexpr float kTreeShift = 0.f;
 template <>
 constexpr float kTreeShift<half> = 8.f;
 
-// The throughput form (tree_attn_tc.cu).
+// The throughput form (tree_attn_tc.cu) has 256 rows of a request and KV head a CTA, and takes what TMA can fetch.
+constexpr int kTreeTcRows = 256;
+bool tree_attn_tc_takes(int block_size, int64_t k_block, int64_t k_head, int64_t k_tok, int64_t v_block, int64_t v_head, int64_t v_tok);
 int tree_attn_tc_launch(const TreeArgs& a, bool bf16, int dim, cudaStream_t stream);
 
 }  // namespace quic

@@ -11,14 +11,15 @@
 //   O += P V       B = the V tile as it lies in the cache (token-major, the transposed form), 64 dims a product.
 // The reference point of a row's exponentials moves only when its maximum has grown by more than 2^8 (P and the sums stay far
 // within their types' ranges); O is rescaled in tensor memory then.
-// K and V come by cp.async from four warps, 16 keys of the tile each: that takes blocks and strides of any size, and leaves
-// zeros where there is no key.  They signal a stage after their copies have landed and a proxy fence; while the next
-// stage is not yet free they wait for the oldest copy under way, so that no more than that is ever held back.
+// K and V come by TMA, in boxes of as many tokens as lie together in a block for sure (the largest power of two that divides
+// the block size, 8 to 64); positions without a block are fetched from beyond the planes, as zeros.  (By cp.async, which takes
+// any block size, the loaders had to fence every stage for the tensor cores, and the fence waited for all copies under way:
+// 215 us instead of CHECK at 8 requests x 64 nodes x 16384 tokens, 32:8 heads of 128.)
 // Only tiles that reach beyond the cached tokens look at masks.  A V row of a node may hold infinities or NaN that most rows
 // must not see: such values are zeroed in shared memory and added, at the end, to the rows that see them.
 //
-// Roles: warps 0-7 softmax and epilogue, warp 8 MMA issuer (next scores or next product, whichever is ready), warps 9-12
-// loaders.  Every wait is bounded; a wait that runs out sets word 0 of the tensor path's error words and the CTA leaves with
+// Roles: warps 0-7 queries, softmax and epilogue, warp 8 MMA issuer (next scores or next product, whichever is ready), warp 9
+// TMA.  Every wait is bounded; a wait that runs out sets word 0 of the tensor path's error words and the CTA leaves with
 // its MMAs and copies complete and its tensor memory released.
 #include "tc_common.cuh"
 #include "tree_attn.cuh"
@@ -26,9 +27,9 @@
 namespace quic {
 namespace {
 
-constexpr int kRows = 128, kKeys = 64, kGroupWarps = 4, kSoftmaxWarps = 2 * kGroupWarps, kLoaders = 4;
-constexpr int kThreads = (kSoftmaxWarps + 1 + kLoaders) * 32;
-constexpr int kLoadKeys = kKeys / kLoaders;
+constexpr int kRows = 128, kKeys = 64, kGroupWarps = 4, kSoftmaxWarps = 2 * kGroupWarps;
+constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
+static_assert(2 * kRows == kTreeTcRows, "two streams of rows");
 constexpr float kGrowth = 8.f;    // of a row's maximum (base 2) before its reference point follows
 template <typename T>
 constexpr float kShift = 0.f;     // P = 2^(score - reference + shift)
@@ -38,7 +39,7 @@ constexpr uint32_t kHalfQ = kRows * 128, kHalfK = kKeys * 128;  // 64 dims of Q,
 
 struct TreeTcArgs {
   TreeArgs t;
-  int32_t tiles;          // 256-row tiles of a request and KV head
+  int32_t box, log_boxes; // tokens of a TMA box, log2 of the boxes of a tile
   uint32_t wait_limit_us;
   int32_t skip_tile;      // test hook: this key tile never comes; below -1, all come late (-1: none)
 };
@@ -49,17 +50,11 @@ __device__ __forceinline__ void mbar_arrive_cta(uint32_t bar) {
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {  // zeros beyond `bytes`
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void copies_landed_but(int n) {  // all groups of this thread but the last n
-  switch (n) {
-    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-    case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-    case 6: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
-    default: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
-  }
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
 }
 __device__ __forceinline__ uint64_t pair2(float x, float y) {
   uint64_t d;
@@ -118,24 +113,26 @@ constexpr int kStages = D == 64 ? 8 : 5;
 template <int D>
 constexpr uint32_t kTcSmem = (D / 64) * (2 * kHalfQ + kStages<D> * 2 * kHalfK) + 1024;  // Q of both streams, stages of K and V
 static_assert(kTcSmem<128> + 1024 <= 232448 && kTcSmem<64> > 115 * 1024, "one CTA fills an SM: it takes all tensor memory");
-static_assert(kStages<64> <= 8 && kStages<128> <= 8, "copies_landed_but");
-static_assert(kRows * 64 * 4 <= kStages<64> * 2 * kHalfK && kRows * 128 * 4 <= 2 * kStages<128> * 2 * kHalfK, "O of a stream fits the stages");
+// O of a stream (fp32), and behind it the results of both (16 bits), lie in the stages at the end
+static_assert(kRows * 64 * (4 + 2 * 2) <= kStages<64> * 2 * kHalfK && kRows * 128 * (4 + 2 * 2) <= 2 * kStages<128> * 2 * kHalfK, "stages");
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_constant__ TreeTcArgs args, int* status) {
+__global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k,
+                                                                   const __grid_constant__ CUtensorMap tm_v,
+                                                                   const __grid_constant__ TreeTcArgs args, int* status) {
   constexpr int kHalves = D / 64, kRing = kStages<D>;
   constexpr uint32_t kColO = 256, kTmemCols = 512;  // scores of stream g, buffer x: 128 g + 64 x; O of stream g: 256 + 128 g
   constexpr uint32_t kQ = kHalves * kHalfQ, kK = 2 * kQ, kTile = kHalves * kHalfK, kStage = 2 * kTile;  // a stage: K, V
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t bar_full[kRing], bar_empty[kRing], bar_s[2][2], bar_p[2][2], bar_o[2][2], bar_drain;
-  __shared__ __align__(8) uint16_t valid_s[kRing][kLoaders];
+  __shared__ __align__(8) uint64_t bar_full[kRing], bar_empty[kRing], bar_s[2][2], bar_p[2][2], bar_o[2][2], bar_q, bar_drain;
+  __shared__ uint32_t valid_s[kRing];  // which boxes of the stage have a block
   __shared__ float2 other_s[kRows];
   __shared__ uint32_t tmem_base_s;
   __shared__ int fail_s, odd_s;  // odd_s: the first tile in which V held what is not finite
 
   const TreeArgs& a = args.t;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int tile = blockIdx.x % args.tiles, split = blockIdx.x / args.tiles, kvh = blockIdx.y;
+  const int tile = blockIdx.x % a.tiles, split = blockIdx.x / a.tiles, kvh = blockIdx.y;
   const TreeRequest r = tree_request(a, blockIdx.z);
   const int all = min(r.n, a.max_new) * (int)a.group.d, r0 = tile * 2 * kRows;
   if (r0 >= all) return;
@@ -152,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
 
   if (tid == 0) {
     for (int s = 0; s < kRing; ++s) {
-      mbar_init(smem_u32(&bar_full[s]), kLoaders);
+      mbar_init(smem_u32(&bar_full[s]), 1);
       mbar_init(smem_u32(&bar_empty[s]), 1);
     }
     for (int g = 0; g < 2; ++g)
@@ -161,28 +158,26 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
         mbar_init(smem_u32(&bar_p[g][x]), warps_of(g));
         mbar_init(smem_u32(&bar_o[g][x]), 1);
       }
+    mbar_init(smem_u32(&bar_q), kSoftmaxWarps);
     mbar_init(smem_u32(&bar_drain), 1);
     fail_s = 0;
     odd_s = 0x7fffffff;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 0) {
+  if (warp == kSoftmaxWarps) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  if (warp <= kSoftmaxWarps) {  // queries; rows that are none are zero
-    for (int i = tid; i < (halves ? 2 : 1) * kRows * (D / 8); i += (kSoftmaxWarps + 1) * 32) {
-      const int row = i / (D / 8), chunk = i % (D / 8);
-      uint4 w = make_uint4(0u, 0u, 0u, 0u);
-      if (r0 + row < all) {
-        const int node = (int)a.group.div(r0 + row), head = kvh * (int)a.group.d + (r0 + row) - node * (int)a.group.d;
-        w = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (int64_t)(r.start + node) * a.q_row +
-                                                 (int64_t)head * a.q_head) + chunk);
-      }
-      *reinterpret_cast<uint4*>(smem + (row / kRows) * kQ + (chunk >> 3) * kHalfQ + sw128_offset(row % kRows, chunk & 7)) = w;
+  } else if (warp < kSoftmaxWarps) {  // queries; rows that are none are zero
+    const int rows = halves ? 2 * kRows : kRows;
+#pragma unroll 4
+    for (int i = tid; i < rows * (D / 8); i += kSoftmaxWarps * 32) {
+      const int row = i / (D / 8), chunk = i % (D / 8), number = min(r0 + row, all - 1);
+      const int node = (int)a.group.div(number), head = kvh * (int)a.group.d + number - node * (int)a.group.d;
+      copy16(base + (row / kRows) * kQ + (chunk >> 3) * kHalfQ + sw128_offset(row % kRows, chunk & 7),
+             reinterpret_cast<const T*>(a.q) + (int64_t)(r.start + node) * a.q_row + (int64_t)head * a.q_head + 8 * chunk,
+             r0 + row < all ? 16u : 0u);
     }
-    fence_proxy_async();
   }
   tc_fence_before();
   __syncthreads();
@@ -195,119 +190,113 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
   float m_run = -INFINITY, l_run = 0.f;
   int steps = 0;
   if (warp > kSoftmaxWarps) {
-    // ---------------- loaders ----------------
-    const int me = warp - kSoftmaxWarps - 1;
+    // ---------------- TMA: a lane a box of 64 dims of K or V ----------------
+    const int boxes = 1 << args.log_boxes, box = lane & (boxes - 1), what = lane >> args.log_boxes;
+    const bool copies = what < 2 * kHalves;
+    const CUtensorMap* const map = what & 1 ? &tm_v : &tm_k;
+    const uint32_t dst = base + kK + (what & 1) * kTile + (what >> 1) * kHalfK + box * args.box * 128;
     const int32_t* table = a.tables + (int64_t)blockIdx.z * a.table_row;
-    auto place = [&](int i) { return t_begin + i * kKeys + kLoadKeys * me + (lane & (kLoadKeys - 1)); };
-    auto fetch = [&](int i) {  // the block of this lane's key of tile i, -1 where there is none
-      const int p = place(i);
-      const int id = p < t_end ? __ldg(table + a.block.div(p)) : -1;
-      return id < a.n_blocks ? id : -1;
+    if (lane < 2) tma_prefetch_desc(lane ? &tm_v : &tm_k);
+    auto place = [&](int i) { return t_begin + i * kKeys + box * args.box; };
+    auto fetch = [&](int i) {  // the block of this lane's box of tile i, n_blocks (beyond the planes) where there is none
+      const int p = place(i), id = p < t_end ? __ldg(table + a.block.div(p)) : -1;
+      return id >= 0 && id < a.n_blocks ? id : a.n_blocks;
     };
-    int landed = 0, id = fetch(0);  // tiles that have been signalled
-    auto signal = [&](int issued) {
-      copies_landed_but(issued - landed - 1);
-      fence_proxy_async();
+    int id = fetch(0), next = fetch(1);
+    for (int i = 0; i < n_tiles; ++i) {
+      const int st = i % kRing, after = fetch(i + 2);
+      if (i >= kRing && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_empty[st]), (i / kRing - 1) & 1, args.wait_limit_us))) {
+        fail_s = 2;
+        break;
+      }
+      if (args.skip_tile < -1) pause_us(-args.skip_tile);
+      const uint32_t there = __ballot_sync(0xffffffffu, id < a.n_blocks) & (0xffffffffu >> (32 - boxes));
+      const uint32_t full = smem_u32(&bar_full[st]);
+      if (lane == 0) {
+        valid_s[st] = there;
+        mbar_expect_tx(full, kStage);
+      }
       __syncwarp();
-      if (lane == 0 && landed != args.skip_tile) mbar_arrive_cta(smem_u32(&bar_full[landed % kRing]));
-      ++landed;
-    };
-    bool ok = true;
-    for (int i = 0; ok && i < n_tiles; ++i) {
-      const int st = i % kRing;
-      if (i >= kRing) {
-        const uint32_t bar = smem_u32(&bar_empty[st]), parity = (i / kRing - 1) & 1;
-        while (landed < i && !__all_sync(0xffffffffu, mbar_test(bar, parity))) signal(i);
-        ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, args.wait_limit_us));
-        if (!ok) {
-          fail_s = 2;
+      const int p = place(i);
+      if (copies && (i != args.skip_tile || (what & 1)))
+        tma_load_4d(dst + st * kStage, map, 64 * (what >> 1), p - (int)a.block.div(p) * (int)a.block.d, kvh, id, full);
+      id = next;
+      next = after;
+    }
+  } else if (warp == kSoftmaxWarps) {
+    // ---------------- MMA issuer: a warp in step, one lane of which issues ----------------
+    issuer = elect_one();
+    const uint64_t q0 = umma_desc_sw128(base), k0 = umma_desc_sw128(base + kK);
+    // V: head dims contiguous, the two halves of 128 dims kHalfK apart (leading byte offset)
+    const uint64_t v0 = umma_desc_sw128(base + kK + kTile) + ((uint64_t)(kHalfK / 16 - 1) << 16);
+    constexpr uint32_t kType = kTreeExponent<T> == kTreeExponent<__nv_bfloat16> ? (1u << 7) | (1u << 10) : 0u;  // bf16 x bf16
+    const uint32_t idesc = umma_idesc_f16(kKeys) | kType;        // M = 128, N = 64
+    const uint32_t idesc_v = umma_idesc_f16(D) | kType | (1u << 16);  // N = the head dims, B transposed
+    int next_s = 0, next_p = 0, idle = 0;
+    uint32_t since = 0;
+    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_q), 0, args.wait_limit_us))) {
+      fail_s = 3;
+      next_p = items;
+    }
+    while (next_p < items) {
+      bool moved = false;
+      if (next_s < items && next_s < next_p + 4) {  // (the buffer's last P is with the product of item next_s - 4)
+        const int g = next_s & 1, u = next_s >> 1, i = halves ? u : next_s, st = i % kRing;
+        if (__all_sync(0xffffffffu, mbar_test(smem_u32(&bar_full[st]), (i / kRing) & 1) &&
+                                        (u < 2 || mbar_test(smem_u32(&bar_o[g][u & 1]), ((u >> 1) - 1) & 1)))) {
+          tc_fence_after();
+          const uint64_t q = q0 + (uint64_t)((halves ? g : 0) * (kQ / 16)), kt = k0 + (uint64_t)(st * (kStage / 16));
+          const uint32_t to = tmem + 128u * g + 64u * (u & 1), bar = smem_u32(&bar_s[g][u & 1]);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              umma_f16(to, q + (uint64_t)((k >> 2) * (kHalfQ / 16)) + 2 * (k & 3), kt + (uint64_t)((k >> 2) * (kHalfK / 16)) + 2 * (k & 3),
+                       idesc, k > 0 ? 1u : 0u);
+            umma_commit(bar);
+          }
+          __syncwarp();
+          ++next_s;
+          moved = true;
+        }
+      }
+      if (next_p < next_s) {
+        const int g = next_p & 1, u = next_p >> 1, i = halves ? u : next_p, st = i % kRing;
+        if (__all_sync(0xffffffffu, mbar_test(smem_u32(&bar_p[g][u & 1]), (u >> 1) & 1))) {  // P is there, O rescaled where need be
+          tc_fence_after();
+          const uint64_t vt = v0 + (uint64_t)(st * (kStage / 16));
+          const uint32_t to = tmem + kColO + 128u * g, from = tmem + 128u * g + 64u * (u & 1), bar = smem_u32(&bar_o[g][u & 1]);
+          const uint32_t free = smem_u32(&bar_empty[st]), more = u > 0 ? 1u : 0u;
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)  // sixteen tokens a step: two groups of eight rows of the V tile, eight columns of P
+              umma_ts(to, from + 8u * k, vt + k * (2048 / 16), idesc_v, k > 0 ? 1u : more);
+            umma_commit(bar);
+            if (!halves || g == 1) umma_commit(free);
+          }
+          __syncwarp();
+          ++next_p;
+          moved = true;
+        }
+      }
+      if (moved) {
+        idle = 0;
+      } else if ((++idle & 63) == 0) {
+        const uint32_t now = __shfl_sync(0xffffffffu, clock_us(), 0);
+        if (idle == 64) since = now;
+        else if (now - since >= args.wait_limit_us) {
+          fail_s = 3;
           break;
         }
       }
-      if (args.skip_tile < -1) pause_us(-args.skip_tile);
-      const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
-      if (lane == 0) valid_s[st][me] = (uint16_t)there;
-      const int p = place(i), off = p - (int)a.block.div(p) * (int)a.block.d;
-      const int64_t k_at = id >= 0 ? id * a.k_block + off * a.k_tok : 0, v_at = id >= 0 ? id * a.v_block + off * a.v_tok : 0;
-      const int chunk = lane & 7;  // four rows of eight 16-byte chunks an instruction
-      const T* const k0 = reinterpret_cast<const T*>(a.k) + kvh * a.k_head + chunk * 8;
-      const T* const v0 = reinterpret_cast<const T*>(a.v) + kvh * a.v_head + chunk * 8;
-#pragma unroll
-      for (int j = 0; j < kLoadKeys / 4; ++j) {
-        const int key = 4 * j + (lane >> 3);
-        const T* const k = k0 + __shfl_sync(0xffffffffu, k_at, key);
-        const T* const v = v0 + __shfl_sync(0xffffffffu, v_at, key);
-        const uint32_t bytes = there >> key & 1u ? 16u : 0u;
-        const uint32_t dst = base + kK + st * kStage + sw128_offset(kLoadKeys * me + key, chunk);
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          copy16(dst + h * kHalfK, k + 64 * h, bytes);
-          copy16(dst + kTile + h * kHalfK, v + 64 * h, bytes);
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      id = fetch(i + 1);
     }
-    while (ok && landed < n_tiles) signal(n_tiles);
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == kSoftmaxWarps) {
-    // ---------------- MMA issuer ----------------
-    issuer = elect_one();
-    if (issuer) {
-      const uint64_t q0 = umma_desc_sw128(base), k0 = umma_desc_sw128(base + kK), v0 = umma_desc_sw128(base + kK + kTile);
-      constexpr uint32_t kType = kTreeExponent<T> == kTreeExponent<__nv_bfloat16> ? (1u << 7) | (1u << 10) : 0u;  // bf16 x bf16
-      const uint32_t idesc = umma_idesc_f16(kKeys) | kType;  // M = 128, N = 64
-      const uint32_t idesc_v = idesc | (1u << 16);           // B transposed: N (the head dims) contiguous
-      int next_s = 0, next_p = 0, idle = 0;
-      uint32_t since = 0;
-      while (next_p < items) {
-        bool moved = false;
-        if (next_s < items && next_s < next_p + 4) {  // (the buffer's last P is with the product of item next_s - 4)
-          const int g = next_s & 1, u = next_s >> 1, i = halves ? u : next_s, st = i % kRing;
-          if (mbar_test(smem_u32(&bar_full[st]), (i / kRing) & 1) &&
-              (u < 2 || mbar_test(smem_u32(&bar_o[g][u & 1]), ((u >> 1) - 1) & 1))) {
-            tc_fence_after();
-            const uint64_t q = q0 + (uint64_t)((halves ? g : 0) * (kQ / 16)), kt = k0 + (uint64_t)(st * (kStage / 16));
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              umma_f16(tmem + 128u * g + 64u * (u & 1), q + (uint64_t)((k >> 2) * (kHalfQ / 16)) + 2 * (k & 3),
-                       kt + (uint64_t)((k >> 2) * (kHalfK / 16)) + 2 * (k & 3), idesc, k > 0 ? 1u : 0u);
-            umma_commit(smem_u32(&bar_s[g][u & 1]));
-            ++next_s;
-            moved = true;
-          }
-        }
-        if (next_p < next_s) {
-          const int g = next_p & 1, u = next_p >> 1, i = halves ? u : next_p, st = i % kRing;
-          if (mbar_test(smem_u32(&bar_p[g][u & 1]), (u >> 1) & 1)) {  // P is in tensor memory, O rescaled where need be
-            tc_fence_after();
-            const uint64_t vt = v0 + (uint64_t)(st * (kStage / 16));
-#pragma unroll
-            for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)  // sixteen tokens a step: two groups of eight rows of the V tile, eight columns of P
-                umma_ts(tmem + kColO + 128u * g + 64u * h, tmem + 128u * g + 64u * (u & 1) + 8u * k,
-                        vt + (uint64_t)(h * (kHalfK / 16)) + k * (2048 / 16), idesc_v, (u > 0 || k > 0) ? 1u : 0u);
-            umma_commit(smem_u32(&bar_o[g][u & 1]));
-            if (!halves || g == 1) umma_commit(smem_u32(&bar_empty[st]));
-            ++next_p;
-            moved = true;
-          }
-        }
-        if (moved) {
-          idle = 0;
-        } else if ((++idle & 63) == 0) {
-          const uint32_t now = clock_us();
-          if (idle == 64) since = now;
-          else if (now - since >= args.wait_limit_us) {
-            fail_s = 3;
-            break;
-          }
-        }
-      }
-    }
-  } else if (quarter < warps_of(group)) {
+  } else {
     // ---------------- softmax ----------------
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive_cta(smem_u32(&bar_q));
+  }
+  if (warp < kSoftmaxWarps && quarter < warps_of(group)) {
     const int mine = min(r0 + (halves ? group * kRows : 0) + 32 * quarter + lane, all - 1), node = (int)a.group.div(mine);
     const uint32_t lane_addr = (uint32_t)(32 * quarter) << 16;
     const uint32_t at_o = tmem + kColO + 128u * group + lane_addr;
@@ -325,27 +314,37 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
       tc_fence_after();
       float s[64];
       tmem_ld_cols<64>(at_s, s);
-      const uint2 valid = *reinterpret_cast<const uint2*>(valid_s[st]);
+      const uint32_t there = valid_s[st];
       const bool tree = t + kKeys > r.len;
       if (tree) {  // (the same for all the CTA's rows)
         unsigned char* const v_tile = smem + kK + st * kStage + kTile;
-        bool odd = false;
+        bool odd = false, changed = false;
         for (int c = 32 * quarter + lane; c < (int)kTile / 16; c += 32 * warps_of(group)) {
           uint4 w = reinterpret_cast<const uint4*>(v_tile)[c];
           if (tree_not_finite<T>(w.x) || tree_not_finite<T>(w.y) || tree_not_finite<T>(w.z) || tree_not_finite<T>(w.w)) {
             w.x = tree_finite<T>(w.x), w.y = tree_finite<T>(w.y), w.z = tree_finite<T>(w.z), w.w = tree_finite<T>(w.w);
             reinterpret_cast<uint4*>(v_tile)[c] = w;
-            odd = true;
+            odd |= t + (c % (kKeys * 8)) / 8 < t_end;  // (rows behind the last key may hold anything)
+            changed = true;
           }
         }
-        if (odd) {
-          fence_proxy_async();
-          atomicMin(&odd_s, i);
-        }
+        if (changed) fence_proxy_async();
+        if (odd) atomicMin(&odd_s, i);
         __syncwarp();
       }
-      if (tree || (valid.x & valid.y) != 0xffffffffu) {
-        const uint32_t seen0 = valid.x & tree_visible32(a, r, node, t), seen1 = valid.y & tree_visible32(a, r, node, t + 32);
+      if (tree || there != (0xffffffffu >> (32 - (1 << args.log_boxes)))) {
+        uint32_t seen0 = tree_visible32(a, r, node, t), seen1 = tree_visible32(a, r, node, t + 32);
+        const int left = t_end - t;
+        if (left < 64) {
+          seen0 &= left < 32 ? (1u << max(left, 0)) - 1u : 0xffffffffu;
+          seen1 &= left < 32 ? 0u : (1u << (left - 32)) - 1u;
+        }
+        if (there != (0xffffffffu >> (32 - (1 << args.log_boxes)))) {
+          for (int j = 0; j < 32; ++j) {
+            if (!(there >> (j / args.box) & 1u)) seen0 &= ~(1u << j);
+            if (!(there >> ((j + 32) / args.box) & 1u)) seen1 &= ~(1u << j);
+          }
+        }
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
           if (!(seen0 >> j & 1u)) s[j] = -INFINITY;
@@ -431,8 +430,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
   if (!halves) __syncthreads();
   if (has_rows && (halves || group == 0)) {
     const int row = 32 * quarter + lane, number = r0 + (halves ? group * kRows : 0) + row;
-    const int mine = min(number, all - 1), node = (int)a.group.div(mine), head = kvh * (int)a.group.d + mine - node * (int)a.group.d;
-    const int64_t line = (int64_t)(r.start + node) * a.heads + head;
+    const int node = (int)a.group.div(min(number, all - 1));
+    const int64_t part = tree_part(a, blockIdx.z, kvh, tile, split);
+    unsigned char* const lines = smem + kK + kRows * D * 4 + warp * 32 * D * 2;
     const int odd_from = odd_s;
     float f0 = 1.f, f1 = 0.f;
     if (!halves && n_tiles > 1) {
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
     }
     const float inv = parts > 1 ? 1.f : (l_run != 0.f ? 1.f / l_run : 0.f);
     const bool write = number < all;
-    if (parts > 1 && write) a.part_ml[line * a.splits + split] = make_float2(m_run, l_run);
+    if (parts > 1 && write) a.part_ml[part * a.tile_rows + number - r0] = make_float2(m_run, l_run);
 #pragma unroll 1
     for (int c = 0; c < D / 16; ++c) {
       float o[16] = {};
@@ -474,16 +474,31 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
           }
         }
       }
-      if (write && parts > 1) {
-        float4* const to = reinterpret_cast<float4*>(a.part_o + (line * a.splits + split) * D + 16 * c);
+      if (parts > 1) {
+        if (write) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) to[x] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
-      } else if (write) {
-        uint4* const to = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + line * D + 16 * c);
+          for (int x = 0; x < 4; ++x)
+            a.part_o[(part * (D / 4) + 4 * c + x) * a.tile_rows + number - r0] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        }
+      } else {
 #pragma unroll
         for (int x = 0; x < 2; ++x)
-          to[x] = make_uint4(tree_pack<T>(o[8 * x] * inv, o[8 * x + 1] * inv), tree_pack<T>(o[8 * x + 2] * inv, o[8 * x + 3] * inv),
-                             tree_pack<T>(o[8 * x + 4] * inv, o[8 * x + 5] * inv), tree_pack<T>(o[8 * x + 6] * inv, o[8 * x + 7] * inv));
+          *reinterpret_cast<uint4*>(lines + lane * (D * 2) + (((2 * c + x) ^ (lane & 7)) << 4)) =
+              make_uint4(tree_pack<T>(o[8 * x] * inv, o[8 * x + 1] * inv), tree_pack<T>(o[8 * x + 2] * inv, o[8 * x + 3] * inv),
+                         tree_pack<T>(o[8 * x + 4] * inv, o[8 * x + 5] * inv), tree_pack<T>(o[8 * x + 6] * inv, o[8 * x + 7] * inv));
+      }
+    }
+    if (parts == 1) {  // whole rows, from shared memory
+      __syncwarp();
+      const int first = number - lane;
+#pragma unroll 4
+      for (int i = lane; i < 32 * (D / 8); i += 32) {
+        const int at = i / (D / 8), chunk = i % (D / 8);
+        if (first + at < all) {
+          const int nd = (int)a.group.div(first + at), hd = kvh * (int)a.group.d + first + at - nd * (int)a.group.d;
+          reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + ((int64_t)(r.start + nd) * a.heads + hd) * D)[chunk] =
+              *reinterpret_cast<const uint4*>(lines + at * (D * 2) + ((chunk ^ (at & 7)) << 4));
+        }
       }
     }
   }
@@ -494,29 +509,57 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
     if (tid == 0) tc_report(status, (fail_s << 16) | 0x3000 | ((int)blockIdx.x & 0xfff));
     drain_failed(issuer, smem_u32(&bar_drain));
   }
-  if (warp == 0)
+  if (warp == kSoftmaxWarps)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_s), "r"(kTmemCols) : "memory");
 }
 
 template <typename T, int D>
-int launch_tc(const TreeTcArgs& a, cudaStream_t stream, int* status) {
+int launch_tc(const TreeTcArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t stream, int* status) {
   QUIC_CUDA((allow_smem<tree_attn_tc_kernel<T, D>>(kTcSmem<D>)));
-  QUIC_CUDA(launch(tree_attn_tc_kernel<T, D>, dim3((unsigned)(a.tiles * a.t.splits), a.t.kv_heads, a.t.requests), dim3(kThreads),
-                   kTcSmem<D>, stream, false, a, status));
+  QUIC_CUDA(launch(tree_attn_tc_kernel<T, D>, dim3((unsigned)(a.t.tiles * a.t.splits), a.t.kv_heads, a.t.requests), dim3(kThreads),
+                   kTcSmem<D>, stream, false, tm_k, tm_v, a, status));
   return QUIC_OK;
 }
 
+int box_tokens(int block_size) {
+  int box = block_size & -block_size;
+  return box < kKeys ? box : kKeys;
+}
+
+// [n_blocks][kv heads][block][dim] by strides, 64 dims of `box` tokens at a time
+int plane_map(CUtensorMap* map, const TreeArgs& t, const void* base, int64_t block, int64_t head, int64_t tok, int dim, int box, bool bf16) {
+  const cuuint64_t dims[4] = {(cuuint64_t)dim, t.block.d, (cuuint64_t)t.kv_heads, (cuuint64_t)t.n_blocks};
+  const cuuint64_t strides[3] = {(cuuint64_t)tok * 2, (cuuint64_t)head * 2, (cuuint64_t)block * 2};
+  const cuuint32_t shape[4] = {64, (cuuint32_t)box, 1, 1};
+  return make_tiled_map(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, shape,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+}
+
 }  // namespace
+
+// Boxes of whole groups of eight rows (the swizzle's period) and strides that a tensor map can have.
+bool tree_attn_tc_takes(int block_size, int64_t k_block, int64_t k_head, int64_t k_tok, int64_t v_block, int64_t v_head, int64_t v_tok) {
+  if (block_size % 8 != 0) return false;
+  for (int64_t s : {k_block, k_head, k_tok, v_block, v_head, v_tok})
+    if (s <= 0 || s >= (1ll << 39)) return false;
+  return true;
+}
 
 int tree_attn_tc_launch(const TreeArgs& t, bool bf16, int dim, cudaStream_t stream) {
   int* status = tc_status_words();
   QUIC_REQUIRE(status != nullptr, QUIC_E_CUDA, "tree_attn: no address for the tensor path's error words");
   TreeTcArgs a = {};
   a.t = t;
-  a.tiles = (int)(((int64_t)t.max_new * t.group.d + 2 * kRows - 1) / (2 * kRows));
+  a.box = box_tokens((int)t.block.d);
+  while ((a.box << a.log_boxes) < kKeys) ++a.log_boxes;
   tc_test_hook(&a.wait_limit_us, &a.skip_tile);
-  if (dim == 128) return bf16 ? launch_tc<__nv_bfloat16, 128>(a, stream, status) : launch_tc<half, 128>(a, stream, status);
-  return bf16 ? launch_tc<__nv_bfloat16, 64>(a, stream, status) : launch_tc<half, 64>(a, stream, status);
+  CUtensorMap tm_k, tm_v;
+  int rc = plane_map(&tm_k, t, t.k, t.k_block, t.k_head, t.k_tok, dim, a.box, bf16);
+  if (rc == QUIC_OK) rc = plane_map(&tm_v, t, t.v, t.v_block, t.v_head, t.v_tok, dim, a.box, bf16);
+  if (rc != QUIC_OK) return rc;
+  if (dim == 128)
+    return bf16 ? launch_tc<__nv_bfloat16, 128>(a, tm_k, tm_v, stream, status) : launch_tc<half, 128>(a, tm_k, tm_v, stream, status);
+  return bf16 ? launch_tc<__nv_bfloat16, 64>(a, tm_k, tm_v, stream, status) : launch_tc<half, 64>(a, tm_k, tm_v, stream, status);
 }
 
 }  // namespace quic

@@ -182,7 +182,7 @@ SIGNATURES = {
     "quic_decode_persist_watch": (C.c_int, [C.POINTER(Model), C.POINTER(Decode), _P, _P, _I32, _P, _P]),
     "quic_decode_persist_status": (C.c_int, [_P, _P, C.POINTER(_I32)]),
     "quic_tree_attn": (C.c_int, [_P, _P, _P]),
-    "quic_tree_attn_scratch_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32, _I64]),
+    "quic_tree_attn_scratch_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I64]),
     "quic_block_tables": (C.c_int, [_P, _I64, _I32, _P, _P, _I32, _P, _P, _I32, _I32, _P, _I32, _P, _P, _P, _P, _I32, _I32, _P]),
     "quic_tree_commit": (C.c_int, [_P, _P]),
     "quic_qkv_rope_append_at": (C.c_int, [_P, _P, _P, _P, _P, _I32, _P, _P, _P, _I32, _I32, _I32, _P]),
@@ -741,8 +741,8 @@ _TREE_COMMIT = struct.Struct("=Q5qQq5Q10i4Q")       # quic_tree_commit_t
 
 
 @functools.lru_cache(maxsize=4096)
-def _tree_scratch_bytes(rows: int, requests: int, heads: int, kv_heads: int, dim: int, max_new: int, max_len: int) -> int:
-    return lib().quic_tree_attn_scratch_bytes(rows, requests, heads, kv_heads, dim, max_new, max_len)
+def _tree_scratch_bytes(requests: int, heads: int, kv_heads: int, dim: int, max_new: int, max_len: int) -> int:
+    return lib().quic_tree_attn_scratch_bytes(requests, heads, kv_heads, dim, max_new, max_len)
 
 
 def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor,
@@ -798,7 +798,7 @@ def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, table
     max_len = width * block if max_len is None else min(max_len, width * block)
     if max_new < 1 or max_len < 0:
         raise RuntimeError("tree_attn: max_new must be positive and max_len not negative")
-    need = _tree_scratch_bytes(rows, requests, heads, kv_heads, dim, max_new, max_len)
+    need = _tree_scratch_bytes(requests, heads, kv_heads, dim, max_new, max_len)
     stream = _raw_stream(device)
     scratch = _thread_scratch(("tree", device, stream), need, 1 << 20, 0).data_ptr() if need > 0 else None
     call = _TREE_ATTN.pack(q.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), out.data_ptr(), qs[0], qs[1], ks[0], ks[1], ks[2],

@@ -134,9 +134,9 @@ def test_nothing_to_do_is_no_error():
 
 def test_attention_scratch():
     size = K.lib().quic_tree_attn_scratch_bytes
-    assert size(1, 1, 14, 2, 64, 1, 64) == 0
-    assert size(1, 1, 14, 2, 64, 1, 8192) >= 14 * 2 * 66 * 4
-    assert size(1, 1, 15, 2, 64, 1, 8192) == 0
+    assert size(1, 14, 2, 64, 1, 64) == 0
+    assert size(1, 14, 2, 64, 1, 8192) >= 14 * 2 * 66 * 4
+    assert size(1, 15, 2, 64, 1, 8192) == 0
 
 
 def test_commit_entry_point_refuses():
