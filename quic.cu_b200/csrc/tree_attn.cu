@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
       if (c == 0) line[D] = l != l ? INFINITY : m_run[m][h], line[D + 1] = l;  // (a maximum passes over NaN)
     }
   __syncthreads();
-  const int64_t part = tree_part(a, blockIdx.z, kvh, tile, split);
+  const int64_t part = tree_part(a, blockIdx.z, kvh, tile) + split;
   for (int i = tid; i < kRows * (D / 4); i += kWarps * 32) {
     const int row = i % kRows, c4 = i / kRows;
     if (r0 + row >= all) continue;
@@ -343,32 +343,46 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
 
 // Rows whose keys several CTAs shared: sum of the parts, each by 2^(its maximum - the largest).  A CTA has 32 rows of a tile,
 // a row a lane, so that parts are read in whole lines; its four warps have a quarter of the head dimensions each.
-template <typename T, int D>
+template <typename T, int D, bool kTc>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a) {
   constexpr int kMine = D / 16;  // float4 of a thread
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y;
   const int per_tile = a.tile_rows / 32, tile = blockIdx.x / per_tile, row = blockIdx.x % per_tile * 32 + lane;
   const TreeRequest r = tree_request(a, blockIdx.z);
-  int per;
-  const int parts = tree_parts(a, r.end, per);
   const int all = min(r.n, a.max_new) * (int)a.group.d, number = tile * a.tile_rows + row;
   pdl_wait();
-  if (parts == 1 || number >= all) return;
-  const int64_t part = tree_part(a, blockIdx.z, kvh, tile, 0);
-  const float2* const ml = a.part_ml + part * a.tile_rows + row;
-  const float4* const po = a.part_o + (part * (D / 4) + warp * kMine) * a.tile_rows + row;
+  if (number >= all) return;
+  int parts;
+  int64_t part, step;  // the parts are part0, then part, part + step, ...
+  int64_t part0;
+  if constexpr (kTc) {  // the CTA where the row tile begins has it as its last segment, the others as their first
+    const TreeUnits u = tree_units(a, r);
+    const int64_t share = a.first[a.requests + 1], t0 = a.first[blockIdx.z] + ((int64_t)kvh * u.row_tiles + tile) * u.key_tiles;
+    const int64_t c0 = t0 / share, c1 = (t0 + u.key_tiles - 1) / share;
+    parts = (int)(c1 - c0) + 1;
+    part0 = 2 * c0 + 1, part = 2 * c0, step = 2;
+  } else {
+    int per;
+    parts = tree_parts(a, r.end, per);
+    part0 = part = tree_part(a, blockIdx.z, kvh, tile), step = 1;
+  }
+  if (parts == 1) return;
+  auto place = [&](int s) { return s == 0 ? part0 : part + s * step; };
+  const float2* const ml = a.part_ml + row;
+  const float4* const po = a.part_o + (int64_t)warp * kMine * a.tile_rows + row;
   float top = -INFINITY;
 #pragma unroll 8
-  for (int s = 0; s < parts; ++s) top = fmaxf(top, ml[(int64_t)s * a.tile_rows].x);
+  for (int s = 0; s < parts; ++s) top = fmaxf(top, ml[place(s) * a.tile_rows].x);
   const float ref = top == -INFINITY ? 0.f : top;
   float l = 0.f;
   float4 o[kMine] = {};
-#pragma unroll 2
+#pragma unroll 4
   for (int s = 0; s < parts; ++s) {
-    const float2 x = ml[(int64_t)s * a.tile_rows];
+    const int64_t at = place(s);
+    const float2 x = ml[at * a.tile_rows];
     float4 y[kMine];
 #pragma unroll
-    for (int c = 0; c < kMine; ++c) y[c] = po[((int64_t)s * (D / 4) + c) * a.tile_rows];
+    for (int c = 0; c < kMine; ++c) y[c] = po[(at * (D / 4) + c) * a.tile_rows];
     const float f = tree_ex2(x.x - ref);
     if (f != 0.f) {
       l += f * x.y;
@@ -393,26 +407,15 @@ int launch_few(const TreeArgs& a, cudaStream_t st) {
   return QUIC_OK;
 }
 
-template <typename T, int D>
-int launch_typed(const TreeArgs& a, bool tc, cudaStream_t st) {
-  const int rc = tc                ? tree_attn_tc_launch(a, kTreeExponent<T> == kTreeExponent<__nv_bfloat16>, D, st)
-                 : a.max_new * (int64_t)a.group.d <= 16 ? launch_few<T, D, 1>(a, st)
-                                   : launch_few<T, D, 2>(a, st);
-  if (rc != QUIC_OK || a.splits == 1) return rc;
-  QUIC_CUDA(launch(tree_merge_kernel<T, D>, dim3((unsigned)(a.tiles * (a.tile_rows / 32)), a.kv_heads, a.requests), dim3(128), 0, st,
-                   true, a));
-  return QUIC_OK;
-}
-
 constexpr int64_t kMostTokens = 1 << 29;  // of a request: sums of two counts stay within an int
 // Rows of a request and KV head beyond which the tcgen05 form takes a call.
 constexpr int64_t kFewRows = 32;
 
 struct Plan {
   bool tc;
-  int64_t tiles;                       // row tiles of a request and KV head
-  int tile_rows, splits, chunk;        // rows of one (a multiple of 32), CTAs that share its keys, the keys of one
-  int64_t parts(int requests, int kv_heads) const { return (int64_t)requests * kv_heads * tiles * splits * tile_rows; }
+  int64_t tiles;                   // row tiles of a request and KV head
+  int tile_rows, splits, chunk;    // rows of one (a multiple of 32); mma.sync form: CTAs that share its keys, the keys of one
+  int64_t parts;                   // partial results
 };
 // `bound`: keys of a request at most.
 Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound, int dim, bool tma) {
@@ -421,8 +424,13 @@ Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound
   p.tc = tma && rows > kFewRows;
   p.tile_rows = p.tc ? (int)(rows < kTreeTcRows ? (rows + 31) / 32 * 32 : kTreeTcRows) : 32;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+  p.splits = 1;
+  if (p.tc) {
+    p.parts = 2 * kTreeTcCtas;
+    return p;
+  }
   bound = bound < kMostTokens ? bound : kMostTokens;
-  const int64_t units = (int64_t)requests * kv_heads * p.tiles, slots = 148 * (!p.tc && dim == 64 ? 2 : 1);
+  const int64_t units = (int64_t)requests * kv_heads * p.tiles, slots = 148 * (dim == 64 ? 2 : 1);
   int64_t best = 1, least = INT64_MAX;
   for (int64_t s = 1; s <= 128 && (s == 1 || (s - 1) * 256 < bound); ++s) {
     const int64_t part = ((bound + s - 1) / s + 63) / 64 * 64;
@@ -433,7 +441,20 @@ Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound
   if (p.chunk < 64) p.chunk = 64;
   p.splits = (int)((bound + p.chunk - 1) / p.chunk);
   if (p.splits < 1) p.splits = 1;
+  p.parts = p.splits > 1 ? units * p.splits : 0;
   return p;
+}
+int64_t first_bytes(const Plan& p, int requests) { return p.tc ? ((int64_t)requests + 2 + 1) / 2 * 16 : 0; }
+
+template <typename T, int D>
+int launch_typed(const TreeArgs& a, const Plan& p, cudaStream_t st) {
+  const int rc = p.tc              ? tree_attn_tc_launch(a, kTreeExponent<T> == kTreeExponent<__nv_bfloat16>, D, st)
+                 : a.max_new * (int64_t)a.group.d <= 16 ? launch_few<T, D, 1>(a, st)
+                                   : launch_few<T, D, 2>(a, st);
+  if (rc != QUIC_OK || p.parts == 0) return rc;
+  const dim3 grid((unsigned)(a.tiles * (a.tile_rows / 32)), a.kv_heads, a.requests);
+  QUIC_CUDA(launch(p.tc ? tree_merge_kernel<T, D, true> : tree_merge_kernel<T, D, false>, grid, dim3(128), 0, st, true, a));
+  return QUIC_OK;
 }
 
 }  // namespace
@@ -447,7 +468,7 @@ extern "C" int64_t quic_tree_attn_scratch_bytes(int32_t requests, int32_t heads,
   int64_t most = 0;  // (by either form: strides decide)
   for (int tma = 0; tma < 2; ++tma) {
     const Plan p = make_plan(requests, kv_heads, heads, max_new, max_len + max_new, dim, tma != 0);
-    const int64_t need = p.splits > 1 ? p.parts(requests, kv_heads) * (dim + 2) * 4 : 0;
+    const int64_t need = first_bytes(p, requests) + p.parts * p.tile_rows * (dim + 2) * 4;
     most = need > most ? need : most;
   }
   return most;
@@ -478,7 +499,7 @@ extern "C" int quic_tree_attn(const quic_tree_attn_t* t, void* scratch, void* st
                "tree_attn: more than 65535 requests, or row tiles of one");
   TreeArgs a = {};
   a.splits = p.splits, a.chunk = p.chunk, a.tiles = (int)p.tiles, a.tile_rows = p.tile_rows;
-  QUIC_REQUIRE(a.splits == 1 || (scratch != nullptr && (uintptr_t)scratch % 16 == 0), QUIC_E_ARG,
+  QUIC_REQUIRE(p.parts == 0 || (scratch != nullptr && (uintptr_t)scratch % 16 == 0), QUIC_E_ARG,
                "tree_attn: scratch missing or not 16-byte aligned");
   a.q = t->q, a.k = t->k, a.v = t->v, a.out = t->out;
   a.q_row = t->q_row, a.q_head = t->q_head;
@@ -487,8 +508,9 @@ extern "C" int quic_tree_attn(const quic_tree_attn_t* t, void* scratch, void* st
   a.table_row = t->table_row, a.mask_row = t->mask_row;
   a.tables = t->tables, a.lengths = t->lengths, a.row_start = t->row_start;
   a.mask = (const uint32_t*)t->mask, a.mask_words = t->mask_words;
-  a.part_o = (float4*)scratch;
-  a.part_ml = (float2*)(a.part_o + p.parts(t->requests, t->kv_heads) * (t->dim / 4));
+  a.first = (int64_t*)scratch;
+  a.part_o = (float4*)((char*)scratch + first_bytes(p, t->requests));
+  a.part_ml = (float2*)(a.part_o + p.parts * p.tile_rows * (t->dim / 4));
   a.block = FastDiv::of((uint32_t)t->block_size);
   a.group = FastDiv::of((uint32_t)(t->heads / t->kv_heads));
   a.rows = t->rows, a.requests = t->requests, a.heads = t->heads, a.kv_heads = t->kv_heads;
@@ -496,6 +518,6 @@ extern "C" int quic_tree_attn(const quic_tree_attn_t* t, void* scratch, void* st
   a.scale_log2 = (t->scale > 0.f ? t->scale : 1.f / sqrtf((float)t->dim)) * 1.4426950408889634f;
   cudaStream_t st = (cudaStream_t)stream;
   if (t->dtype == QUIC_DTYPE_F16)
-    return t->dim == 64 ? launch_typed<half, 64>(a, p.tc, st) : launch_typed<half, 128>(a, p.tc, st);
-  return t->dim == 64 ? launch_typed<__nv_bfloat16, 64>(a, p.tc, st) : launch_typed<__nv_bfloat16, 128>(a, p.tc, st);
+    return t->dim == 64 ? launch_typed<half, 64>(a, p, st) : launch_typed<half, 128>(a, p, st);
+  return t->dim == 64 ? launch_typed<__nv_bfloat16, 64>(a, p, st) : launch_typed<__nv_bfloat16, 128>(a, p, st);
 }

@@ -25,12 +25,13 @@ struct TreeArgs {
   int64_t q_row, q_head, k_block, k_head, k_tok, v_block, v_head, v_tok, table_row, mask_row;
   const int32_t *tables, *lengths, *row_start;
   const uint32_t* mask;              // [rows][mask_words] by mask_row, or nullptr: node i sees nodes 0 .. i
-  float4* part_o;                    // [requests][kv heads][tiles][splits][dim / 4][tile_rows]
-  float2* part_ml;                   // [requests][kv heads][tiles][splits][tile_rows]: maximum (base 2), sum
+  float4* part_o;                    // partial results [parts][dim / 4][tile_rows]
+  float2* part_ml;                   // [parts][tile_rows]: maximum (base 2), sum
+  int64_t* first;                    // tcgen05 form: key tiles of the requests before each and of all, then a CTA's share
   FastDiv block, group;              // tokens per block, query heads per KV head
   int32_t rows, requests, heads, kv_heads, n_blocks, max_blocks, mask_words, max_new;
-  int32_t tiles, tile_rows;          // row tiles of a request and KV head, rows of one
-  int32_t splits, chunk;             // CTAs per request, KV head and row tile at most; the tokens of one
+  int32_t tiles, tile_rows;          // row tiles of a request and KV head at most, rows of one
+  int32_t splits, chunk;             // mma.sync form: CTAs per request, KV head and row tile at most; the tokens of one
   float scale_log2;
 };
 
@@ -49,16 +50,33 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeArgs& a, int b) {
   r.end = (int)min((int64_t)r.len + r.n, room);
   return r;
 }
-// How many CTAs share a request's keys, and the keys of each: equal parts, whole tiles of 64.
+// mma.sync form: how many CTAs share a request's keys, and the keys of each: equal parts, whole tiles of 64.
 __device__ __forceinline__ int tree_parts(const TreeArgs& a, int end, int& per) {
   const int parts = max(1, min(a.splits, (end + a.chunk - 1) / a.chunk));
   per = ((end + parts - 1) / parts + 63) & ~63;
   return per > 0 ? (end + per - 1) / per : 1;
 }
 
-// A row tile's part number `split` of the partial results.
-__device__ __forceinline__ int64_t tree_part(const TreeArgs& a, int b, int kvh, int tile, int split) {
-  return (((int64_t)b * a.kv_heads + kvh) * a.tiles + tile) * a.splits + split;
+// ... and the first part of a row tile in the partial results.
+__device__ __forceinline__ int64_t tree_part(const TreeArgs& a, int b, int kvh, int tile) {
+  return (((int64_t)b * a.kv_heads + kvh) * a.tiles + tile) * a.splits;
+}
+
+// tcgen05 form: the work is a line of key tiles (64 keys of one row tile), request after request, KV head after KV head, row
+// tile after row tile; every CTA has an equal share of the line.  A row tile's tiles that one CTA has are a segment.
+constexpr int kTreeTcRows = 256, kTreeTcKeys = 64, kTreeTcCtas = 148;
+struct TreeUnits {   // of a request
+  int rows;          // (node, head) pairs per KV head
+  int row_tiles;
+  int key_tiles;     // of each row tile; one without keys writes zeros
+  __device__ __forceinline__ int64_t all(const TreeArgs& a) const { return (int64_t)row_tiles * a.kv_heads * key_tiles; }
+};
+__device__ __forceinline__ TreeUnits tree_units(const TreeArgs& a, const TreeRequest& r) {
+  TreeUnits u;
+  u.rows = min(r.n, a.max_new) * (int)a.group.d;
+  u.row_tiles = (u.rows + kTreeTcRows - 1) / kTreeTcRows;
+  u.key_tiles = max(1, (r.end + kTreeTcKeys - 1) / kTreeTcKeys);
+  return u;
 }
 
 // Which of the 32 positions from t on node `node` sees, the positions up to `end` taken for present: bit j for t + j.
@@ -133,8 +151,7 @@ constexpr float kTreeShift = 0.f;
 template <>
 constexpr float kTreeShift<half> = 8.f;
 
-// The throughput form (tree_attn_tc.cu) has 256 rows of a request and KV head a CTA, and takes what TMA can fetch.
-constexpr int kTreeTcRows = 256;
+// The throughput form (tree_attn_tc.cu) takes what TMA can fetch.
 bool tree_attn_tc_takes(int block_size, int64_t k_block, int64_t k_head, int64_t k_tok, int64_t v_block, int64_t v_head, int64_t v_tok);
 int tree_attn_tc_launch(const TreeArgs& a, bool bf16, int dim, cudaStream_t stream);
 

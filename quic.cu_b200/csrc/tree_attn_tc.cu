@@ -28,8 +28,9 @@ namespace quic {
 namespace {
 
 constexpr int kRows = 128, kKeys = 64, kGroupWarps = 4, kSoftmaxWarps = 2 * kGroupWarps;
-constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
-static_assert(2 * kRows == kTreeTcRows, "two streams of rows");
+constexpr int kTmaWarp = kSoftmaxWarps + 2, kThreads = (kTmaWarp + 1) * 32;
+constexpr int kLeastShare = 4;  // key tiles of a CTA
+static_assert(2 * kRows == kTreeTcRows && kKeys == kTreeTcKeys, "two streams of rows");
 constexpr float kGrowth = 8.f;    // of a row's maximum (base 2) before its reference point follows
 template <typename T>
 constexpr float kShift = 0.f;     // P = 2^(score - reference + shift)
@@ -95,26 +96,57 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Whether the phase is complete, at once (a try_wait may sleep).
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
-}
+// Barrier 1: the softmax warps.
+__device__ __forceinline__ void softmax_barrier() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory"); }
 
 template <int D>
 constexpr int kStages = D == 64 ? 8 : 5;
 template <int D>
 constexpr uint32_t kTcSmem = (D / 64) * (2 * kHalfQ + kStages<D> * 2 * kHalfK) + 1024;  // Q of both streams, stages of K and V
 static_assert(kTcSmem<128> + 1024 <= 232448 && kTcSmem<64> > 115 * 1024, "one CTA fills an SM: it takes all tensor memory");
-// O of a stream (fp32), and behind it the results of both (16 bits), lie in the stages at the end
-static_assert(kRows * 64 * (4 + 2 * 2) <= kStages<64> * 2 * kHalfK && kRows * 128 * (4 + 2 * 2) <= 2 * kStages<128> * 2 * kHalfK, "stages");
+
+// A CTA's way through its share of the line of key tiles.
+struct Segment {
+  TreeRequest r;
+  int b, kvh, r0, rows;             // request, KV head, first row of the row tile, rows of the request
+  int tile0, n_tiles, key_tiles;    // key tiles of the row tile: the first of the segment, their number, all
+  bool halves;                      // two streams of rows, or of key tiles
+  __device__ __forceinline__ int steps(int g) const { return halves ? n_tiles : (n_tiles + 1 - g) / 2; }
+  __device__ __forceinline__ int step_tile(int g, int k) const { return halves ? k : 2 * k + g; }
+  __device__ __forceinline__ int warps(int g) const {  // of a stream that have rows
+    return max(0, min((rows - r0 - (halves ? g * kRows : 0) + 31) / 32, kGroupWarps));
+  }
+  __device__ __forceinline__ int begin() const { return tile0 * kKeys; }
+  __device__ __forceinline__ int end() const { return min((tile0 + n_tiles) * kKeys, r.end); }
+};
+struct Walk {
+  int b;
+  int64_t at, left;  // tile of the request, tiles still to do
+  __device__ __forceinline__ bool next(const TreeArgs& a, Segment& s) {
+    while (left > 0) {
+      s.r = tree_request(a, b);
+      const TreeUnits u = tree_units(a, s.r);
+      if (u.rows == 0) {
+        ++b;
+        continue;
+      }
+      const int64_t unit = at / u.key_tiles;
+      s.b = b;
+      s.kvh = (int)(unit / u.row_tiles);
+      s.r0 = (int)(unit % u.row_tiles) * kTreeTcRows;
+      s.rows = u.rows;
+      s.halves = u.rows - s.r0 > kRows;
+      s.key_tiles = u.key_tiles;
+      s.tile0 = (int)(at % u.key_tiles);
+      s.n_tiles = (int)min(left, (int64_t)(u.key_tiles - s.tile0));
+      at += s.n_tiles;
+      left -= s.n_tiles;
+      if (at == u.all(a)) ++b, at = 0;
+      return true;
+    }
+    return false;
+  }
+};
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k,
@@ -126,387 +158,420 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kRing], bar_empty[kRing], bar_s[2][2], bar_p[2][2], bar_o[2][2], bar_q, bar_drain;
   __shared__ uint32_t valid_s[kRing];  // which boxes of the stage have a block
-  __shared__ float2 other_s[kRows];
+  __shared__ float2 other_s[kRows];    // maximum and sum of stream 1, where the streams share rows
+  __shared__ int64_t sums_s[kThreads / 32];
+  __shared__ Walk walk_s;
   __shared__ uint32_t tmem_base_s;
-  __shared__ int fail_s, odd_s;  // odd_s: the first tile in which V held what is not finite
+  __shared__ int fail_s, odd_s[2];  // odd_s: the first tile of an even, odd segment in which V held what is not finite
 
   const TreeArgs& a = args.t;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int tile = blockIdx.x % a.tiles, split = blockIdx.x / a.tiles, kvh = blockIdx.y;
-  const TreeRequest r = tree_request(a, blockIdx.z);
-  const int all = min(r.n, a.max_new) * (int)a.group.d, r0 = tile * 2 * kRows;
-  if (r0 >= all) return;
-  int per;
-  const int parts = tree_parts(a, r.end, per);
-  if (split >= parts) return;
-  const int t_begin = split * per, t_end = min(t_begin + per, r.end);
-  const int n_tiles = (t_end - t_begin + kKeys - 1) / kKeys;
-  const bool halves = all - r0 > kRows;  // two streams of rows, or of key tiles
-  const int items = halves ? 2 * n_tiles : n_tiles;  // item j: step j / 2 of stream j % 2
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* const smem = smem_raw + (base - smem_u32(smem_raw));
-  auto warps_of = [&](int g) { return min((all - r0 - (halves ? g * kRows : 0) + 31) / 32, kGroupWarps); };  // with rows
 
-  if (tid == 0) {
-    for (int s = 0; s < kRing; ++s) {
-      mbar_init(smem_u32(&bar_full[s]), 1);
-      mbar_init(smem_u32(&bar_empty[s]), 1);
+  // ---- the line of key tiles, and where in it this CTA begins
+  {
+    const int each = (a.requests + kThreads - 1) / kThreads, b0 = min(tid * each, a.requests), b1 = min(b0 + each, a.requests);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += tree_units(a, tree_request(a, b)).all(a);
+    int64_t before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += y;
     }
-    for (int g = 0; g < 2; ++g)
-      for (int x = 0; x < 2; ++x) {
-        mbar_init(smem_u32(&bar_s[g][x]), 1);
-        mbar_init(smem_u32(&bar_p[g][x]), warps_of(g));
-        mbar_init(smem_u32(&bar_o[g][x]), 1);
+    if (lane == 31) sums_s[warp] = before;
+    before -= mine;
+    if (warp == kTmaWarp && lane == 0) {
+      for (int s = 0; s < kRing; ++s) {
+        mbar_init(smem_u32(&bar_full[s]), 1);
+        mbar_init(smem_u32(&bar_empty[s]), 2);
       }
-    mbar_init(smem_u32(&bar_q), kSoftmaxWarps);
-    mbar_init(smem_u32(&bar_drain), 1);
-    fail_s = 0;
-    odd_s = 0x7fffffff;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == kSoftmaxWarps) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  } else if (warp < kSoftmaxWarps) {  // queries; rows that are none are zero
-    const int rows = halves ? 2 * kRows : kRows;
-#pragma unroll 4
-    for (int i = tid; i < rows * (D / 8); i += kSoftmaxWarps * 32) {
-      const int row = i / (D / 8), chunk = i % (D / 8), number = min(r0 + row, all - 1);
-      const int node = (int)a.group.div(number), head = kvh * (int)a.group.d + number - node * (int)a.group.d;
-      copy16(base + (row / kRows) * kQ + (chunk >> 3) * kHalfQ + sw128_offset(row % kRows, chunk & 7),
-             reinterpret_cast<const T*>(a.q) + (int64_t)(r.start + node) * a.q_row + (int64_t)head * a.q_head + 8 * chunk,
-             r0 + row < all ? 16u : 0u);
+      for (int g = 0; g < 2; ++g)
+        for (int x = 0; x < 2; ++x) {
+          mbar_init(smem_u32(&bar_s[g][x]), 1);
+          mbar_init(smem_u32(&bar_p[g][x]), kGroupWarps);
+          mbar_init(smem_u32(&bar_o[g][x]), 1);
+        }
+      mbar_init(smem_u32(&bar_q), kSoftmaxWarps);
+      mbar_init(smem_u32(&bar_drain), 2);
+      fail_s = 0;
+      odd_s[0] = odd_s[1] = 0x7fffffff;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += sums_s[w];
+      total += sums_s[w];
+    }
+    const int64_t share = max((int64_t)kLeastShare, (total + kTreeTcCtas - 1) / kTreeTcCtas), start = blockIdx.x * share;
+    if (blockIdx.x == 0) {  // for the merge
+      int64_t sum = before;
+      for (int b = b0; b < b1; ++b) {
+        a.first[b] = sum;
+        sum += tree_units(a, tree_request(a, b)).all(a);
+      }
+      if (tid == 0) a.first[a.requests] = total, a.first[a.requests + 1] = share;
+    }
+    if (start >= total) return;
+    if (before <= start && start < before + mine) {
+      int b = b0;
+      for (int64_t n; (n = tree_units(a, tree_request(a, b)).all(a)) <= start - before; ++b) before += n;
+      walk_s.b = b;
+      walk_s.at = start - before;
+      walk_s.left = min(share, total - start);
+    }
+    if (warp == kSoftmaxWarps) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(kTmemCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
   const uint32_t tmem = tmem_base_s;
-
+  Walk walk = walk_s;
+  Segment s;
+  int ring = 0;  // tiles of the segments before
   bool issuer = false;
-  // what a softmax thread has at the end
-  const int group = warp / kGroupWarps, quarter = warp % kGroupWarps;
-  float m_run = -INFINITY, l_run = 0.f;
-  int steps = 0;
-  if (warp > kSoftmaxWarps) {
+
+  if (warp == kTmaWarp) {
     // ---------------- TMA: a lane a box of 64 dims of K or V ----------------
     const int boxes = 1 << args.log_boxes, box = lane & (boxes - 1), what = lane >> args.log_boxes;
     const bool copies = what < 2 * kHalves;
     const CUtensorMap* const map = what & 1 ? &tm_v : &tm_k;
     const uint32_t dst = base + kK + (what & 1) * kTile + (what >> 1) * kHalfK + box * args.box * 128;
-    const int32_t* table = a.tables + (int64_t)blockIdx.z * a.table_row;
     if (lane < 2) tma_prefetch_desc(lane ? &tm_v : &tm_k);
-    auto place = [&](int i) { return t_begin + i * kKeys + box * args.box; };
-    auto fetch = [&](int i) {  // the block of this lane's box of tile i, n_blocks (beyond the planes) where there is none
-      const int p = place(i), id = p < t_end ? __ldg(table + a.block.div(p)) : -1;
-      return id >= 0 && id < a.n_blocks ? id : a.n_blocks;
-    };
-    int id = fetch(0), next = fetch(1);
-    for (int i = 0; i < n_tiles; ++i) {
-      const int st = i % kRing, after = fetch(i + 2);
-      if (i >= kRing && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_empty[st]), (i / kRing - 1) & 1, args.wait_limit_us))) {
-        fail_s = 2;
-        break;
+    bool ok = true;
+    while (ok && walk.next(a, s)) {
+      const int32_t* table = a.tables + (int64_t)s.b * a.table_row;
+      const int t_begin = s.begin(), t_end = s.end();
+      auto fetch = [&](int i) {  // the block of this lane's box of tile i, n_blocks (beyond the planes) where there is none
+        const int p = t_begin + i * kKeys + box * args.box, id = p < t_end ? __ldg(table + a.block.div(p)) : -1;
+        return id >= 0 && id < a.n_blocks ? id : a.n_blocks;
+      };
+      int id = fetch(0), next = fetch(1);
+      for (int i = 0; i < s.n_tiles; ++i, ++ring) {
+        const int st = ring % kRing, after = fetch(i + 2);
+        if (ring >= kRing && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_empty[st]), (ring / kRing - 1) & 1, args.wait_limit_us))) {
+          fail_s = 2;
+          ok = false;
+          break;
+        }
+        if (args.skip_tile < -1) pause_us(-args.skip_tile);
+        const uint32_t there = __ballot_sync(0xffffffffu, id < a.n_blocks) & (0xffffffffu >> (32 - boxes));
+        const uint32_t full = smem_u32(&bar_full[st]);
+        if (lane == 0) {
+          valid_s[st] = there;
+          mbar_expect_tx(full, kStage);
+        }
+        __syncwarp();
+        const int p = t_begin + i * kKeys + box * args.box;
+        if (copies && (ring != args.skip_tile || (what & 1)))
+          tma_load_4d(dst + st * kStage, map, 64 * (what >> 1), p - (int)a.block.div(p) * (int)a.block.d, s.kvh, id, full);
+        id = next;
+        next = after;
       }
-      if (args.skip_tile < -1) pause_us(-args.skip_tile);
-      const uint32_t there = __ballot_sync(0xffffffffu, id < a.n_blocks) & (0xffffffffu >> (32 - boxes));
-      const uint32_t full = smem_u32(&bar_full[st]);
-      if (lane == 0) {
-        valid_s[st] = there;
-        mbar_expect_tx(full, kStage);
-      }
-      __syncwarp();
-      const int p = place(i);
-      if (copies && (i != args.skip_tile || (what & 1)))
-        tma_load_4d(dst + st * kStage, map, 64 * (what >> 1), p - (int)a.block.div(p) * (int)a.block.d, kvh, id, full);
-      id = next;
-      next = after;
     }
-  } else if (warp == kSoftmaxWarps) {
-    // ---------------- MMA issuer: a warp in step, one lane of which issues ----------------
+  } else if (warp >= kSoftmaxWarps) {
+    // ---------------- MMA issuers, one per stream: a warp in step, one lane of which issues ----------------
+    const int g = warp - kSoftmaxWarps;
     issuer = elect_one();
     const uint64_t q0 = umma_desc_sw128(base), k0 = umma_desc_sw128(base + kK);
     // V: head dims contiguous, the two halves of 128 dims kHalfK apart (leading byte offset)
     const uint64_t v0 = umma_desc_sw128(base + kK + kTile) + ((uint64_t)(kHalfK / 16 - 1) << 16);
     constexpr uint32_t kType = kTreeExponent<T> == kTreeExponent<__nv_bfloat16> ? (1u << 7) | (1u << 10) : 0u;  // bf16 x bf16
-    const uint32_t idesc = umma_idesc_f16(kKeys) | kType;        // M = 128, N = 64
+    const uint32_t idesc = umma_idesc_f16(kKeys) | kType;             // M = 128, N = 64
     const uint32_t idesc_v = umma_idesc_f16(D) | kType | (1u << 16);  // N = the head dims, B transposed
-    int next_s = 0, next_p = 0, idle = 0;
-    uint32_t since = 0;
-    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_q), 0, args.wait_limit_us))) {
-      fail_s = 3;
-      next_p = items;
-    }
-    while (next_p < items) {
-      bool moved = false;
-      if (next_s < items && next_s < next_p + 4) {  // (the buffer's last P is with the product of item next_s - 4)
-        const int g = next_s & 1, u = next_s >> 1, i = halves ? u : next_s, st = i % kRing;
-        if (__all_sync(0xffffffffu, mbar_test(smem_u32(&bar_full[st]), (i / kRing) & 1) &&
-                                        (u < 2 || mbar_test(smem_u32(&bar_o[g][u & 1]), ((u >> 1) - 1) & 1)))) {
-          tc_fence_after();
-          const uint64_t q = q0 + (uint64_t)((halves ? g : 0) * (kQ / 16)), kt = k0 + (uint64_t)(st * (kStage / 16));
-          const uint32_t to = tmem + 128u * g + 64u * (u & 1), bar = smem_u32(&bar_s[g][u & 1]);
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              umma_f16(to, q + (uint64_t)((k >> 2) * (kHalfQ / 16)) + 2 * (k & 3), kt + (uint64_t)((k >> 2) * (kHalfK / 16)) + 2 * (k & 3),
-                       idesc, k > 0 ? 1u : 0u);
-            umma_commit(bar);
-          }
-          __syncwarp();
-          ++next_s;
-          moved = true;
-        }
-      }
-      if (next_p < next_s) {
-        const int g = next_p & 1, u = next_p >> 1, i = halves ? u : next_p, st = i % kRing;
-        if (__all_sync(0xffffffffu, mbar_test(smem_u32(&bar_p[g][u & 1]), (u >> 1) & 1))) {  // P is there, O rescaled where need be
-          tc_fence_after();
-          const uint64_t vt = v0 + (uint64_t)(st * (kStage / 16));
-          const uint32_t to = tmem + kColO + 128u * g, from = tmem + 128u * g + 64u * (u & 1), bar = smem_u32(&bar_o[g][u & 1]);
-          const uint32_t free = smem_u32(&bar_empty[st]), more = u > 0 ? 1u : 0u;
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)  // sixteen tokens a step: two groups of eight rows of the V tile, eight columns of P
-              umma_ts(to, from + 8u * k, vt + k * (2048 / 16), idesc_v, k > 0 ? 1u : more);
-            umma_commit(bar);
-            if (!halves || g == 1) umma_commit(free);
-          }
-          __syncwarp();
-          ++next_p;
-          moved = true;
-        }
-      }
-      if (moved) {
-        idle = 0;
-      } else if ((++idle & 63) == 0) {
-        const uint32_t now = __shfl_sync(0xffffffffu, clock_us(), 0);
-        if (idle == 64) since = now;
-        else if (now - since >= args.wait_limit_us) {
-          fail_s = 3;
-          break;
-        }
-      }
-    }
-  } else {
-    // ---------------- softmax ----------------
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    fence_proxy_async();
-    __syncwarp();
-    if (lane == 0) mbar_arrive_cta(smem_u32(&bar_q));
-  }
-  if (warp < kSoftmaxWarps && quarter < warps_of(group)) {
-    const int mine = min(r0 + (halves ? group * kRows : 0) + 32 * quarter + lane, all - 1), node = (int)a.group.div(mine);
-    const uint32_t lane_addr = (uint32_t)(32 * quarter) << 16;
-    const uint32_t at_o = tmem + kColO + 128u * group + lane_addr;
-    const uint32_t limit = 2 * args.wait_limit_us;  // (the issuer and the loaders give up first)
-    const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2);
-    steps = halves ? n_tiles : (n_tiles + 1 - group) / 2;
+    const uint32_t at_s = tmem + 128u * g, at_o = tmem + kColO + 128u * g;
+    auto wait = [&](uint64_t* bar, int parity) {
+      return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, args.wait_limit_us)) != 0;
+    };
+    int u = 0;  // steps of the segments before
     bool ok = true;
-    for (int u = 0; u < steps; ++u) {
-      const int i = halves ? u : 2 * u + group, st = i % kRing, t = t_begin + i * kKeys;
-      const uint32_t at_s = tmem + 128u * group + 64u * (u & 1) + lane_addr;
-      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_s[group][u & 1]), (u >> 1) & 1, limit));
-      // (complete: for what the loaders wrote, which this thread reads itself)
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_full[st]), (i / kRing) & 1, limit));
-      if (!ok) break;
-      tc_fence_after();
-      float s[64];
-      tmem_ld_cols<64>(at_s, s);
-      const uint32_t there = valid_s[st];
-      const bool tree = t + kKeys > r.len;
-      if (tree) {  // (the same for all the CTA's rows)
-        unsigned char* const v_tile = smem + kK + st * kStage + kTile;
-        bool odd = false, changed = false;
-        for (int c = 32 * quarter + lane; c < (int)kTile / 16; c += 32 * warps_of(group)) {
-          uint4 w = reinterpret_cast<const uint4*>(v_tile)[c];
-          if (tree_not_finite<T>(w.x) || tree_not_finite<T>(w.y) || tree_not_finite<T>(w.z) || tree_not_finite<T>(w.w)) {
-            w.x = tree_finite<T>(w.x), w.y = tree_finite<T>(w.y), w.z = tree_finite<T>(w.z), w.w = tree_finite<T>(w.w);
-            reinterpret_cast<uint4*>(v_tile)[c] = w;
-            odd |= t + (c % (kKeys * 8)) / 8 < t_end;  // (rows behind the last key may hold anything)
-            changed = true;
-          }
+    for (int seg = 0; ok && walk.next(a, s); ++seg) {
+      const int steps = s.steps(g);
+      const uint64_t q = q0 + (uint64_t)((s.halves ? g : 0) * (kQ / 16));
+      auto scores = [&](int k) {
+        const int n = ring + s.step_tile(g, k), st = n % kRing, x = (u + k) & 1;
+        if (!wait(&bar_full[st], (n / kRing) & 1)) return false;
+        // the product that read the buffer's last P is complete
+        if (u + k >= 2 && !wait(&bar_o[g][x], (((u + k) >> 1) - 1) & 1)) return false;
+        tc_fence_after();
+        const uint64_t kt = k0 + (uint64_t)(st * (kStage / 16));
+        const uint32_t to = at_s + 64u * x, bar = smem_u32(&bar_s[g][x]);
+        if (elect_one()) {
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c)
+            umma_f16(to, q + (uint64_t)((c >> 2) * (kHalfQ / 16)) + 2 * (c & 3), kt + (uint64_t)((c >> 2) * (kHalfK / 16)) + 2 * (c & 3),
+                     idesc, c > 0 ? 1u : 0u);
+          umma_commit(bar);
         }
-        if (changed) fence_proxy_async();
-        if (odd) atomicMin(&odd_s, i);
         __syncwarp();
-      }
-      if (tree || there != (0xffffffffu >> (32 - (1 << args.log_boxes)))) {
-        uint32_t seen0 = tree_visible32(a, r, node, t), seen1 = tree_visible32(a, r, node, t + 32);
-        const int left = t_end - t;
-        if (left < 64) {
-          seen0 &= left < 32 ? (1u << max(left, 0)) - 1u : 0xffffffffu;
-          seen1 &= left < 32 ? 0u : (1u << (left - 32)) - 1u;
-        }
-        if (there != (0xffffffffu >> (32 - (1 << args.log_boxes)))) {
-          for (int j = 0; j < 32; ++j) {
-            if (!(there >> (j / args.box) & 1u)) seen0 &= ~(1u << j);
-            if (!(there >> ((j + 32) / args.box) & 1u)) seen1 &= ~(1u << j);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          if (!(seen0 >> j & 1u)) s[j] = -INFINITY;
-          if (!(seen1 >> j & 1u)) s[32 + j] = -INFINITY;
-        }
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // independent chains
-#pragma unroll
-      for (int j = 0; j < 64; j += 2) mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], s[j], s[j + 1]);
-      const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;  // (the scale is positive)
-      const bool grown = mt > m_run + kGrowth;  // (from -inf: by any score)
-      if (u == 0) {
-        m_run = mt;
-      } else if (__any_sync(0xffffffffu, grown)) {
-        const float alpha = grown ? tree_ex2(m_run - mt) : 1.f;
-        if (grown) m_run = mt;
-        l_run *= alpha;
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_o[group][(u - 1) & 1]), ((u - 1) >> 1) & 1, limit));
+        return true;
+      };
+      ok = wait(&bar_q, seg & 1) && (steps == 0 || scores(0));
+      for (int k = 0; ok && k < steps; ++k) {
+        const int n = ring + s.step_tile(g, k), st = n % kRing, x = (u + k) & 1;
+        ok = (k + 1 == steps || scores(k + 1)) && wait(&bar_p[g][x], ((u + k) >> 1) & 1);  // P is there, O rescaled where need be
         if (!ok) break;
         tc_fence_after();
+        const uint64_t vt = v0 + (uint64_t)(st * (kStage / 16));
+        const uint32_t from = at_s + 64u * x, bar = smem_u32(&bar_o[g][x]), free = smem_u32(&bar_empty[st]);
+        const uint32_t more = k > 0 ? 1u : 0u;
+        if (elect_one()) {
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          float v[16];
-          uint32_t w[16];
-          tmem_ld_cols<16>(at_o + 16u * c, v);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[j] * alpha);
-          tmem_st16(at_o + 16u * c, w);
+          for (int c = 0; c < 4; ++c)  // sixteen tokens a step: two groups of eight rows of the V tile, eight columns of P
+            umma_ts(at_o, from + 8u * c, vt + c * (2048 / 16), idesc_v, c > 0 ? 1u : more);
+          umma_commit(bar);
+          umma_commit(free);
+          if (!s.halves) umma_commit(free);  // (nobody else reads the tile)
         }
+        __syncwarp();
       }
-      const float ref = kShift<T> - (m_run == -INFINITY ? 0.f : m_run);
-      const uint64_t ref2 = pair2(ref, ref);
-      uint64_t l2[2] = {0ull, 0ull};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float p0, p1;
-          unpair2(fma2(pair2(s[32 * h + 2 * j], s[32 * h + 2 * j + 1]), scale2, ref2), p0, p1);
-          p0 = tree_ex2(p0);  // 2^-inf = 0 for keys that are not seen
-          p1 = tree_ex2(p1);
-          w[j] = tree_pack<T>(p0, p1);
-          l2[j & 1] = add2(l2[j & 1], pair2(p0, p1));
-        }
-        tmem_st16(at_s + 16u * h, w);  // (P in the scores' own columns: they have all been read)
-      }
-      float la, lb;
-      unpair2(add2(l2[0], l2[1]), la, lb);
-      l_run += la + lb;
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cta(smem_u32(&bar_p[group][u & 1]));
+      u += steps;
+      ring += s.n_tiles;
     }
-    if (ok && steps > 0)
-      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_o[group][(steps - 1) & 1]), ((steps - 1) >> 1) & 1, limit));
-    if (!ok && fail_s == 0) fail_s = 1;
-    if (l_run != l_run) m_run = INFINITY;  // (a maximum passes over NaN)
-  }
-  __syncwarp();
-  tc_fence_before();
-  __syncthreads();  // every product is complete, every copy landed
-  tc_fence_after();
-  const bool failed = fail_s != 0;
-  pdl_launch_dependents();
+    if (!ok) fail_s = 3;
+  } else {
+    // ---------------- queries, softmax, epilogue ----------------
+    const int group = warp / kGroupWarps, quarter = warp % kGroupWarps;
+    const uint32_t lane_addr = (uint32_t)(32 * quarter) << 16;
+    const uint32_t at_o = tmem + kColO + 128u * group + lane_addr;
+    const uint32_t limit = 2 * args.wait_limit_us;  // (the issuers and the TMA warp give up first)
+    const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2);
+    int u0 = 0;  // steps of the segments before
+    bool ok = true;  // (without it a warp goes on to the end, past all waits, for the barriers of the segments)
+    for (int seg = 0; walk.next(a, s); ++seg) {
+      const int t_begin = s.begin(), t_end = s.end(), steps = s.steps(group);
+      // ---- queries of the stream's rows (the first stream's, where they are the same); rows that are none are zero
+      if (s.halves || group == 0) {
+#pragma unroll 4
+        for (int i = lane; i < 32 * (D / 8); i += 32) {  // (a warp its own rows: in their place it gathers its results)
+          const int row = 32 * quarter + i / (D / 8), chunk = i % (D / 8);
+          const int number = s.r0 + group * kRows + row, mine = min(number, s.rows - 1);
+          const int node = (int)a.group.div(mine), head = s.kvh * (int)a.group.d + mine - node * (int)a.group.d;
+          copy16(base + group * kQ + (chunk >> 3) * kHalfQ + sw128_offset(row, chunk & 7),
+                 reinterpret_cast<const T*>(a.q) + (int64_t)(s.r.start + node) * a.q_row + (int64_t)head * a.q_head + 8 * chunk,
+                 number < s.rows ? 16u : 0u);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cta(smem_u32(&bar_q));
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_q), seg & 1, limit));
+      if (tid == 0) odd_s[(seg + 1) & 1] = 0x7fffffff;  // (all are through with the segment before, none with this)
 
-  // ---------------- epilogue: the streams of key tiles meet in shared memory ----------------
-  const bool has_rows = warp < kSoftmaxWarps && quarter < warps_of(group) && !failed;
-  const uint32_t at_o = tmem + kColO + 128u * group + ((uint32_t)(32 * quarter) << 16);
-  float4* const other_o = reinterpret_cast<float4*>(smem + kK);  // [D / 4][128 rows]
-  if (!halves && has_rows && group == 1) {
-    const int row = 32 * quarter + lane;
-    other_s[row] = make_float2(m_run, l_run);
-#pragma unroll 1
-    for (int c = 0; c < D / 16 && steps > 0; ++c) {
-      float o[16];
-      tmem_ld_cols<16>(at_o + 16u * c, o);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) other_o[(4 * c + x) * kRows + row] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
-    }
-  }
-  if (!halves) __syncthreads();
-  if (has_rows && (halves || group == 0)) {
-    const int row = 32 * quarter + lane, number = r0 + (halves ? group * kRows : 0) + row;
-    const int node = (int)a.group.div(min(number, all - 1));
-    const int64_t part = tree_part(a, blockIdx.z, kvh, tile, split);
-    unsigned char* const lines = smem + kK + kRows * D * 4 + warp * 32 * D * 2;
-    const int odd_from = odd_s;
-    float f0 = 1.f, f1 = 0.f;
-    if (!halves && n_tiles > 1) {
-      const float2 other = other_s[row];
-      const float top = fmaxf(m_run, other.x), ref = top == -INFINITY ? 0.f : top;
-      f0 = tree_ex2(m_run - ref);
-      f1 = tree_ex2(other.x - ref);
-      l_run = (f0 != 0.f ? f0 * l_run : 0.f) + (f1 != 0.f ? f1 * other.y : 0.f);
-      m_run = top;
-    }
-    const float inv = parts > 1 ? 1.f : (l_run != 0.f ? 1.f / l_run : 0.f);
-    const bool write = number < all;
-    if (parts > 1 && write) a.part_ml[part * a.tile_rows + number - r0] = make_float2(m_run, l_run);
-#pragma unroll 1
-    for (int c = 0; c < D / 16; ++c) {
-      float o[16] = {};
-      __syncwarp();
-      if (n_tiles > 0) tmem_ld_cols<16>(at_o + 16u * c, o);
-      if (!halves && n_tiles > 1) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float4 w = other_o[(4 * c + x) * kRows + row];
-          const float y[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int z = 0; z < 4; ++z) o[4 * x + z] = (f0 != 0.f ? f0 * o[4 * x + z] : 0.f) + (f1 != 0.f ? f1 * y[z] : 0.f);
+      // ---- softmax
+      const bool works = quarter < s.warps(group);
+      const int number = s.r0 + (s.halves ? group * kRows : 0) + 32 * quarter + lane, mine = min(number, s.rows - 1);
+      const int node = (int)a.group.div(mine);
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int k = 0; k < steps && ok; ++k) {
+        const int u = u0 + k, i = s.step_tile(group, k), n = ring + i, st = n % kRing, t = t_begin + i * kKeys;
+        const uint32_t at_s = tmem + 128u * group + 64u * (u & 1) + lane_addr;
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_s[group][u & 1]), (u >> 1) & 1, limit));
+        if (!ok) break;
+        if (!works) {
+          if (lane == 0) mbar_arrive_cta(smem_u32(&bar_p[group][u & 1]));
+          continue;
         }
-      }
-      if (odd_from < n_tiles) {
-        for (int p = t_begin + odd_from * kKeys; p < t_end; ++p) {
-          const int j = (int)a.block.div(p), id = a.tables[(int64_t)blockIdx.z * a.table_row + j];
-          if (id < 0 || id >= a.n_blocks || !(tree_visible32(a, r, node, p) & 1u)) continue;
-          const uint32_t* v = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(a.v) + (int64_t)id * a.v_block +
-                                                                kvh * a.v_head + (int64_t)(p - j * (int)a.block.d) * a.v_tok + 16 * c);
+        // (complete: for what the TMA warp wrote, which this thread reads itself)
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_full[st]), (n / kRing) & 1, limit));
+        if (!ok) break;
+        tc_fence_after();
+        float x[64];
+        tmem_ld_cols<64>(at_s, x);
+        const uint32_t there = valid_s[st], whole = 0xffffffffu >> (32 - (1 << args.log_boxes));
+        const bool tree = t + kKeys > s.r.len;
+        if (tree) {  // (the same for all the CTA's rows)
+          unsigned char* const v_tile = smem + kK + st * kStage + kTile;
+          // (written back and fenced by each stream for itself, changed or not: the other's change may be under way)
+          for (int c = 32 * quarter + lane; c < (int)kTile / 16; c += 32 * s.warps(group)) {
+            uint4 w = reinterpret_cast<const uint4*>(v_tile)[c];
+            if (tree_not_finite<T>(w.x) || tree_not_finite<T>(w.y) || tree_not_finite<T>(w.z) || tree_not_finite<T>(w.w)) {
+              w.x = tree_finite<T>(w.x), w.y = tree_finite<T>(w.y), w.z = tree_finite<T>(w.z), w.w = tree_finite<T>(w.w);
+              if (t + (c % (kKeys * 8)) / 8 < t_end) {  // (rows behind the last key may hold anything)
+                atomicMin(&odd_s[seg & 1], i);
+                __threadfence_block();  // known before it is gone
+              }
+            }
+            reinterpret_cast<uint4*>(v_tile)[c] = w;
+          }
+          fence_proxy_async();
+          __syncwarp();
+        }
+        if (tree || there != whole) {
+          uint32_t seen0 = tree_visible32(a, s.r, node, t), seen1 = tree_visible32(a, s.r, node, t + 32);
+          const int left = t_end - t;
+          if (left < 64) {
+            seen0 &= left < 32 ? (1u << max(left, 0)) - 1u : 0xffffffffu;
+            seen1 &= left < 32 ? 0u : (1u << (left - 32)) - 1u;
+          }
+          if (there != whole) {
+            for (int j = 0; j < 32; ++j) {
+              if (!(there >> (j / args.box) & 1u)) seen0 &= ~(1u << j);
+              if (!(there >> ((j + 32) / args.box) & 1u)) seen1 &= ~(1u << j);
+            }
+          }
 #pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const float2 f = tree_unpack<T>(v[x]), z = tree_unpack<T>(tree_finite<T>(v[x]));
-            o[2 * x] += f.x - z.x;  // (x - x = 0 for what is finite)
-            o[2 * x + 1] += f.y - z.y;
+          for (int j = 0; j < 32; ++j) {
+            if (!(seen0 >> j & 1u)) x[j] = -INFINITY;
+            if (!(seen1 >> j & 1u)) x[32 + j] = -INFINITY;
           }
         }
-      }
-      if (parts > 1) {
-        if (write) {
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // independent chains
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            a.part_o[(part * (D / 4) + 4 * c + x) * a.tile_rows + number - r0] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        for (int j = 0; j < 64; j += 2) mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], x[j], x[j + 1]);
+        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;  // (the scale is positive)
+        const bool grown = mt > m_run + kGrowth;  // (from -inf: by any score)
+        if (k == 0) {
+          m_run = mt;
+        } else if (__any_sync(0xffffffffu, grown)) {
+          const float alpha = grown ? tree_ex2(m_run - mt) : 1.f;
+          if (grown) m_run = mt;
+          l_run *= alpha;
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_o[group][(u - 1) & 1]), ((u - 1) >> 1) & 1, limit));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            float v[16];
+            uint32_t w[16];
+            tmem_ld_cols<16>(at_o + 16u * c, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[j] * alpha);
+            tmem_st16(at_o + 16u * c, w);
+          }
         }
-      } else {
+        const float ref = kShift<T> - (m_run == -INFINITY ? 0.f : m_run);
+        const uint64_t ref2 = pair2(ref, ref);
+        uint64_t l2[2] = {0ull, 0ull};
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          *reinterpret_cast<uint4*>(lines + lane * (D * 2) + (((2 * c + x) ^ (lane & 7)) << 4)) =
-              make_uint4(tree_pack<T>(o[8 * x] * inv, o[8 * x + 1] * inv), tree_pack<T>(o[8 * x + 2] * inv, o[8 * x + 3] * inv),
-                         tree_pack<T>(o[8 * x + 4] * inv, o[8 * x + 5] * inv), tree_pack<T>(o[8 * x + 6] * inv, o[8 * x + 7] * inv));
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            float p0, p1;
+            unpair2(fma2(pair2(x[32 * h + 2 * j], x[32 * h + 2 * j + 1]), scale2, ref2), p0, p1);
+            p0 = tree_ex2(p0);  // 2^-inf = 0 for keys that are not seen
+            p1 = tree_ex2(p1);
+            w[j] = tree_pack<T>(p0, p1);
+            l2[j & 1] = add2(l2[j & 1], pair2(p0, p1));
+          }
+          tmem_st16(at_s + 16u * h, w);  // (P in the scores' own columns: they have all been read)
+        }
+        float la, lb;
+        unpair2(add2(l2[0], l2[1]), la, lb);
+        l_run += la + lb;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cta(smem_u32(&bar_p[group][u & 1]));
       }
-    }
-    if (parts == 1) {  // whole rows, from shared memory
-      __syncwarp();
-      const int first = number - lane;
+      u0 += steps;
+      ring += s.n_tiles;
+      if (ok && steps > 0)  // the last product
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_o[group][(u0 - 1) & 1]), ((u0 - 1) >> 1) & 1, limit));
+      tc_fence_after();
+      if (l_run != l_run) m_run = INFINITY;  // (a maximum passes over NaN)
+
+      // ---- epilogue; streams that share their rows meet here (both accumulators are in reach of the first one's warps)
+      if (!s.halves) {
+        if (group == 1) other_s[32 * quarter + lane] = make_float2(m_run, l_run);
+        tc_fence_before();
+        softmax_barrier();
+        tc_fence_after();
+      }
+      if (ok && works && (s.halves || group == 0)) {
+        const bool both = s.steps(1) > 0 && !s.halves, alone = s.n_tiles == s.key_tiles;
+        float f0 = 1.f, f1 = 0.f;
+        if (both) {
+          const float2 other = other_s[32 * quarter + lane];
+          const float top = fmaxf(m_run, other.x), ref = top == -INFINITY ? 0.f : top;
+          f0 = tree_ex2(m_run - ref);
+          f1 = tree_ex2(other.x - ref);
+          l_run = (f0 != 0.f ? f0 * l_run : 0.f) + (f1 != 0.f ? f1 * other.y : 0.f);
+          m_run = top;
+        }
+        const float inv = !alone ? 1.f : (l_run != 0.f ? 1.f / l_run : 0.f);
+        const bool write = number < s.rows;
+        const int64_t part = 2 * blockIdx.x + (s.tile0 == 0 ? 1 : 0);
+        const int odd_from = odd_s[seg & 1];
+        // (the queries' place: the stream's own, or that of the stream without)
+        unsigned char* const lines = smem + (s.halves ? group : 1) * kQ;
+        auto line_at = [&](int row, int chunk) { return (chunk >> 3) * kHalfQ + sw128_offset(32 * quarter + row, chunk & 7); };
+        if (!alone && write) a.part_ml[part * a.tile_rows + number - s.r0] = make_float2(m_run, l_run);
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {
+          float o[16];
+          __syncwarp();
+          tmem_ld_cols<16>(at_o + 16u * c, o);
+          if (both) {
+            float y[16];
+            tmem_ld_cols<16>(at_o + 128u + 16u * c, y);
+#pragma unroll
+            for (int z = 0; z < 16; ++z) o[z] = (f0 != 0.f ? f0 * o[z] : 0.f) + (f1 != 0.f ? f1 * y[z] : 0.f);
+          }
+          if (odd_from < s.n_tiles) {
+            for (int p = t_begin + odd_from * kKeys; p < t_end; ++p) {
+              const int j = (int)a.block.div(p), id = a.tables[(int64_t)s.b * a.table_row + j];
+              if (id < 0 || id >= a.n_blocks || !(tree_visible32(a, s.r, node, p) & 1u)) continue;
+              const uint32_t* v = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(a.v) + (int64_t)id * a.v_block +
+                                                                    s.kvh * a.v_head + (int64_t)(p - j * (int)a.block.d) * a.v_tok + 16 * c);
+#pragma unroll
+              for (int z = 0; z < 8; ++z) {
+                const float2 f = tree_unpack<T>(v[z]), w = tree_unpack<T>(tree_finite<T>(v[z]));
+                o[2 * z] += f.x - w.x;  // (x - x = 0 for what is finite)
+                o[2 * z + 1] += f.y - w.y;
+              }
+            }
+          }
+          if (!alone) {
+            if (write) {
+#pragma unroll
+              for (int z = 0; z < 4; ++z)
+                a.part_o[(part * (D / 4) + 4 * c + z) * a.tile_rows + number - s.r0] =
+                    make_float4(o[4 * z], o[4 * z + 1], o[4 * z + 2], o[4 * z + 3]);
+            }
+          } else {
+#pragma unroll
+            for (int z = 0; z < 2; ++z)
+              *reinterpret_cast<uint4*>(lines + line_at(lane, 2 * c + z)) =
+                  make_uint4(tree_pack<T>(o[8 * z] * inv, o[8 * z + 1] * inv), tree_pack<T>(o[8 * z + 2] * inv, o[8 * z + 3] * inv),
+                             tree_pack<T>(o[8 * z + 4] * inv, o[8 * z + 5] * inv), tree_pack<T>(o[8 * z + 6] * inv, o[8 * z + 7] * inv));
+          }
+        }
+        __syncwarp();
+        if (alone) {  // whole rows, from shared memory
+          const int first = number - lane;
 #pragma unroll 4
-      for (int i = lane; i < 32 * (D / 8); i += 32) {
-        const int at = i / (D / 8), chunk = i % (D / 8);
-        if (first + at < all) {
-          const int nd = (int)a.group.div(first + at), hd = kvh * (int)a.group.d + first + at - nd * (int)a.group.d;
-          reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + ((int64_t)(r.start + nd) * a.heads + hd) * D)[chunk] =
-              *reinterpret_cast<const uint4*>(lines + at * (D * 2) + ((chunk ^ (at & 7)) << 4));
+          for (int i = lane; i < 32 * (D / 8); i += 32) {
+            const int at = i / (D / 8), chunk = i % (D / 8);
+            if (first + at < s.rows) {
+              const int nd = (int)a.group.div(first + at), head = s.kvh * (int)a.group.d + first + at - nd * (int)a.group.d;
+              reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + ((int64_t)(s.r.start + nd) * a.heads + head) * D)[chunk] =
+                  *reinterpret_cast<const uint4*>(lines + line_at(at, chunk));
+            }
+          }
+          __syncwarp();
         }
+        tc_fence_before();
       }
+      if (!s.halves) softmax_barrier();  // the second stream's accumulator and the queries' place are free
     }
+    if (!ok && fail_s == 0) fail_s = 1;
   }
   __syncwarp();
+  pdl_launch_dependents();
   tc_fence_before();
   __syncthreads();
-  if (failed) {
-    if (tid == 0) tc_report(status, (fail_s << 16) | 0x3000 | ((int)blockIdx.x & 0xfff));
+  if (fail_s != 0) {
+    if (tid == 0) tc_report(status, (fail_s << 16) | 0x3000 | (blockIdx.x & 0xfff));
     drain_failed(issuer, smem_u32(&bar_drain));
   }
   if (warp == kSoftmaxWarps)
@@ -516,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
 template <typename T, int D>
 int launch_tc(const TreeTcArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t stream, int* status) {
   QUIC_CUDA((allow_smem<tree_attn_tc_kernel<T, D>>(kTcSmem<D>)));
-  QUIC_CUDA(launch(tree_attn_tc_kernel<T, D>, dim3((unsigned)(a.t.tiles * a.t.splits), a.t.kv_heads, a.t.requests), dim3(kThreads),
+  QUIC_CUDA(launch(tree_attn_tc_kernel<T, D>, dim3(kTreeTcCtas), dim3(kThreads),
                    kTcSmem<D>, stream, false, tm_k, tm_v, a, status));
   return QUIC_OK;
 }
