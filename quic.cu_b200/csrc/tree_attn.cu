@@ -72,6 +72,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
   __shared__ uint32_t valid_s[kWarps][kStages<D>];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, kvh = blockIdx.y % a.kv_heads, tile = blockIdx.y / a.kv_heads;
+  pdl_wait();
   const TreeRequest r = tree_request(a, blockIdx.z);
   const int all = min(r.n, a.max_new) * (int)a.group.d, r0 = tile * 16 * MT;  // row = node x group + head of the group
   if (r0 >= all) return;
@@ -341,20 +342,22 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
   }
 }
 
-// Rows whose keys several CTAs shared: sum of the parts, each by 2^(its maximum - the largest).  A CTA has 32 rows of a tile,
-// a row a lane, so that parts are read in whole lines; its four warps have a quarter of the head dimensions each.
+// Rows whose keys several CTAs shared: sum of the parts, each by 2^(its maximum - the largest).  A CTA has 32 rows of a tile
+// (a row a lane, so that parts are read in whole lines) and 16 head dimensions, a warp every eighth part; the warps meet in
+// shared memory.  Bound by two rounds of loads (with four warps that each read all parts of a row, 17 parts took 22 us).
 template <typename T, int D, bool kTc>
-__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a) {
-  constexpr int kMine = D / 16;  // float4 of a thread
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y;
-  const int per_tile = a.tile_rows / 32, tile = blockIdx.x / per_tile, row = blockIdx.x % per_tile * 32 + lane;
+__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a) {
+  __shared__ float4 o_s[8][4][32];
+  __shared__ float2 ml_s[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y, quarter = blockIdx.x % (D / 16);
+  const int per_tile = a.tile_rows / 32, rows32 = blockIdx.x / (D / 16), tile = rows32 / per_tile, row = rows32 % per_tile * 32 + lane;
+  pdl_launch_dependents();
+  pdl_wait();
   const TreeRequest r = tree_request(a, blockIdx.z);
   const int all = min(r.n, a.max_new) * (int)a.group.d, number = tile * a.tile_rows + row;
-  pdl_wait();
-  if (number >= all) return;
+  if (number - lane >= all) return;
   int parts;
-  int64_t part, step;  // the parts are part0, then part, part + step, ...
-  int64_t part0;
+  int64_t part0, part, step;  // the parts are part0, then part + step, part + 2 step, ...
   if constexpr (kTc) {  // the CTA where the row tile begins has it as its last segment, the others as their first
     const TreeUnits u = tree_units(a, r);
     const int64_t share = a.first[a.requests + 1], t0 = a.first[blockIdx.z] + ((int64_t)kvh * u.row_tiles + tile) * u.key_tiles;
@@ -367,43 +370,55 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a) {
     part0 = part = tree_part(a, blockIdx.z, kvh, tile), step = 1;
   }
   if (parts == 1) return;
-  auto place = [&](int s) { return s == 0 ? part0 : part + s * step; };
-  const float2* const ml = a.part_ml + row;
-  const float4* const po = a.part_o + (int64_t)warp * kMine * a.tile_rows + row;
-  float top = -INFINITY;
-#pragma unroll 8
-  for (int s = 0; s < parts; ++s) top = fmaxf(top, ml[place(s) * a.tile_rows].x);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float l = 0.f;
-  float4 o[kMine] = {};
-#pragma unroll 4
-  for (int s = 0; s < parts; ++s) {
-    const int64_t at = place(s);
-    const float2 x = ml[at * a.tile_rows];
-    float4 y[kMine];
+  float top = -INFINITY, l = 0.f;
+  float4 o[4] = {};
+#pragma unroll 2
+  for (int s = warp; s < parts; s += 8) {  // running maximum and sum
+    const int64_t at = s == 0 ? part0 : part + s * step;
+    const float2 x = a.part_ml[at * a.tile_rows + row];
+    float4 y[4];
 #pragma unroll
-    for (int c = 0; c < kMine; ++c) y[c] = po[(at * (D / 4) + c) * a.tile_rows];
-    const float f = tree_ex2(x.x - ref);
-    if (f != 0.f) {
-      l += f * x.y;
+    for (int c = 0; c < 4; ++c) y[c] = a.part_o[(at * (D / 4) + 4 * quarter + c) * a.tile_rows + row];
+    const float m = fmaxf(top, x.x), ref = m == -INFINITY ? 0.f : m, f = tree_ex2(top - ref), g = tree_ex2(x.x - ref);
+    top = m;
+    l = (f != 0.f ? f * l : 0.f) + (g != 0.f ? g * x.y : 0.f);
 #pragma unroll
-      for (int c = 0; c < kMine; ++c) o[c].x += f * y[c].x, o[c].y += f * y[c].y, o[c].z += f * y[c].z, o[c].w += f * y[c].w;
+    for (int c = 0; c < 4; ++c) {
+      o[c].x = (f != 0.f ? f * o[c].x : 0.f) + (g != 0.f ? g * y[c].x : 0.f);
+      o[c].y = (f != 0.f ? f * o[c].y : 0.f) + (g != 0.f ? g * y[c].y : 0.f);
+      o[c].z = (f != 0.f ? f * o[c].z : 0.f) + (g != 0.f ? g * y[c].z : 0.f);
+      o[c].w = (f != 0.f ? f * o[c].w : 0.f) + (g != 0.f ? g * y[c].w : 0.f);
     }
   }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  const int node = (int)a.group.div(number), head = kvh * (int)a.group.d + number - node * (int)a.group.d;
-  uint4* const out = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + ((int64_t)(r.start + node) * a.heads + head) * D + warp * kMine * 4);
 #pragma unroll
-  for (int c = 0; c < kMine; c += 2)
-    out[c / 2] = make_uint4(tree_pack<T>(o[c].x * inv, o[c].y * inv), tree_pack<T>(o[c].z * inv, o[c].w * inv),
-                            tree_pack<T>(o[c + 1].x * inv, o[c + 1].y * inv), tree_pack<T>(o[c + 1].z * inv, o[c + 1].w * inv));
+  for (int c = 0; c < 4; ++c) o_s[warp][c][lane] = o[c];
+  ml_s[warp][lane] = make_float2(top, l);
+  __syncthreads();
+  if (warp >= 4 || number >= all) return;  // a warp four dims
+  float m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, ml_s[w][lane].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float sum = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const float2 x = ml_s[w][lane];
+    const float4 y = o_s[w][warp][lane];
+    const float f = tree_ex2(x.x - ref);
+    if (f != 0.f) sum += f * x.y, v.x += f * y.x, v.y += f * y.y, v.z += f * y.z, v.w += f * y.w;
+  }
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  const int node = (int)a.group.div(number), head = kvh * (int)a.group.d + number - node * (int)a.group.d;
+  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + ((int64_t)(r.start + node) * a.heads + head) * D + 16 * quarter + 4 * warp) =
+      make_uint2(tree_pack<T>(v.x * inv, v.y * inv), tree_pack<T>(v.z * inv, v.w * inv));
 }
 
 template <typename T, int D, int MT>
 int launch_few(const TreeArgs& a, cudaStream_t st) {
   QUIC_CUDA((allow_smem<tree_attn_kernel<T, D, MT>>(kSmem<D, MT>)));
   QUIC_CUDA(launch(tree_attn_kernel<T, D, MT>, dim3(a.splits, a.kv_heads * a.tiles, a.requests), dim3(kWarps * 32), kSmem<D, MT>, st,
-                   false, a));
+                   true, a));
   return QUIC_OK;
 }
 
@@ -452,8 +467,8 @@ int launch_typed(const TreeArgs& a, const Plan& p, cudaStream_t st) {
                  : a.max_new * (int64_t)a.group.d <= 16 ? launch_few<T, D, 1>(a, st)
                                    : launch_few<T, D, 2>(a, st);
   if (rc != QUIC_OK || p.parts == 0) return rc;
-  const dim3 grid((unsigned)(a.tiles * (a.tile_rows / 32)), a.kv_heads, a.requests);
-  QUIC_CUDA(launch(p.tc ? tree_merge_kernel<T, D, true> : tree_merge_kernel<T, D, false>, grid, dim3(128), 0, st, true, a));
+  const dim3 grid((unsigned)(a.tiles * (a.tile_rows / 32) * (D / 16)), a.kv_heads, a.requests);
+  QUIC_CUDA(launch(p.tc ? tree_merge_kernel<T, D, true> : tree_merge_kernel<T, D, false>, grid, dim3(256), 0, st, true, a));
   return QUIC_OK;
 }
 

@@ -18,8 +18,8 @@
 // Only tiles that reach beyond the cached tokens look at masks.  A V row of a node may hold infinities or NaN that most rows
 // must not see: such values are zeroed in shared memory and added, at the end, to the rows that see them.
 //
-// Roles: warps 0-7 queries, softmax and epilogue, warp 8 MMA issuer (next scores or next product, whichever is ready), warp 9
-// TMA.  Every wait is bounded; a wait that runs out sets word 0 of the tensor path's error words and the CTA leaves with
+// Roles: warps 0-7 queries, softmax and epilogue, warps 8 and 9 MMA issuers of the two streams, warps 10 and 11
+// TMA of K and V.  Every wait is bounded; a wait that runs out sets word 0 of the tensor path's error words and the CTA leaves with
 // its MMAs and copies complete and its tensor memory released.
 #include "tc_common.cuh"
 #include "tree_attn.cuh"
@@ -28,7 +28,7 @@ namespace quic {
 namespace {
 
 constexpr int kRows = 128, kKeys = 64, kGroupWarps = 4, kSoftmaxWarps = 2 * kGroupWarps;
-constexpr int kTmaWarp = kSoftmaxWarps + 2, kThreads = (kTmaWarp + 1) * 32;
+constexpr int kTmaWarp = kSoftmaxWarps + 2, kThreads = (kTmaWarp + 2) * 32;
 constexpr int kLeastShare = 4;  // key tiles of a CTA
 static_assert(2 * kRows == kTreeTcRows && kKeys == kTreeTcKeys, "two streams of rows");
 constexpr float kGrowth = 8.f;    // of a row's maximum (base 2) before its reference point follows
@@ -94,6 +94,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st2(uint32_t taddr, uint32_t a, uint32_t b) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1,%2};" ::"r"(taddr), "r"(a), "r"(b) : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Barrier 1: the softmax warps.
@@ -130,14 +133,15 @@ struct Walk {
         ++b;
         continue;
       }
-      const int64_t unit = at / u.key_tiles;
+      // (a division of 64 bits takes longer than a key tile's products)
+      const uint32_t unit = at <= 0xffffffffll ? (uint32_t)at / (uint32_t)u.key_tiles : (uint32_t)(at / u.key_tiles);
       s.b = b;
-      s.kvh = (int)(unit / u.row_tiles);
-      s.r0 = (int)(unit % u.row_tiles) * kTreeTcRows;
+      s.kvh = (int)(unit / (uint32_t)u.row_tiles);
+      s.r0 = (int)(unit - (uint32_t)s.kvh * u.row_tiles) * kTreeTcRows;
       s.rows = u.rows;
       s.halves = u.rows - s.r0 > kRows;
       s.key_tiles = u.key_tiles;
-      s.tile0 = (int)(at % u.key_tiles);
+      s.tile0 = (int)(at - (int64_t)unit * u.key_tiles);
       s.n_tiles = (int)min(left, (int64_t)(u.key_tiles - s.tile0));
       at += s.n_tiles;
       left -= s.n_tiles;
@@ -158,7 +162,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kRing], bar_empty[kRing], bar_s[2][2], bar_p[2][2], bar_o[2][2], bar_q, bar_drain;
   __shared__ uint32_t valid_s[kRing];  // which boxes of the stage have a block
-  __shared__ float2 other_s[kRows];    // maximum and sum of stream 1, where the streams share rows
   __shared__ int64_t sums_s[kThreads / 32];
   __shared__ Walk walk_s;
   __shared__ uint32_t tmem_base_s;
@@ -169,7 +172,33 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* const smem = smem_raw + (base - smem_u32(smem_raw));
 
+  // ---- barriers and tensor memory, before the kernels in front have ended
+  if (warp == kTmaWarp && lane == 0) {
+    for (int s = 0; s < kRing; ++s) {
+      mbar_init(smem_u32(&bar_full[s]), 2);
+      mbar_init(smem_u32(&bar_empty[s]), 2);
+    }
+    for (int g = 0; g < 2; ++g)
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(smem_u32(&bar_s[g][x]), 1);
+        mbar_init(smem_u32(&bar_p[g][x]), kGroupWarps);
+        mbar_init(smem_u32(&bar_o[g][x]), 1);
+      }
+    mbar_init(smem_u32(&bar_q), kSoftmaxWarps);
+    mbar_init(smem_u32(&bar_drain), 2);
+    fail_s = 0;
+    odd_s[0] = odd_s[1] = 0x7fffffff;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kSoftmaxWarps) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+
   // ---- the line of key tiles, and where in it this CTA begins
+  uint32_t tmem;
   {
     const int each = (a.requests + kThreads - 1) / kThreads, b0 = min(tid * each, a.requests), b1 = min(b0 + each, a.requests);
     int64_t mine = 0;
@@ -182,24 +211,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
     }
     if (lane == 31) sums_s[warp] = before;
     before -= mine;
-    if (warp == kTmaWarp && lane == 0) {
-      for (int s = 0; s < kRing; ++s) {
-        mbar_init(smem_u32(&bar_full[s]), 1);
-        mbar_init(smem_u32(&bar_empty[s]), 2);
-      }
-      for (int g = 0; g < 2; ++g)
-        for (int x = 0; x < 2; ++x) {
-          mbar_init(smem_u32(&bar_s[g][x]), 1);
-          mbar_init(smem_u32(&bar_p[g][x]), kGroupWarps);
-          mbar_init(smem_u32(&bar_o[g][x]), 1);
-        }
-      mbar_init(smem_u32(&bar_q), kSoftmaxWarps);
-      mbar_init(smem_u32(&bar_drain), 2);
-      fail_s = 0;
-      odd_s[0] = odd_s[1] = 0x7fffffff;
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
+    tc_fence_before();
     __syncthreads();
+    tc_fence_after();
+    tmem = tmem_base_s;
     int64_t total = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
@@ -215,7 +230,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
       }
       if (tid == 0) a.first[a.requests] = total, a.first[a.requests + 1] = share;
     }
-    if (start >= total) return;
+    if (start >= total) {
+      if (warp == kSoftmaxWarps)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+      return;
+    }
     if (before <= start && start < before + mine) {
       int b = b0;
       for (int64_t n; (n = tree_units(a, tree_request(a, b)).all(a)) <= start - before; ++b) before += n;
@@ -223,39 +242,40 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
       walk_s.at = start - before;
       walk_s.left = min(share, total - start);
     }
-    if (warp == kSoftmaxWarps) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(kTmemCols)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_fence_before();
     __syncthreads();
-    tc_fence_after();
   }
-  const uint32_t tmem = tmem_base_s;
   Walk walk = walk_s;
-  Segment s;
+  Segment s, later;  // this one and the next, whose numbers are fetched ahead
+  bool more = walk.next(a, s), more_later = false;
   int ring = 0;  // tiles of the segments before
   bool issuer = false;
 
-  if (warp == kTmaWarp) {
-    // ---------------- TMA: a lane a box of 64 dims of K or V ----------------
-    const int boxes = 1 << args.log_boxes, box = lane & (boxes - 1), what = lane >> args.log_boxes;
-    const bool copies = what < 2 * kHalves;
-    const CUtensorMap* const map = what & 1 ? &tm_v : &tm_k;
-    const uint32_t dst = base + kK + (what & 1) * kTile + (what >> 1) * kHalfK + box * args.box * 128;
-    if (lane < 2) tma_prefetch_desc(lane ? &tm_v : &tm_k);
+  if (warp >= kTmaWarp) {
+    // ---------------- TMA, K and V: a lane a box of 64 dims.  (A warp's copies go out one after the other, 80 clocks each) ----------------
+    const int what = warp - kTmaWarp, boxes = 1 << args.log_boxes, box = lane & (boxes - 1), half = lane >> args.log_boxes;
+    const bool copies = half < kHalves;
+    const CUtensorMap* const map = what ? &tm_v : &tm_k;
+    const uint32_t dst = base + kK + what * kTile + half * kHalfK + box * args.box * 128;
+    if (lane == 0) tma_prefetch_desc(map);
     bool ok = true;
-    while (ok && walk.next(a, s)) {
+    for (; ok && more; s = later, more = more_later) {
+      more_later = walk.next(a, later);
       const int32_t* table = a.tables + (int64_t)s.b * a.table_row;
       const int t_begin = s.begin(), t_end = s.end();
-      auto fetch = [&](int i) {  // the block of this lane's box of tile i, n_blocks (beyond the planes) where there is none
-        const int p = t_begin + i * kKeys + box * args.box, id = p < t_end ? __ldg(table + a.block.div(p)) : -1;
+      // the blocks of 32 boxes, n_blocks (beyond the planes) where there is none; those of the next 32 are under way meanwhile
+      const int at_once = 32 >> args.log_boxes;
+      auto fetch = [&](int i) {
+        const int p = t_begin + i * kKeys + lane * args.box, id = p < t_end ? __ldg(table + a.block.div(p)) : -1;
         return id >= 0 && id < a.n_blocks ? id : a.n_blocks;
       };
-      int id = fetch(0), next = fetch(1);
+      int ids = 0, next = fetch(0);
       for (int i = 0; i < s.n_tiles; ++i, ++ring) {
-        const int st = ring % kRing, after = fetch(i + 2);
+        const int st = ring % kRing;
+        if ((i & (at_once - 1)) == 0) {
+          ids = next;
+          next = fetch(i + at_once);
+        }
+        const int id = __shfl_sync(0xffffffffu, ids, ((i & (at_once - 1)) << args.log_boxes) + box);
         if (ring >= kRing && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_empty[st]), (ring / kRing - 1) & 1, args.wait_limit_us))) {
           fail_s = 2;
           ok = false;
@@ -265,15 +285,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
         const uint32_t there = __ballot_sync(0xffffffffu, id < a.n_blocks) & (0xffffffffu >> (32 - boxes));
         const uint32_t full = smem_u32(&bar_full[st]);
         if (lane == 0) {
-          valid_s[st] = there;
-          mbar_expect_tx(full, kStage);
+          if (what == 0) valid_s[st] = there;
+          mbar_expect_tx(full, kTile);
         }
         __syncwarp();
         const int p = t_begin + i * kKeys + box * args.box;
-        if (copies && (ring != args.skip_tile || (what & 1)))
-          tma_load_4d(dst + st * kStage, map, 64 * (what >> 1), p - (int)a.block.div(p) * (int)a.block.d, s.kvh, id, full);
-        id = next;
-        next = after;
+        if (copies && (ring != args.skip_tile || what))
+          tma_load_4d(dst + st * kStage, map, 64 * half, p - (int)a.block.div(p) * (int)a.block.d, s.kvh, id, full);
       }
     }
   } else if (warp >= kSoftmaxWarps) {
@@ -292,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
     };
     int u = 0;  // steps of the segments before
     bool ok = true;
-    for (int seg = 0; ok && walk.next(a, s); ++seg) {
+    for (int seg = 0; ok && more; s = later, more = more_later, ++seg) {
       const int steps = s.steps(g);
       const uint64_t q = q0 + (uint64_t)((s.halves ? g : 0) * (kQ / 16));
       auto scores = [&](int k) {
@@ -313,6 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
         __syncwarp();
         return true;
       };
+      more_later = walk.next(a, later);
       ok = wait(&bar_q, seg & 1) && (steps == 0 || scores(0));
       for (int k = 0; ok && k < steps; ++k) {
         const int n = ring + s.step_tile(g, k), st = n % kRing, x = (u + k) & 1;
@@ -321,11 +340,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
         tc_fence_after();
         const uint64_t vt = v0 + (uint64_t)(st * (kStage / 16));
         const uint32_t from = at_s + 64u * x, bar = smem_u32(&bar_o[g][x]), free = smem_u32(&bar_empty[st]);
-        const uint32_t more = k > 0 ? 1u : 0u;
+        const uint32_t onto = k > 0 ? 1u : 0u;
         if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)  // sixteen tokens a step: two groups of eight rows of the V tile, eight columns of P
-            umma_ts(at_o, from + 8u * c, vt + c * (2048 / 16), idesc_v, c > 0 ? 1u : more);
+            umma_ts(at_o, from + 8u * c, vt + c * (2048 / 16), idesc_v, c > 0 ? 1u : onto);
           umma_commit(bar);
           umma_commit(free);
           if (!s.halves) umma_commit(free);  // (nobody else reads the tile)
@@ -345,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
     const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2);
     int u0 = 0;  // steps of the segments before
     bool ok = true;  // (without it a warp goes on to the end, past all waits, for the barriers of the segments)
-    for (int seg = 0; walk.next(a, s); ++seg) {
+    for (int seg = 0; more; s = later, more = more_later, ++seg) {
       const int t_begin = s.begin(), t_end = s.end(), steps = s.steps(group);
       // ---- queries of the stream's rows (the first stream's, where they are the same); rows that are none are zero
       if (s.halves || group == 0) {
@@ -358,6 +377,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
                  reinterpret_cast<const T*>(a.q) + (int64_t)(s.r.start + node) * a.q_row + (int64_t)head * a.q_head + 8 * chunk,
                  number < s.rows ? 16u : 0u);
         }
+      }
+      // ---- meanwhile: the next segment, and what the row sees of the first tile that reaches beyond the cached tokens
+      more_later = walk.next(a, later);
+      const bool works = quarter < s.warps(group);
+      const int number = s.r0 + (s.halves ? group * kRows : 0) + 32 * quarter + lane, mine = min(number, s.rows - 1);
+      const int node = (int)a.group.div(mine);
+      const int tree_from = max(t_begin, s.r.len & ~(kKeys - 1));
+      const uint32_t first0 = tree_visible32(a, s.r, node, tree_from), first1 = tree_visible32(a, s.r, node, tree_from + 32);
+      if (s.halves || group == 0) {
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async();
       }
@@ -367,56 +395,58 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
       if (tid == 0) odd_s[(seg + 1) & 1] = 0x7fffffff;  // (all are through with the segment before, none with this)
 
       // ---- softmax
-      const bool works = quarter < s.warps(group);
-      const int number = s.r0 + (s.halves ? group * kRows : 0) + 32 * quarter + lane, mine = min(number, s.rows - 1);
-      const int node = (int)a.group.div(mine);
       float m_run = -INFINITY, l_run = 0.f;
       for (int k = 0; k < steps && ok; ++k) {
         const int u = u0 + k, i = s.step_tile(group, k), n = ring + i, st = n % kRing, t = t_begin + i * kKeys;
         const uint32_t at_s = tmem + 128u * group + 64u * (u & 1) + lane_addr;
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_s[group][u & 1]), (u >> 1) & 1, limit));
         if (!ok) break;
-        if (!works) {
-          if (lane == 0) mbar_arrive_cta(smem_u32(&bar_p[group][u & 1]));
-          continue;
-        }
-        // (complete: for what the TMA warp wrote, which this thread reads itself)
+        // (complete: for what the TMA warps wrote, which this thread reads itself)
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_full[st]), (n / kRing) & 1, limit));
         if (!ok) break;
-        tc_fence_after();
-        float x[64];
-        tmem_ld_cols<64>(at_s, x);
-        const uint32_t there = valid_s[st], whole = 0xffffffffu >> (32 - (1 << args.log_boxes));
         const bool tree = t + kKeys > s.r.len;
         if (tree) {  // (the same for all the CTA's rows)
           unsigned char* const v_tile = smem + kK + st * kStage + kTile;
-          // (written back and fenced by each stream for itself, changed or not: the other's change may be under way)
-          for (int c = 32 * quarter + lane; c < (int)kTile / 16; c += 32 * s.warps(group)) {
+#pragma unroll 2
+          for (int c = 32 * quarter + lane; c < (int)kTile / 16; c += 32 * kGroupWarps) {
             uint4 w = reinterpret_cast<const uint4*>(v_tile)[c];
+            bool store = s.halves;  // (each stream for itself, changed or not: the other's change may be under way)
             if (tree_not_finite<T>(w.x) || tree_not_finite<T>(w.y) || tree_not_finite<T>(w.z) || tree_not_finite<T>(w.w)) {
               w.x = tree_finite<T>(w.x), w.y = tree_finite<T>(w.y), w.z = tree_finite<T>(w.z), w.w = tree_finite<T>(w.w);
               if (t + (c % (kKeys * 8)) / 8 < t_end) {  // (rows behind the last key may hold anything)
                 atomicMin(&odd_s[seg & 1], i);
                 __threadfence_block();  // known before it is gone
               }
+              store = true;
             }
-            reinterpret_cast<uint4*>(v_tile)[c] = w;
+            if (store) reinterpret_cast<uint4*>(v_tile)[c] = w;
           }
           fence_proxy_async();
           __syncwarp();
         }
+        if (!works) {
+          if (lane == 0) mbar_arrive_cta(smem_u32(&bar_p[group][u & 1]));
+          continue;
+        }
+        tc_fence_after();
+        float x[64];
+        tmem_ld_cols<64>(at_s, x);
+        const uint32_t there = valid_s[st], whole = 0xffffffffu >> (32 - (1 << args.log_boxes));
         if (tree || there != whole) {
-          uint32_t seen0 = tree_visible32(a, s.r, node, t), seen1 = tree_visible32(a, s.r, node, t + 32);
+          uint32_t seen0 = first0, seen1 = first1;
+          if (t != tree_from) seen0 = tree_visible32(a, s.r, node, t), seen1 = tree_visible32(a, s.r, node, t + 32);
           const int left = t_end - t;
           if (left < 64) {
             seen0 &= left < 32 ? (1u << max(left, 0)) - 1u : 0xffffffffu;
             seen1 &= left < 32 ? 0u : (1u << (left - 32)) - 1u;
           }
           if (there != whole) {
-            for (int j = 0; j < 32; ++j) {
-              if (!(there >> (j / args.box) & 1u)) seen0 &= ~(1u << j);
-              if (!(there >> ((j + 32) / args.box) & 1u)) seen1 &= ~(1u << j);
-            }
+            const uint64_t tokens = 0xffffffffffffffffull >> (64 - args.box);
+            uint64_t have = 0ull;
+            for (int j = 0; j < 1 << args.log_boxes; ++j)
+              if (there >> j & 1u) have |= tokens << (j * args.box);
+            seen0 &= (uint32_t)have;
+            seen1 &= (uint32_t)(have >> 32);
           }
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
@@ -480,22 +510,28 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
       tc_fence_after();
       if (l_run != l_run) m_run = INFINITY;  // (a maximum passes over NaN)
 
-      // ---- epilogue; streams that share their rows meet here (both accumulators are in reach of the first one's warps)
+      // ---- epilogue; streams that share their rows meet here: both accumulators are in reach of both streams' warps, which
+      // have half of the head dims each
       if (!s.halves) {
-        if (group == 1) other_s[32 * quarter + lane] = make_float2(m_run, l_run);
+        tmem_st2(tmem + 128u * group + lane_addr, __float_as_uint(m_run), __float_as_uint(l_run));  // (the scores have been used)
+        tmem_wait_st();
         tc_fence_before();
         softmax_barrier();
         tc_fence_after();
       }
-      if (ok && works && (s.halves || group == 0)) {
+      if (ok && works) {
         const bool both = s.steps(1) > 0 && !s.halves, alone = s.n_tiles == s.key_tiles;
+        const int c_begin = s.halves ? 0 : group * (D / 32), c_end = s.halves ? D / 16 : (group + 1) * (D / 32);
+        const uint32_t at_o0 = tmem + kColO + (s.halves ? 128u * group : 0u) + lane_addr;
         float f0 = 1.f, f1 = 0.f;
-        if (both) {
-          const float2 other = other_s[32 * quarter + lane];
-          const float top = fmaxf(m_run, other.x), ref = top == -INFINITY ? 0.f : top;
-          f0 = tree_ex2(m_run - ref);
-          f1 = tree_ex2(other.x - ref);
-          l_run = (f0 != 0.f ? f0 * l_run : 0.f) + (f1 != 0.f ? f1 * other.y : 0.f);
+        if (!s.halves) {
+          float one[2], two[2];
+          tmem_ld_cols<2>(tmem + lane_addr, one);
+          tmem_ld_cols<2>(tmem + 128u + lane_addr, two);
+          const float top = fmaxf(one[0], two[0]), ref = top == -INFINITY ? 0.f : top;
+          f0 = tree_ex2(one[0] - ref);
+          f1 = tree_ex2(two[0] - ref);
+          l_run = (f0 != 0.f ? f0 * one[1] : 0.f) + (f1 != 0.f ? f1 * two[1] : 0.f);
           m_run = top;
         }
         const float inv = !alone ? 1.f : (l_run != 0.f ? 1.f / l_run : 0.f);
@@ -505,15 +541,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
         // (the queries' place: the stream's own, or that of the stream without)
         unsigned char* const lines = smem + (s.halves ? group : 1) * kQ;
         auto line_at = [&](int row, int chunk) { return (chunk >> 3) * kHalfQ + sw128_offset(32 * quarter + row, chunk & 7); };
-        if (!alone && write) a.part_ml[part * a.tile_rows + number - s.r0] = make_float2(m_run, l_run);
+        if (!alone && write && c_begin == 0) a.part_ml[part * a.tile_rows + number - s.r0] = make_float2(m_run, l_run);
 #pragma unroll 1
-        for (int c = 0; c < D / 16; ++c) {
+        for (int c = c_begin; c < c_end; ++c) {
           float o[16];
           __syncwarp();
-          tmem_ld_cols<16>(at_o + 16u * c, o);
+          tmem_ld_cols<16>(at_o0 + 16u * c, o);
           if (both) {
             float y[16];
-            tmem_ld_cols<16>(at_o + 128u + 16u * c, y);
+            tmem_ld_cols<16>(at_o0 + 128u + 16u * c, y);
 #pragma unroll
             for (int z = 0; z < 16; ++z) o[z] = (f0 != 0.f ? f0 * o[z] : 0.f) + (f1 != 0.f ? f1 * y[z] : 0.f);
           }
@@ -550,8 +586,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
         if (alone) {  // whole rows, from shared memory
           const int first = number - lane;
 #pragma unroll 4
-          for (int i = lane; i < 32 * (D / 8); i += 32) {
-            const int at = i / (D / 8), chunk = i % (D / 8);
+          for (int i = lane; i < 32 * 2 * (c_end - c_begin); i += 32) {
+            const int at = s.halves ? i / (D / 8) : i / (D / 16), chunk = 2 * c_begin + (s.halves ? i % (D / 8) : i % (D / 16));
             if (first + at < s.rows) {
               const int nd = (int)a.group.div(first + at), head = s.kvh * (int)a.group.d + first + at - nd * (int)a.group.d;
               reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + ((int64_t)(s.r.start + nd) * a.heads + head) * D)[chunk] =
@@ -575,14 +611,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
     drain_failed(issuer, smem_u32(&bar_drain));
   }
   if (warp == kSoftmaxWarps)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_s), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
 template <typename T, int D>
 int launch_tc(const TreeTcArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t stream, int* status) {
   QUIC_CUDA((allow_smem<tree_attn_tc_kernel<T, D>>(kTcSmem<D>)));
   QUIC_CUDA(launch(tree_attn_tc_kernel<T, D>, dim3(kTreeTcCtas), dim3(kThreads),
-                   kTcSmem<D>, stream, false, tm_k, tm_v, a, status));
+                   kTcSmem<D>, stream, true, tm_k, tm_v, a, status));
   return QUIC_OK;
 }
 
