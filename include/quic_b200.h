@@ -355,6 +355,22 @@ int64_t quic_tree_attn_scratch_bytes(int32_t requests, int32_t heads,
                                      int32_t kv_heads, int32_t dim,
                                      int32_t max_new, int64_t max_len);
 
+typedef struct {
+  int32_t *tables; /* [requests, max_blocks], rows table_row apart */
+  int64_t table_row;
+  int32_t *held;          /* [requests] */
+  int32_t *pool;          /* [4 + n_blocks] */
+  const int32_t *lengths; /* [requests] */
+  const int32_t *n_new;   /* [requests] */
+  const int32_t *parents; /* [parent_rows] or NULL */
+  int32_t *row_start;     /* [requests + 1] */
+  int64_t *slot_map;      /* [max_rows] */
+  int32_t *positions;     /* [max_rows] */
+  int32_t *mask;          /* [max_rows, mask_words], with parents */
+  void *reserved;         /* NULL */
+  int32_t max_blocks, n_blocks, requests, block_size, parent_rows, mask_words, max_rows;
+} quic_block_tables_t;
+
 /* What a step needs to know of its requests, built on the device from their
  * lengths.  n_new[b] > 0: request b gets that many rows behind lengths[b] cached
  * tokens, and from the pool the blocks that it needs for them beyond its held[b]
@@ -377,14 +393,7 @@ int64_t quic_tree_attn_scratch_bytes(int32_t requests, int32_t heads,
  * (status -2), no request gets rows or blocks: row_start is all 0.  Ended requests give theirs back all the
  * same.  Status 0: done.  A pool serves one stream at a time.  At most 4096
  * requests and 65535 * 256 rows.  Positions reach 2^29 at most. */
-int quic_block_tables(int32_t *tables, int64_t table_row, int32_t max_blocks,
-                      int32_t *held, int32_t *pool, int32_t n_blocks,
-                      const int32_t *lengths, const int32_t *n_new,
-                      int32_t requests, int32_t block_size,
-                      const int32_t *parents, int32_t parent_rows,
-                      int32_t *row_start,
-                      int64_t *slot_map, int32_t *positions, int32_t *mask,
-                      int32_t mask_words, int32_t max_rows, void *stream);
+int quic_block_tables(const quic_block_tables_t *t, void *stream);
 
 typedef struct {
   /* [layers, 2 (K, V), n_blocks, kv_heads, block_size, dim] of 2-byte elements,

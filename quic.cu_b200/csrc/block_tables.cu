@@ -193,20 +193,22 @@ __global__ void __launch_bounds__(kThreads) block_tables_kernel(const TablesArgs
 
 using namespace quic;
 
-extern "C" int quic_block_tables(int32_t* tables, int64_t table_row, int32_t max_blocks, int32_t* held, int32_t* pool,
-                                 int32_t n_blocks, const int32_t* lengths, const int32_t* n_new, int32_t requests,
-                                 int32_t block_size, const int32_t* parents, int32_t parent_rows, int32_t* row_start, int64_t* slot_map,
-                                 int32_t* positions, int32_t* mask, int32_t mask_words, int32_t max_rows, void* stream) {
-  QUIC_REQUIRE(tables && held && pool && lengths && n_new && row_start, QUIC_E_ARG, "block_tables: null tensor");
-  QUIC_REQUIRE(max_rows >= 0 && (max_rows == 0 || (slot_map && positions)), QUIC_E_ARG, "block_tables: null tensor");
-  QUIC_REQUIRE(parents == nullptr || (mask_words >= 1 && parent_rows >= 0 && (mask || max_rows == 0)), QUIC_E_ARG, "block_tables: parents without a mask");
-  QUIC_REQUIRE(requests >= 1 && max_blocks >= 1 && n_blocks >= 0 && block_size >= 1 && n_blocks < (1 << 30) &&
-                   (int64_t)max_blocks * block_size <= kMostPositions,
+extern "C" int quic_block_tables(const quic_block_tables_t* t, void* stream) {
+  QUIC_REQUIRE(t != nullptr && t->tables && t->held && t->pool && t->lengths && t->n_new && t->row_start, QUIC_E_ARG,
+               "block_tables: null tensor");
+  QUIC_REQUIRE(t->max_rows >= 0 && (t->max_rows == 0 || (t->slot_map && t->positions)), QUIC_E_ARG, "block_tables: null tensor");
+  QUIC_REQUIRE(t->parents == nullptr || (t->mask_words >= 1 && t->parent_rows >= 0 && (t->mask || t->max_rows == 0)), QUIC_E_ARG,
+               "block_tables: parents without a mask");
+  QUIC_REQUIRE(t->requests >= 1 && t->max_blocks >= 1 && t->n_blocks >= 0 && t->block_size >= 1 && t->n_blocks < (1 << 30) &&
+                   (int64_t)t->max_blocks * t->block_size <= kMostPositions,
                QUIC_E_SHAPE, "block_tables: bad request count or block geometry");
-  QUIC_REQUIRE(requests <= kMostRequests && max_rows <= 65535 * 256, QUIC_E_LIMIT, "block_tables: more than 4096 requests, or too many rows");
-  TablesArgs a = {tables, held, pool, row_start, positions, mask, slot_map, lengths, n_new, parents, table_row,
-                  max_blocks, n_blocks, requests, block_size, mask_words, max_rows,
-                  parents != nullptr && parent_rows < max_rows ? parent_rows : max_rows};
+  QUIC_REQUIRE(t->requests <= kMostRequests && t->max_rows <= 65535 * 256, QUIC_E_LIMIT,
+               "block_tables: more than 4096 requests, or too many rows");
+  const int32_t requests = t->requests, max_rows = t->max_rows, mask_words = t->mask_words;
+  const int32_t* const parents = t->parents;
+  const TablesArgs a = {t->tables, t->held, t->pool, t->row_start, t->positions, t->mask, t->slot_map, t->lengths, t->n_new, parents,
+                        t->table_row, t->max_blocks, t->n_blocks, requests, t->block_size, mask_words, max_rows,
+                        parents != nullptr && t->parent_rows < max_rows ? t->parent_rows : max_rows};
   const int64_t work = (int64_t)max_rows * (parents != nullptr ? mask_words : 1);
   int64_t ctas = (work + 4 * kThreads - 1) / (4 * kThreads);
   ctas = ctas < 1 ? 1 : (ctas > 148 * 4 ? 148 * 4 : ctas);

@@ -183,7 +183,7 @@ SIGNATURES = {
     "quic_decode_persist_status": (C.c_int, [_P, _P, C.POINTER(_I32)]),
     "quic_tree_attn": (C.c_int, [_P, _P, _P]),
     "quic_tree_attn_scratch_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I64]),
-    "quic_block_tables": (C.c_int, [_P, _I64, _I32, _P, _P, _I32, _P, _P, _I32, _I32, _P, _I32, _P, _P, _P, _P, _I32, _I32, _P]),
+    "quic_block_tables": (C.c_int, [_P, _P]),
     "quic_tree_commit": (C.c_int, [_P, _P]),
     "quic_qkv_rope_append_at": (C.c_int, [_P, _P, _P, _P, _P, _I32, _P, _P, _P, _I32, _I32, _I32, _P]),
     "quic_decode_persist_run_host": (C.c_int, [C.POINTER(Model), C.POINTER(Decode), _P, _P, _I32, _P, _P, _P, _I32,
@@ -727,17 +727,20 @@ def _on(device: int):
 
 def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
     device = first.get_device()
+    if device < 0:
+        raise RuntimeError("quic_b200: CUDA tensors required (no CPU path)")
     for t in others:
         if t is not None and t.get_device() != device:
             raise RuntimeError("quic_b200: CUDA tensors of one device required (no CPU path)")
-    if device < 0:
-        raise RuntimeError("quic_b200: CUDA tensors required (no CPU path)")
     return device
 
 
 _TREE_TYPES = {torch.float16: 0, torch.bfloat16: 1}
+# (a struct's bytes cross to C in a third of the time that ctypes takes for as many arguments)
 _TREE_ATTN = struct.Struct("=4Q8qQqQQQq11i4xqf4x")  # quic_tree_attn_t
 _TREE_COMMIT = struct.Struct("=Q5qQq5Q10i4Q")       # quic_tree_commit_t
+_BLOCK_TABLES = struct.Struct("=Qq10Q7i4x")         # quic_block_tables_t
+_I32_TYPE = torch.int32
 
 
 @functools.lru_cache(maxsize=4096)
@@ -760,53 +763,70 @@ def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, table
     (None: what the tables hold); both only plan the launch, tight bounds make it faster.  Returns [rows, heads, dim]
     (``out`` if given, contiguous; rows outside row_start[0] .. row_start[-1] - 1 stay as they were): rows that see nothing
     are zero."""
-    dtype = _TREE_TYPES.get(q.dtype)
-    if dtype is None or kcache.dtype != q.dtype or vcache.dtype != q.dtype:
+    kind = q.dtype
+    dtype = _TREE_TYPES.get(kind)
+    if dtype is None or kcache.dtype is not kind or vcache.dtype is not kind:
         raise RuntimeError("tree_attn: q, kcache and vcache must be of one type, fp16 or bf16")
-    if q.dim() != 3 or kcache.dim() != 4 or kcache.shape != vcache.shape:
+    qs, kshape, tshape = q.shape, kcache.shape, tables.shape
+    if len(qs) != 3 or len(kshape) != 4 or vcache.shape != kshape:
         raise RuntimeError("tree_attn: expected q [rows, heads, dim] and planes [blocks, KV heads, block size, dim]")
-    rows, heads, dim = q.shape
-    blocks, kv_heads, block, kv_dim = kcache.shape
-    if dim not in (64, 128) or kv_dim != dim or kv_heads < 1 or heads < 1 or heads % kv_heads:
+    rows, heads, dim = qs
+    blocks, kv_heads, block, kv_dim = kshape
+    if (dim != 64 and dim != 128) or kv_dim != dim or kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise RuntimeError("tree_attn: the head dimension is 64 or 128, the query heads a multiple of the KV heads")
-    if tables.dim() != 2 or lengths.dim() != 1 or row_start.dim() != 1:
+    if len(tshape) != 2 or lengths.shape != tshape[:1] or row_start.dim() != 1 or row_start.shape[0] != tshape[0] + 1:
         raise RuntimeError("tree_attn: expected tables [requests, blocks], lengths [requests], row_start [requests + 1]")
-    requests, width = tables.shape
-    if lengths.shape[0] != requests or row_start.shape[0] != requests + 1:
-        raise RuntimeError("tree_attn: expected tables [requests, blocks], lengths [requests], row_start [requests + 1]")
-    if not (tables.dtype is lengths.dtype is row_start.dtype is torch.int32) or (mask is not None and mask.dtype is not torch.int32):
+    requests, width = tshape
+    if not (tables.dtype is lengths.dtype is row_start.dtype is _I32_TYPE):
         raise RuntimeError("tree_attn: tables, lengths, row_start and mask must be int32")
-    qs, ks, vs, ts = q.stride(), kcache.stride(), vcache.stride(), tables.stride()
-    if (qs[2] != 1 or ks[3] != 1 or vs[3] != 1 or (ts[1] != 1 and width > 1) or not lengths.is_contiguous() or
+    q0, q1, q2 = q.stride()
+    k0, k1, k2, k3 = kcache.stride()
+    v0, v1, v2, v3 = vcache.stride()
+    t0, t1 = tables.stride()
+    if (q2 != 1 or k3 != 1 or v3 != 1 or (t1 != 1 and width > 1) or not lengths.is_contiguous() or
             not row_start.is_contiguous()):
         raise RuntimeError("tree_attn: the last dimension of every tensor must be contiguous")
     words = mask_row = mask_ptr = 0
     if mask is not None:
-        if mask.dim() != 2 or mask.shape[0] != rows or mask.shape[1] < 1 or (mask.stride(1) != 1 and mask.shape[1] > 1):
+        mshape = mask.shape
+        if mask.dtype is not _I32_TYPE:
+            raise RuntimeError("tree_attn: tables, lengths, row_start and mask must be int32")
+        if len(mshape) != 2 or mshape[0] != rows or mshape[1] < 1 or (mask.stride(1) != 1 and mshape[1] > 1):
             raise RuntimeError("tree_attn: mask must be [rows, words], its words contiguous")
-        words, mask_row, mask_ptr = mask.shape[1], mask.stride(0), mask.data_ptr()
-    device = _same_device(q, kcache, vcache, tables, lengths, row_start, mask, out)
+        words, mask_row, mask_ptr = mshape[1], mask.stride(0), mask.data_ptr()
+    device = q.get_device()
+    if (device < 0 or kcache.get_device() != device or vcache.get_device() != device or tables.get_device() != device or
+            lengths.get_device() != device or row_start.get_device() != device or
+            (mask is not None and mask.get_device() != device)):
+        _same_device(q, kcache, vcache, tables, lengths, row_start, mask)
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        out = q.new_empty(rows, heads, dim)
+    elif out.shape != qs or out.dtype is not kind or not out.is_contiguous():
         raise RuntimeError("tree_attn: out must be contiguous [rows, heads, dim] of q's type")
+    else:
+        _same_device(q, out)
     if rows == 0 or requests == 0:
         return out
-    if width < 1 or blocks < 1 or block < 1:
+    room = width * block
+    if room < 1 or blocks < 1:
         raise RuntimeError("tree_attn: no blocks")
-    max_new = rows if max_new is None else min(max_new, rows)
-    max_len = width * block if max_len is None else min(max_len, width * block)
+    if max_new is None or max_new > rows:
+        max_new = rows
+    if max_len is None or max_len > room:
+        max_len = room
     if max_new < 1 or max_len < 0:
         raise RuntimeError("tree_attn: max_new must be positive and max_len not negative")
     need = _tree_scratch_bytes(requests, heads, kv_heads, dim, max_new, max_len)
     stream = _raw_stream(device)
     scratch = _thread_scratch(("tree", device, stream), need, 1 << 20, 0).data_ptr() if need > 0 else None
-    call = _TREE_ATTN.pack(q.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), out.data_ptr(), qs[0], qs[1], ks[0], ks[1], ks[2],
-                           vs[0], vs[1], vs[2], tables.data_ptr(), ts[0], lengths.data_ptr(), row_start.data_ptr(), mask_ptr,
-                           mask_row, words, rows, requests, heads, kv_heads, dim, blocks, block, width, dtype, max_new,
-                           max_len, softmax_scale)
-    with _on(device):
+    call = _TREE_ATTN.pack(q.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), out.data_ptr(), q0, q1, k0, k1, k2, v0, v1, v2,
+                           tables.data_ptr(), t0, lengths.data_ptr(), row_start.data_ptr(), mask_ptr, mask_row, words, rows,
+                           requests, heads, kv_heads, dim, blocks, block, width, dtype, max_new, max_len, softmax_scale)
+    if torch.cuda.current_device() == device:
         rc = lib().quic_tree_attn(call, scratch, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = lib().quic_tree_attn(call, scratch, stream)
     if rc != 0:
         check(rc, "tree_attn")
     return out
@@ -840,40 +860,49 @@ def block_tables(tables: torch.Tensor, held: torch.Tensor, pool: torch.Tensor, l
     All or nothing: pool[3] is 0, or the number of blocks that the pool lacks, or -1 (a request needs more blocks than
     its table row has) or -2 (more rows than max_rows or parents, or than the mask has bits): then no request gets rows or
     blocks and row_start is all zero, which the operators that read it take for no work.  A pool belongs to one stream at a time."""
-    if any(t.dtype is not torch.int32 for t in (tables, held, pool, lengths, n_new)) or (parents is not None and parents.dtype is not torch.int32):
+    if not (tables.dtype is held.dtype is pool.dtype is lengths.dtype is n_new.dtype is _I32_TYPE):
         raise RuntimeError("block_tables: tables, held, pool, lengths, n_new and parents must be int32")
-    if tables.dim() != 2 or tables.shape[1] < 1 or (tables.stride(1) != 1 and tables.shape[1] > 1) or \
-            (tables.shape[0] > 1 and tables.stride(0) < tables.shape[1]):
+    tshape = tables.shape
+    if len(tshape) != 2 or tshape[1] < 1 or (tables.stride(1) != 1 and tshape[1] > 1) or \
+            (tshape[0] > 1 and tables.stride(0) < tshape[1]):
         raise RuntimeError("block_tables: tables must be [requests, blocks], rows contiguous")
-    requests, width = tables.shape
-    if any(t.shape != (requests,) or not t.is_contiguous() for t in (held, lengths, n_new)):
+    requests, width = tshape
+    one = tshape[:1]
+    if held.shape != one or lengths.shape != one or n_new.shape != one or not (held.is_contiguous() and lengths.is_contiguous() and
+                                                                             n_new.is_contiguous()):
         raise RuntimeError("block_tables: held, lengths and n_new must be contiguous [requests]")
     if pool.dim() != 1 or pool.shape[0] < 4 or not pool.is_contiguous():
         raise RuntimeError("block_tables: pool must be contiguous [4 + blocks]")
-    if max_rows < 0 or (parents is not None and (parents.dim() != 1 or not parents.is_contiguous())):
-        raise RuntimeError("block_tables: max_rows must not be negative, parents contiguous [rows]")
-    device = _same_device(tables, held, pool, lengths, n_new, parents)
-    where = tables.device
-    words = 0
+    if max_rows < 0:
+        raise RuntimeError("block_tables: max_rows must not be negative")
+    words = parent_rows = parent_ptr = mask_ptr = 0
+    mask = None
     if parents is not None:
+        if parents.dtype is not _I32_TYPE:
+            raise RuntimeError("block_tables: tables, held, pool, lengths, n_new and parents must be int32")
+        if parents.dim() != 1 or not parents.is_contiguous():
+            raise RuntimeError("block_tables: parents must be contiguous [rows]")
         words = -(-(max_rows if max_new is None else max_new) // 32) or 1
         if words < 1:
             raise RuntimeError("block_tables: max_new must not be negative")
-    # one allocation, the parts at multiples of 8 bytes
-    cut = (requests + 2) // 2 * 2
-    room = torch.empty(2 * max_rows + cut + (max_rows + 1) // 2 * 2 + max_rows * words, dtype=torch.int32, device=where)
-    slot_map = room[:2 * max_rows].view(torch.int64)
-    row_start = room[2 * max_rows:2 * max_rows + requests + 1]
-    at = 2 * max_rows + cut
-    positions = room[at:at + max_rows]
-    at += (max_rows + 1) // 2 * 2
-    mask = room[at:].view(max_rows, words) if parents is not None else None
-    with _on(device):
-        rc = lib().quic_block_tables(tables.data_ptr(), tables.stride(0), width, held.data_ptr(), pool.data_ptr(), pool.shape[0] - 4,
-                                     lengths.data_ptr(), n_new.data_ptr(), requests, block_size, ptr(parents),
-                                     0 if parents is None else parents.shape[0],
-                                     row_start.data_ptr(), slot_map.data_ptr(), positions.data_ptr(), ptr(mask), words, max_rows,
-                                     _raw_stream(device))
+        parent_rows, parent_ptr = parents.shape[0], parents.data_ptr()
+    device = tables.get_device()
+    if (device < 0 or held.get_device() != device or pool.get_device() != device or lengths.get_device() != device or
+            n_new.get_device() != device or (parents is not None and parents.get_device() != device)):
+        _same_device(tables, held, pool, lengths, n_new, parents)
+    if parents is not None:
+        mask = held.new_empty(max_rows, words)
+        mask_ptr = mask.data_ptr()
+    slot_map = torch.empty(max_rows, dtype=torch.int64, device=tables.device)
+    row_start, positions = held.new_empty(requests + 1 + max_rows).split((requests + 1, max_rows))
+    call = _BLOCK_TABLES.pack(tables.data_ptr(), tables.stride(0), held.data_ptr(), pool.data_ptr(), lengths.data_ptr(),
+                              n_new.data_ptr(), parent_ptr, row_start.data_ptr(), slot_map.data_ptr(), positions.data_ptr(),
+                              mask_ptr, 0, width, pool.shape[0] - 4, requests, block_size, parent_rows, words, max_rows)
+    if torch.cuda.current_device() == device:
+        rc = lib().quic_block_tables(call, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = lib().quic_block_tables(call, _raw_stream(device))
     if rc != 0:
         check(rc, "block_tables")
     return row_start, slot_map, positions, mask
@@ -888,13 +917,15 @@ def tree_commit(kv: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, r
     [b] cached tokens.  Returns (path int32 [requests, max_new], the accepted nodes and -1 behind them; accepted int32
     [requests]; next_token [requests], the target's choice after the last of them, -1 for a request without rows; new_lengths
     int32 [requests]).  Requests with more than ``max_new`` (at most 1024) rows are left alone."""
-    if kv.dim() != 6 or kv.shape[1] != 2 or kv.element_size() != 2:
+    kvshape, tshape, one = kv.shape, tables.shape, tokens.shape
+    if len(kvshape) != 6 or kvshape[1] != 2 or kv.element_size() != 2:
         raise RuntimeError("tree_commit: kv must be [layers, 2, blocks, KV heads, block size, dim] of a 2-byte type")
-    if tables.dim() != 2 or lengths.dim() != 1 or row_start.dim() != 1 or tokens.dim() != 1:
+    if len(tshape) != 2 or lengths.dim() != 1 or row_start.dim() != 1 or len(one) != 1:
         raise RuntimeError("tree_commit: expected tables [requests, blocks], lengths [requests], row_start [requests + 1], tokens [rows]")
-    requests, width = tables.shape
-    rows = tokens.shape[0]
-    if lengths.shape[0] != requests or row_start.shape[0] != requests + 1 or targets.shape != (rows,) or parents.shape != (rows,):
+    layers, _, blocks, kv_heads, block, dim = kvshape
+    requests, width = tshape
+    rows = one[0]
+    if lengths.shape[0] != requests or row_start.shape[0] != requests + 1 or targets.shape != one or parents.shape != one:
         raise RuntimeError("tree_commit: tables, lengths and row_start, or parents, tokens and targets do not match")
     if not (tables.dtype is lengths.dtype is row_start.dtype is parents.dtype is torch.int32):
         raise RuntimeError("tree_commit: tables, lengths, row_start and parents must be int32")
@@ -905,21 +936,25 @@ def tree_commit(kv: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, r
                                                                  parents.is_contiguous() and tokens.is_contiguous() and
                                                                  targets.is_contiguous()):
         raise RuntimeError("tree_commit: the last dimension of every tensor must be contiguous")
-    if kv.numel() == 0 or width < 1:
+    if width < 1 or 0 in kvshape:
         raise RuntimeError("tree_commit: no blocks")
-    device = _same_device(kv, tables, lengths, row_start, parents, tokens, targets)
-    wide = 2 if tokens.dtype is torch.int64 else 1
-    # one allocation: next_token first, where it is aligned
-    room = torch.empty(requests * (wide + 2 + max(max_new, 0)), dtype=torch.int32, device=kv.device)
-    next_token = room[:wide * requests].view(tokens.dtype)
-    accepted, new_lengths = room[wide * requests:(wide + 1) * requests], room[(wide + 1) * requests:(wide + 2) * requests]
-    path = room[(wide + 2) * requests:].view(requests, max(max_new, 0))
+    device = kv.get_device()
+    if (device < 0 or tables.get_device() != device or lengths.get_device() != device or row_start.get_device() != device or
+            parents.get_device() != device or tokens.get_device() != device or targets.get_device() != device):
+        _same_device(kv, tables, lengths, row_start, parents, tokens, targets)
+    if max_new < 1:
+        raise RuntimeError("tree_commit: max_new must be positive")
+    next_token, path = tokens.new_empty(requests), lengths.new_empty(requests, max_new)
+    accepted, new_lengths = lengths.new_empty(2, requests).unbind()
     call = _TREE_COMMIT.pack(kv.data_ptr(), s[0], s[1], s[2], s[3], s[4], tables.data_ptr(), tables.stride(0), lengths.data_ptr(),
-                             row_start.data_ptr(), parents.data_ptr(), tokens.data_ptr(), targets.data_ptr(), 4 * wide, kv.shape[0],
-                             kv.shape[2], kv.shape[3], kv.shape[4], kv.shape[5], width, rows, requests, max_new,
-                             path.data_ptr(), accepted.data_ptr(), next_token.data_ptr(), new_lengths.data_ptr())
-    with _on(device):
+                             row_start.data_ptr(), parents.data_ptr(), tokens.data_ptr(), targets.data_ptr(),
+                             8 if tokens.dtype is torch.int64 else 4, layers, blocks, kv_heads, block, dim, width, rows, requests,
+                             max_new, path.data_ptr(), accepted.data_ptr(), next_token.data_ptr(), new_lengths.data_ptr())
+    if torch.cuda.current_device() == device:
         rc = lib().quic_tree_commit(call, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = lib().quic_tree_commit(call, _raw_stream(device))
     if rc != 0:
         check(rc, "tree_commit")
     return path, accepted, next_token, new_lengths

@@ -1,8 +1,6 @@
 """What tree_attn, block_tables, tree_commit and qkv_rope_append_at refuse, without a GPU: shapes, types and strides by the
 Python layer, sizes and alignments by the C entry points before any launch."""
 
-import ctypes as C
-
 import pytest
 import torch
 
@@ -53,6 +51,7 @@ def _tables(**more):
 @pytest.mark.parametrize("more,match", [
     ({}, "CUDA tensors"),
     (dict(held=torch.zeros(2).long()), "int32"),
+    
     (dict(parents=torch.zeros(4).long()), "int32"),
     (dict(parents=torch.zeros(3, 1, **I32)), "parents"),
     (dict(tables=torch.zeros(2, 0, **I32)), "tables must be"),
@@ -150,10 +149,9 @@ def test_commit_entry_point_refuses():
 
 
 def test_tables_entry_point_refuses():
-    def call(requests=2, block=16, max_rows=4, n_blocks=5, max_blocks=3, parents=None, words=0, tables=4096):
-        p = C.c_void_p(4096)
-        return K.lib().quic_block_tables(tables, 3, max_blocks, p, p, n_blocks, p, p, requests, block, parents, 4, p, p, p, None, words,
-                                         max_rows, None)
-    assert call(tables=None) == -1 and call(parents=4096) == -1 and call(parents=4096, words=1) == -1
+    def call(requests=2, block=16, max_rows=4, n_blocks=5, max_blocks=3, parents=0, words=0, tables=4096):
+        values = (tables, 3, 4096, 4096, 4096, 4096, parents, 4096, 4096, 4096, 0, 0, max_blocks, n_blocks, requests, block, 4, words, max_rows)
+        return K.lib().quic_block_tables(K._BLOCK_TABLES.pack(*values), None)
+    assert call(tables=0) == -1 and call(parents=4096) == -1 and call(parents=4096, words=1) == -1
     assert call(requests=0) == -2 and call(block=0) == -2 and call(max_blocks=0) == -2 and call(n_blocks=-1) == -2
     assert call(requests=4097) == -4 and call(max_rows=1 << 25) == -4 and call(block=1 << 20, max_blocks=1 << 10) == -2
