@@ -7,17 +7,6 @@
 
 namespace quic {
 
-// Division of 0 .. 2^31 - 1 by a divisor that the host knows (Granlund and Montgomery 1994): a multiplication and a shift.
-struct FastDiv {
-  uint32_t d, magic, shift;
-  __host__ static FastDiv of(uint32_t d) {
-    uint32_t l = 0;
-    while ((1ull << l) < d) ++l;
-    return {d, (uint32_t)((((1ull << l) - d) << 32) / d + 1), l};
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, magic) + n) >> shift; }
-};
-
 struct TreeArgs {
   const void* q;                     // [rows][heads][dim] by strides, in elements
   const void *k, *v;                 // [n_blocks][kv heads][block][dim] by strides, in elements

@@ -24,6 +24,8 @@ __global__ void __launch_bounds__(kThreads) tree_commit_kernel(const quic_tree_c
   int32_t* const parent_s = reinterpret_cast<int32_t*>(target_s + t.max_new);
   int32_t* const path_s = parent_s + t.max_new;
   __shared__ int accepted_s;
+  pdl_launch_dependents();
+  pdl_wait();
   const int start = min(max(t.row_start[b], 0), t.rows), end = min(t.row_start[b + 1], t.rows);
   const int len = t.lengths[b];
   int n = end - start;
@@ -138,6 +140,6 @@ extern "C" int quic_tree_commit(const quic_tree_commit_t* t, void* stream) {
   const int64_t planes = (int64_t)t->layers * 2 * t->kv_heads;
   const int64_t ctas = (planes + kThreads / 32 - 1) / (kThreads / 32);
   QUIC_CUDA(launch(tree_commit_kernel, dim3((unsigned)(ctas > 256 ? 256 : ctas), t->requests), dim3(kThreads), (size_t)t->max_new * 24,
-                   (cudaStream_t)stream, false, *t));
+                   (cudaStream_t)stream, true, *t));
   return QUIC_OK;
 }
