@@ -9,7 +9,7 @@
 //
 // This file: the form for few rows (mma.sync), the merge of a request's parts, and the entry point; tree_attn_tc.cu has the form
 // for more rows.
-// A CTA has 16 or 32 rows and a part of the keys, which its four warps walk 32 at a time, each through a ring of its own
+// A CTA has 16 or 32 rows and a part of the keys, which its four warps walk 32 (16 of 128 dims) at a time, each through a ring of its own
 // (cp.async, no barrier between warps), one pass with a running maximum and sum per row; the warps' results meet in
 // shared memory at the end, those of several CTAs in the merge kernel.  Bound: the bytes of K and V.
 #include <math.h>
@@ -19,7 +19,7 @@
 namespace quic {
 namespace {
 
-constexpr int kWarps = 4, kKeys = 32;
+constexpr int kWarps = 4;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {  // zeros beyond `bytes`
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -51,14 +51,18 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Keys of a warp's tile (8 KB of K and V) and tiles of its ring: two CTAs an SM with two tiles a warp under way (with tiles of 32
+// keys for 128 dims too, one CTA fitted an SM).
 template <int D>
-constexpr int kStages = D == 64 ? 3 : 2;
-template <int D>
-constexpr uint32_t kRowsBytes = kKeys * D * 2;                       // K (or V) of a tile
+constexpr int kTileKeys = D == 64 ? 32 : 16;
+#ifndef FEW_STAGES
+#define FEW_STAGES 3
+#endif
+constexpr int kStages = FEW_STAGES;
+constexpr uint32_t kRowsBytes = 32 * 64 * 2;                         // K (or V) of a tile
 template <int D, int MT>
-constexpr uint32_t kSmem = kWarps * kStages<D> * 2 * kRowsBytes<D> > kWarps * MT * 16 * (D + 4) * 4
-                               ? kWarps * kStages<D> * 2 * kRowsBytes<D>
-                               : kWarps * MT * 16 * (D + 4) * 4;
+constexpr uint32_t kSmem = kWarps * kStages * 2 * kRowsBytes > kWarps * MT * 16 * (D + 4) * 4 ? kWarps * kStages * 2 * kRowsBytes
+                                                                                              : kWarps * MT * 16 * (D + 4) * 4;
 
 // Tile element (row, 16-byte chunk): chunks swapped by row so that eight rows of a chunk lie in different banks.
 template <int D>
@@ -68,8 +72,9 @@ __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
 
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a) {
+  constexpr int kKeys = kTileKeys<D>;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ uint32_t valid_s[kWarps][kStages<D>];
+  __shared__ uint32_t valid_s[kWarps][kStages];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, kvh = blockIdx.y % a.kv_heads, tile = blockIdx.y / a.kv_heads;
   pdl_wait();
@@ -103,20 +108,21 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
     }
 
   // ---- the warp's ring
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * kStages<D> * 2 * kRowsBytes<D>;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * kStages * 2 * kRowsBytes;
   constexpr int kPer = D / 8, kAtOnce = 32 / kPer;  // chunks of a row, rows of one instruction
   const int step = kWarps * kKeys;
+  constexpr uint32_t kAllKeys = 0xffffffffu >> (32 - kKeys);
   // the block of position t + lane, or -1 where there is none
   auto fetch = [&](int t) {
-    const int p = t + lane;
+    const int p = t + (lane & (kKeys - 1));
     const int id = p < t_end ? __ldg(table + a.block.div(p)) : -1;
     return id < a.n_blocks ? id : -1;
   };
   auto request = [&](int t, int stage, int id) {
-    const uint32_t ok = __ballot_sync(0xffffffffu, id >= 0);
+    const uint32_t ok = __ballot_sync(0xffffffffu, id >= 0) & kAllKeys;
     if (lane == 0) valid_s[warp][stage] = ok;
-    const int p = t + lane, off = p - (int)a.block.div(p) * (int)a.block.d;
-    const uint32_t dst = ring + stage * 2 * kRowsBytes<D>;
+    const int p = t + (lane & (kKeys - 1)), off = p - (int)a.block.div(p) * (int)a.block.d;
+    const uint32_t dst = ring + stage * 2 * kRowsBytes;
     const int chunk = lane % kPer;
 #pragma unroll
     for (int i = 0; i < kKeys / kAtOnce; ++i) {
@@ -127,7 +133,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
       const uint32_t bytes = bid >= 0 ? 16u : 0u;
       cp_async16(dst + tile_at<D>(row, chunk), reinterpret_cast<const T*>(a.k) + at * a.k_block + kvh * a.k_head + o * a.k_tok + chunk * 8,
                  bytes);
-      cp_async16(dst + kRowsBytes<D> + tile_at<D>(row, chunk),
+      cp_async16(dst + kRowsBytes + tile_at<D>(row, chunk),
                  reinterpret_cast<const T*>(a.v) + at * a.v_block + kvh * a.v_head + o * a.v_tok + chunk * 8, bytes);
     }
   };
@@ -144,7 +150,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
   const int t_warp = t_begin + warp * kKeys;
   int id = fetch(t_warp);
 #pragma unroll
-  for (int s = 0; s < kStages<D> - 1; ++s) {
+  for (int s = 0; s < kStages - 1; ++s) {
     if (t_warp + s * step < t_end) request(t_warp + s * step, s, id);
     asm volatile("cp.async.commit_group;" ::: "memory");
     id = fetch(t_warp + (s + 1) * step);
@@ -152,15 +158,15 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
   int stage = 0;
   for (int t = t_warp; t < t_end; t += step) {
     {
-      const int ahead = t + (kStages<D> - 1) * step;
-      const int to = stage == 0 ? kStages<D> - 1 : stage - 1;
+      const int ahead = t + (kStages - 1) * step;
+      const int to = stage == 0 ? kStages - 1 : stage - 1;
       if (ahead < t_end) request(ahead, to, id);
       asm volatile("cp.async.commit_group;" ::: "memory");
       id = fetch(ahead + step);
     }
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages<D> - 1) : "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
     __syncwarp();
-    const uint32_t k_at = ring + stage * 2 * kRowsBytes<D>, v_at = k_at + kRowsBytes<D>;
+    const uint32_t k_at = ring + stage * 2 * kRowsBytes, v_at = k_at + kRowsBytes;
     const uint32_t valid = valid_s[warp][stage];
 
     // S = Q K^T
@@ -183,7 +189,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
       }
 
     // what each row sees
-    const bool tree = t + kKeys > r.len, masked = tree || valid != 0xffffffffu;
+    const bool tree = t + kKeys > r.len, masked = tree || valid != kAllKeys;
     uint32_t seen[MT][2];
     if (masked) {
 #pragma unroll
@@ -287,7 +293,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
         }
       }
     __syncwarp();  // (the stage is requested anew in the next round)
-    stage = stage == kStages<D> - 1 ? 0 : stage + 1;
+    stage = stage == kStages - 1 ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   pdl_launch_dependents();
@@ -445,7 +451,7 @@ Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound
     return p;
   }
   bound = bound < kMostTokens ? bound : kMostTokens;
-  const int64_t units = (int64_t)requests * kv_heads * p.tiles, slots = 148 * (dim == 64 ? 2 : 1);
+  const int64_t units = (int64_t)requests * kv_heads * p.tiles, slots = 148 * 2;
   int64_t best = 1, least = INT64_MAX;
   for (int64_t s = 1; s <= 128 && (s == 1 || (s - 1) * 256 < bound); ++s) {
     const int64_t part = ((bound + s - 1) / s + 63) / 64 * 64;

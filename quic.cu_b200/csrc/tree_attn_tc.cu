@@ -29,7 +29,7 @@ namespace {
 
 constexpr int kRows = 128, kKeys = 64, kGroupWarps = 4, kSoftmaxWarps = 2 * kGroupWarps;
 constexpr int kTmaWarp = kSoftmaxWarps + 2, kThreads = (kTmaWarp + 2) * 32;
-constexpr int kLeastShare = 4;  // key tiles of a CTA
+constexpr int kLeastShare = 2;  // key tiles of a CTA
 static_assert(2 * kRows == kTreeTcRows && kKeys == kTreeTcKeys, "two streams of rows");
 constexpr float kGrowth = 8.f;    // of a row's maximum (base 2) before its reference point follows
 template <typename T>

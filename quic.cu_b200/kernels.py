@@ -894,7 +894,7 @@ def block_tables(tables: torch.Tensor, held: torch.Tensor, pool: torch.Tensor, l
         mask = held.new_empty(max_rows, words)
         mask_ptr = mask.data_ptr()
     slot_map = torch.empty(max_rows, dtype=torch.int64, device=tables.device)
-    row_start, positions = held.new_empty(requests + 1 + max_rows).split((requests + 1, max_rows))
+    row_start, positions = held.new_empty(requests + 1), held.new_empty(max_rows)
     call = _BLOCK_TABLES.pack(tables.data_ptr(), tables.stride(0), held.data_ptr(), pool.data_ptr(), lengths.data_ptr(),
                               n_new.data_ptr(), parent_ptr, row_start.data_ptr(), slot_map.data_ptr(), positions.data_ptr(),
                               mask_ptr, 0, width, pool.shape[0] - 4, requests, block_size, parent_rows, words, max_rows)
@@ -945,7 +945,7 @@ def tree_commit(kv: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, r
     if max_new < 1:
         raise RuntimeError("tree_commit: max_new must be positive")
     next_token, path = tokens.new_empty(requests), lengths.new_empty(requests, max_new)
-    accepted, new_lengths = lengths.new_empty(2, requests).unbind()
+    accepted, new_lengths = lengths.new_empty(requests), lengths.new_empty(requests)
     call = _TREE_COMMIT.pack(kv.data_ptr(), s[0], s[1], s[2], s[3], s[4], tables.data_ptr(), tables.stride(0), lengths.data_ptr(),
                              row_start.data_ptr(), parents.data_ptr(), tokens.data_ptr(), targets.data_ptr(),
                              8 if tokens.dtype is torch.int64 else 4, layers, blocks, kv_heads, block, dim, width, rows, requests,
