@@ -371,6 +371,11 @@ typedef struct {
   int32_t max_blocks, n_blocks, requests, block_size, parent_rows, mask_words, max_rows;
 } quic_block_tables_t;
 
+/* Which of its two forms quic_tree_attn runs: -1 (default) whichever is faster
+ * by the sizes, 0 the mma.sync form, 1 the tcgen05 form where blocks (a multiple
+ * of 8 tokens) and strides (positive) allow it.  For A/B timing and tests. */
+void quic_set_tree_attn_tensor(int mode);
+
 /* What a step needs to know of its requests, built on the device from their
  * lengths.  n_new[b] > 0: request b gets that many rows behind lengths[b] cached
  * tokens, and from the pool the blocks that it needs for them beyond its held[b]

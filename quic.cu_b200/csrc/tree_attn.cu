@@ -367,7 +367,10 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a) {
   if constexpr (kTc) {  // the CTA where the row tile begins has it as its last segment, the others as their first
     const TreeUnits u = tree_units(a, r);
     const int64_t share = a.first[a.requests + 1], t0 = a.first[blockIdx.z] + ((int64_t)kvh * u.row_tiles + tile) * u.key_tiles;
-    const int64_t c0 = t0 / share, c1 = (t0 + u.key_tiles - 1) / share;
+    const int64_t t1 = t0 + u.key_tiles - 1;
+    const bool narrow = t1 <= 0xffffffffll;  // (a division of 64 bits takes as long as a round of loads)
+    const int64_t c0 = narrow ? (int64_t)((uint32_t)t0 / (uint32_t)share) : t0 / share;
+    const int64_t c1 = narrow ? (int64_t)((uint32_t)t1 / (uint32_t)share) : t1 / share;
     parts = (int)(c1 - c0) + 1;
     part0 = 2 * c0 + 1, part = 2 * c0, step = 2;
   } else {
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a) {
   if (parts == 1) return;
   float top = -INFINITY, l = 0.f;
   float4 o[4] = {};
-#pragma unroll 2
+#pragma unroll 4
   for (int s = warp; s < parts; s += 8) {  // running maximum and sum
     const int64_t at = s == 0 ? part0 : part + s * step;
     const float2 x = a.part_ml[at * a.tile_rows + row];
@@ -429,8 +432,20 @@ int launch_few(const TreeArgs& a, cudaStream_t st) {
 }
 
 constexpr int64_t kMostTokens = 1 << 29;  // of a request: sums of two counts stay within an int
-// Rows of a request and KV head beyond which the tcgen05 form takes a call.
-constexpr int64_t kFewRows = 32;
+// Which form takes a call, by the rows of a request and KV head and by the work of the mma.sync form, in tiles of 32 rows x keys of
+// 64 dims (for all requests, of the longest's keys).  The tcgen05 form has three times its throughput where it has the rows for it,
+// but 8 us more of launch, segments and merge.  us, mma.sync / tcgen05, fp16 or bf16:
+//   heads 14:2, dim 64:  5 requests x 23 nodes x 777 tokens 11.2 / 14.5 (48,000), 1 x 48 x 4096 14.3 / 18.3 (91,000),
+//                        64 x 8 x 1500 25.5 / 26.6 (386,000)
+//   heads 32:8, dim 128: 20 x 28 x 15 19.1 / 24.1 (55,000), 4 x 15 x 6146 54 / 26.5 (790,000), 8 x 64 x 16384 907 / 148
+//   heads 16:1, dim 128: 3 x 46 x 1488 22.4 / 17.1 (210,000)
+// Up to 32 rows it is ahead for long keys of 128 dims alone: 48 x 2 x 11707 (16:1) 65 / 52 (1,100,000); of 64 dims
+// 9 x 13 x 14495 (8:8) 44 / 66, 16 x 1 x 8192 (14:2) 19 / 29.
+bool tensor_pays(int64_t rows, int64_t units, int64_t bound, int dim) {
+  const int64_t work = units * ((rows + 31) / 32) * bound * (dim / 64);
+  if (rows > 32) return work > 150000;
+  return rows > 16 && dim == 128 && work > 700000;
+}
 
 struct Plan {
   bool tc;
@@ -439,10 +454,11 @@ struct Plan {
   int64_t parts;                   // partial results
 };
 // `bound`: keys of a request at most.
-Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound, int dim, bool tma) {
+Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound, int dim, bool tc) {
   Plan p = {};
+  p.tc = tc;
   const int64_t rows = (int64_t)max_new * (heads / kv_heads);
-  p.tc = tma && rows > kFewRows;
+  bound = bound < kMostTokens ? bound : kMostTokens;
   p.tile_rows = p.tc ? (int)(rows < kTreeTcRows ? (rows + 31) / 32 * 32 : kTreeTcRows) : 32;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   p.splits = 1;
@@ -450,7 +466,6 @@ Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound
     p.parts = 2 * kTreeTcCtas;
     return p;
   }
-  bound = bound < kMostTokens ? bound : kMostTokens;
   const int64_t units = (int64_t)requests * kv_heads * p.tiles, slots = 148 * 2;
   int64_t best = 1, least = INT64_MAX;
   for (int64_t s = 1; s <= 128 && (s == 1 || (s - 1) * 256 < bound); ++s) {
@@ -483,12 +498,15 @@ int launch_typed(const TreeArgs& a, const Plan& p, cudaStream_t st) {
 
 using namespace quic;
 
+static int g_tensor_mode = -1;
+extern "C" void quic_set_tree_attn_tensor(int mode) { g_tensor_mode = mode; }
+
 extern "C" int64_t quic_tree_attn_scratch_bytes(int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim, int32_t max_new,
                                                 int64_t max_len) {
   if (requests < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || (dim != 64 && dim != 128) || max_new < 1 || max_len < 0) return 0;
-  int64_t most = 0;  // (by either form: strides decide)
-  for (int tma = 0; tma < 2; ++tma) {
-    const Plan p = make_plan(requests, kv_heads, heads, max_new, max_len + max_new, dim, tma != 0);
+  int64_t most = 0;  // (of either form: strides decide too)
+  for (int tc = 0; tc < 2; ++tc) {
+    const Plan p = make_plan(requests, kv_heads, heads, max_new, max_len + max_new, dim, tc != 0);
     const int64_t need = first_bytes(p, requests) + p.parts * p.tile_rows * (dim + 2) * 4;
     most = need > most ? need : most;
   }
@@ -514,8 +532,11 @@ extern "C" int quic_tree_attn(const quic_tree_attn_t* t, void* scratch, void* st
   QUIC_REQUIRE((int64_t)t->rows * t->heads < (1ll << 31), QUIC_E_LIMIT, "tree_attn: rows times heads reach 2^31");
   const int max_new = t->max_new < t->rows ? t->max_new : t->rows;
   const int64_t room = (int64_t)t->max_blocks * t->block_size, max_len = t->max_len < room ? t->max_len : room;
-  const bool tma = tree_attn_tc_takes(t->block_size, t->k_block, t->k_head, t->k_tok, t->v_block, t->v_head, t->v_tok);
-  const Plan p = make_plan(t->requests, t->kv_heads, t->heads, max_new, max_len + max_new, t->dim, tma);
+  const int mode = g_tensor_mode;
+  const bool tc = mode != 0 && tree_attn_tc_takes(t->block_size, t->k_block, t->k_head, t->k_tok, t->v_block, t->v_head, t->v_tok) &&
+                  (mode == 1 || tensor_pays((int64_t)max_new * (t->heads / t->kv_heads), (int64_t)t->requests * t->kv_heads,
+                                            max_len + max_new, t->dim));
+  const Plan p = make_plan(t->requests, t->kv_heads, t->heads, max_new, max_len + max_new, t->dim, tc);
   QUIC_REQUIRE(t->requests <= 65535 && t->kv_heads * p.tiles <= 65535, QUIC_E_LIMIT,
                "tree_attn: more than 65535 requests, or row tiles of one");
   TreeArgs a = {};

@@ -183,6 +183,7 @@ SIGNATURES = {
     "quic_decode_persist_status": (C.c_int, [_P, _P, C.POINTER(_I32)]),
     "quic_tree_attn": (C.c_int, [_P, _P, _P]),
     "quic_tree_attn_scratch_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I64]),
+    "quic_set_tree_attn_tensor": (None, [C.c_int]),
     "quic_block_tables": (C.c_int, [_P, _P]),
     "quic_tree_commit": (C.c_int, [_P, _P]),
     "quic_qkv_rope_append_at": (C.c_int, [_P, _P, _P, _P, _P, _I32, _P, _P, _P, _I32, _I32, _I32, _P]),

@@ -13,6 +13,14 @@ pytestmark = pytest.mark.gpu
 HALF = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}  # a rounding's relative error at most
 
 
+@pytest.fixture(params=["mma", "tensor"])
+def form(request):
+    """Each of the attention's two forms, whichever the sizes would choose."""
+    K.lib().quic_set_tree_attn_tensor(int(request.param == "tensor"))
+    yield request.param
+    K.lib().quic_set_tree_attn_tensor(-1)
+
+
 def _gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
@@ -133,7 +141,7 @@ LAYOUTS = [(14, 2, 64), (32, 8, 128), (8, 8, 64), (16, 1, 128), (3, 1, 64)]
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("layout", LAYOUTS)
 @pytest.mark.parametrize("tree", [True, False])
-def test_attention_of_ragged_requests(dtype, layout, tree):
+def test_attention_of_ragged_requests(form, dtype, layout, tree):
     heads, kv_heads, dim = layout
     case = Case([0, 1, 63, 64, 65, 500, 1023], [1, 7, 0, 33, 2, 16, 5], 16, heads, kv_heads, dim, dtype, tree, seed=heads)
     case.clear_unused()
@@ -142,7 +150,7 @@ def test_attention_of_ragged_requests(dtype, layout, tree):
 
 @pytest.mark.parametrize("block", [1, 5, 8, 16, 24, 64, 100, 700, 1024])
 @pytest.mark.parametrize("nodes", [1, 3, 40])
-def test_blocks_of_any_size(block, nodes):
+def test_blocks_of_any_size(form, block, nodes):
     case = Case([333, 17, 600], [nodes, 1, nodes], block, seed=block + nodes)
     case.clear_unused()
     case.check(case.call())
@@ -151,13 +159,13 @@ def test_blocks_of_any_size(block, nodes):
 @pytest.mark.parametrize("lengths,new", [([0], [1]), ([1], [1]), ([31], [1]), ([32], [1]), ([4000], [1]), ([4001], [64]), ([0], [64]),
                                          ([20000], [48]), ([9000], [200]), ([0, 0], [130, 1]), ([2000] * 40, [8] * 40)])
 @pytest.mark.parametrize("dtype", TYPES)
-def test_lengths(lengths, new, dtype):
+def test_lengths(form, lengths, new, dtype):
     case = Case(lengths, new, 32, dtype=dtype, seed=len(new))
     case.clear_unused()
     case.check(case.call())
 
 
-def test_a_row_that_sees_nothing_is_zero():
+def test_a_row_that_sees_nothing_is_zero(form):
     case = Case([0, 0, 40], [5, 3, 4], 16, seed=3)
     case.sees[0] = [{0}, set(), {1, 4}, {0, 1, 2, 3, 4}, {7, 40}]  # nodes that are not there, and later ones
     case.sees[2] = [set()] * 4
@@ -172,7 +180,7 @@ def test_a_row_that_sees_nothing_is_zero():
 @pytest.mark.parametrize("layout", LAYOUTS[:2])
 @pytest.mark.parametrize("nodes", [2, 9, 50])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
-def test_what_a_row_does_not_see_does_not_reach_it(layout, nodes, value):
+def test_what_a_row_does_not_see_does_not_reach_it(form, layout, nodes, value):
     """The last node of each tree (which no other sees) holds infinities or NaN in K and V: only its own row shows it."""
     heads, kv_heads, dim = layout
     case = Case([70, 0, 301], [nodes] * 3, 16, heads, kv_heads, dim, seed=nodes)
@@ -198,14 +206,14 @@ def test_what_a_row_does_not_see_does_not_reach_it(layout, nodes, value):
         assert torch.isnan(got[last].float()).all()
 
 
-def test_a_nan_score_reaches_its_rows():
+def test_a_nan_score_reaches_its_rows(form):
     case = Case([3], [2], 16, seed=1)
     case.k[case.place(0, 1)[0], 0, 1] = float("nan")
     got = case.call()
     assert torch.isnan(got[:, :7].float()).all() and torch.isfinite(got[:, 7:].float()).all()
 
 
-def test_scores_of_the_lowest_value():
+def test_scores_of_the_lowest_value(form):
     """Keys that push a score to the type's end in either direction: the softmax stays finite."""
     case = Case([100], [6], 16, seed=2)
     case.q.fill_(255.0)
@@ -217,7 +225,7 @@ def test_scores_of_the_lowest_value():
     case.check(got)
 
 
-def test_rows_outside_the_requests_stay_as_they_were():
+def test_rows_outside_the_requests_stay_as_they_were(form):
     case = Case([30, 50], [4, 3], 16, seed=5, skip_rows=2)
     case.q = torch.cat([case.q, case.q[:5]])
     case.mask = torch.cat([case.mask, case.mask[:5]])
@@ -229,7 +237,7 @@ def test_rows_outside_the_requests_stay_as_they_were():
 
 
 @pytest.mark.parametrize("nodes", [1, 20])
-def test_strides(nodes):
+def test_strides(form, nodes):
     """Heads before rows in q, tokens before heads in the cache, K and V side by side, table rows and mask rows apart."""
     case = Case([200, 90], [nodes, nodes], 16, seed=nodes)
     want = case.call()
@@ -243,7 +251,7 @@ def test_strides(nodes):
     assert torch.equal(case.call(), want)
 
 
-def test_shared_keys():
+def test_shared_keys(form):
     """Two requests over the same blocks, one KV head for all heads (stride 0)."""
     case = Case([130, 130], [3, 3], 16, seed=9)
     case.tables[1] = case.tables[0]
@@ -252,7 +260,7 @@ def test_shared_keys():
 
 
 @pytest.mark.parametrize("nodes", [1, 30])
-def test_bad_blocks_are_seen_by_nobody(nodes):
+def test_bad_blocks_are_seen_by_nobody(form, nodes):
     case = Case([170], [nodes], 16, seed=nodes)
     case.check(case.call())
     whole = case.k.shape[0]
@@ -269,7 +277,7 @@ def test_bad_blocks_are_seen_by_nobody(nodes):
         assert (got[i].double().view(2, 7, 64) - want).abs().max() < 4e-3
 
 
-def test_tables_shorter_than_the_lengths():
+def test_tables_shorter_than_the_lengths(form):
     """Positions that the table has no entry for are seen by nobody; nothing is read there."""
     case = Case([64], [4], 16, seed=4)
     case.tables = case.tables[:, :4].contiguous()
@@ -279,17 +287,17 @@ def test_tables_shorter_than_the_lengths():
 
 
 @pytest.mark.parametrize("bounds", [dict(max_new=None, max_len=None), dict(max_len=0), dict(max_new=100), dict(max_len=10 ** 6)])
-def test_bounds_only_plan(bounds):
+def test_bounds_only_plan(form, bounds):
     case = Case([700, 5], [9, 1], 16, seed=6)
     case.check(case.call(**bounds))
 
 
-def test_scale():
+def test_scale(form):
     case = Case([90], [5], 16, seed=8)
     case.check(case.call(softmax_scale=0.31), 0.31)
 
 
-def test_offsets_beyond_32_bits():
+def test_offsets_beyond_32_bits(form):
     """Blocks that begin beyond element 2^31 of planes of 4.3 GB each."""
     block, blocks = 4096, 4100
     planes = torch.zeros(2, blocks * block * 2 * 64 + 8, dtype=torch.float16, device="cuda")
@@ -302,7 +310,7 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(case.call(), want)
 
 
-def test_another_stream_and_graphs():
+def test_another_stream_and_graphs(form):
     """On a side stream, and in two graphs that are replayed in turn with an eager call between."""
     cases = [Case([3000], [20], 16, seed=1), Case([9000, 10], [1, 4], 32, seed=2)]
     want = [c.call().clone() for c in cases]
@@ -327,11 +335,59 @@ def test_another_stream_and_graphs():
             o.zero_()
 
 
-def test_same_result_every_time():
+def test_same_result_every_time(form):
     case = Case([2500] * 3, [30, 2, 17], 16, seed=12)
     want = case.call()
     for _ in range(5):
         assert torch.equal(case.call(), want)
+
+
+def test_the_rule_between_the_forms():
+    """Calls on both sides of the rule, in either form and by the rule: one result up to the roundings."""
+    for lengths, new, layout in (([1600] * 40, [8] * 40, (14, 2, 64)), ([3000], [48], (14, 2, 64)), ([5000] * 9, [2] * 9, (16, 1, 128))):
+        case = Case(lengths, new, 16, *layout, seed=len(new))
+        got = []
+        for mode in (0, 1, -1):
+            K.lib().quic_set_tree_attn_tensor(mode)
+            got.append(case.call())
+        K.lib().quic_set_tree_attn_tensor(-1)
+        assert torch.equal(got[2], got[0]) or torch.equal(got[2], got[1])
+        case.check(got[0])
+        case.check(got[1])
+
+
+def test_many_requests(form):
+    """More requests than threads look at, empty ones among them, and more rows per request than one tile of any form has."""
+    lengths = [(7 * b) % 90 for b in range(1500)]
+    new = [(b * b) % 4 for b in range(1500)]
+    lengths[700], new[700] = 300, 90
+    case = Case(lengths, new, 8, 8, 8, 64, seed=2)
+    case.check(case.call())
+
+
+@pytest.mark.parametrize("layout", [(14, 2, 64), (32, 8, 128)])
+def test_waits_that_give_up(layout):
+    """The tcgen05 form's bounded waits: K and V that come late change nothing; a tile that never comes sets the error word, and
+    the next call is right."""
+    lib = K.lib()
+    lib.quic_set_tree_attn_tensor(1)
+    try:
+        for nodes in (3, 40):
+            case = Case([2000, 900], [nodes, nodes], 16, *layout, seed=nodes)
+            want = case.call().clone()
+            assert lib.quic_w4a16_tensor_status() == 0
+            for limit, skip, fails in ((1500, -600, False), (1500, 0, True), (1500, 1, True)):
+                lib.quic_w4a16_tensor_test_hook(limit, skip)
+                try:
+                    got = case.call().clone()
+                finally:
+                    lib.quic_w4a16_tensor_test_hook(0, -1)
+                assert (lib.quic_w4a16_tensor_status() != 0) == fails
+                assert fails or torch.equal(got, want)
+                assert torch.equal(case.call(), want)
+                assert lib.quic_w4a16_tensor_status() == 0
+    finally:
+        lib.quic_set_tree_attn_tensor(-1)
 
 
 # ---- block_tables ----------------------------------------------------------------------------

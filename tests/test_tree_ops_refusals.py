@@ -133,9 +133,9 @@ def test_nothing_to_do_is_no_error():
 
 def test_attention_scratch():
     size = K.lib().quic_tree_attn_scratch_bytes
-    assert size(1, 14, 2, 64, 1, 64) == 0
-    assert size(1, 14, 2, 64, 1, 8192) >= 14 * 2 * 66 * 4
-    assert size(1, 15, 2, 64, 1, 8192) == 0
+    assert size(1, 14, 2, 64, 1, 64) >= 2 * 148 * 32 * 66 * 4  # (two parts of 32 rows a CTA of the tcgen05 form)
+    assert size(1, 14, 2, 64, 64, 8192) >= 2 * 148 * 256 * 66 * 4 > size(1, 14, 2, 64, 1, 8192)
+    assert size(1, 15, 2, 64, 1, 8192) == 0 and size(0, 14, 2, 64, 1, 8192) == 0 and size(1, 14, 2, 96, 1, 8192) == 0
 
 
 def test_commit_entry_point_refuses():
