@@ -560,6 +560,77 @@ class QUICForCausalLM:
         rows = [(first + j) % ring for j in range(steps)] if wraps else slice(first, first + steps)
         return plan.host_np[rows][:, slots].T.tolist()
 
+    # ---- drafted tokens ---------------------------------------------------------------------
+    @torch.inference_mode()
+    def verify(self, cache: SlotCache, slots: list[int], drafts: list, parents: list | None = None) -> list[list[int]]:
+        """Several greedy tokens per row in one forward: runs each row's next token and a tree of drafted tokens behind it through
+        the model, keeps the branch that greedy decoding agrees with and drops the others.  What it returns and leaves in the
+        cache is what ``decode`` would have after as many steps: result[i] holds the accepted tokens of drafts[i] and the token
+        after them, at least one.
+
+        ``drafts[i]``: token ids drafted for slots[i], any number (a list or a 1-D tensor on the host); the row's next token is
+        node 0 of the tree, drafts[i][j] node j + 1.  ``parents[i][j]``: the node before which it is drafted to follow, 0 .. j;
+        None: the drafts are a chain.  All rows' nodes must fit behind the cached tokens of their slots.
+
+        The linears run at the sum of the rows' nodes; attention is ``kernels.tree_attn`` over the slots, whose tables
+        ``kernels.block_tables`` builds from the rows' lengths, and ``kernels.tree_commit`` keeps the branch."""
+        cache.check_slots(slots, len(drafts), "verify")
+        if not slots:
+            raise RuntimeError("verify: empty batch")
+        ids = [d.tolist() if isinstance(d, torch.Tensor) else [int(t) for t in d] for d in drafts]
+        if parents is None:
+            trees = [list(range(len(d))) for d in ids]
+        else:
+            trees = [p.tolist() if isinstance(p, torch.Tensor) else [int(x) for x in p] for p in parents]
+            if len(trees) != len(ids) or any(len(t) != len(d) for t, d in zip(trees, ids)):
+                raise ValueError("verify: one parent per drafted token")
+            if any(not 0 <= x <= j for t in trees for j, x in enumerate(t)):
+                raise ValueError("verify: a node's parent is a node before it")
+        if any(not 0 <= t < self.vocab for d in ids for t in d):
+            raise ValueError("verify: a drafted token is outside the vocabulary")
+        counts = [1 + len(d) for d in ids]
+        lens = [cache.host_len[s] for s in slots]
+        if max(counts) > 1024:
+            raise RuntimeError("verify: at most 1023 drafted tokens per row")
+        if any(n < 1 for n in lens):
+            raise RuntimeError("verify: a row has no prompt in its slot")
+        if any(n + c > cache.s_max or n + c > self.max_pos for n, c in zip(lens, counts)):
+            raise RuntimeError("verify: context would exceed the KV slot length")
+        batch, rows, most, longest = len(slots), sum(counts), max(counts), max(lens)
+        table = torch.tensor([t for d in ids for t in [0] + d] + [x for t in trees for x in [-1] + t] + counts + lens + list(slots),
+                             dtype=torch.int32).to(self.device, non_blocking=True)
+        tree, n_new, lengths, slot = table[rows:].split((rows, batch, batch, batch))
+        tokens, at = table[:rows].long(), slot.long()
+        # the slots are blocks of s_max tokens, one to a row, all held
+        pool, held = torch.zeros(4, dtype=torch.int32, device=self.device), torch.ones_like(slot)
+        tables = slot.view(batch, 1).clone()
+        row_start, slot_map, positions, mask = K.block_tables(tables, held, pool, lengths, n_new, cache.s_max, rows, parents=tree,
+                                                              max_new=most)
+        tokens[row_start[:-1].long()] = cache.tok[at].long()
+        h = self.embed[tokens]
+        rms, lin = K.rmsnorm().forward, K.w4a16_linear
+        xn = rms(h, self.layers[0]["ln1"], self.eps)
+        for li, L in enumerate(self.layers):
+            k, v = cache.kv[li, 0], cache.kv[li, 1]
+            q = K.qkv_rope_append_at(lin(L["qkv"], xn), slot_map, positions, self.rope_cos, self.rope_sin, k, v)
+            attn = K.tree_attn(q.transpose(0, 1), k, v, tables, lengths, row_start, mask=mask, max_new=most, max_len=longest)
+            xn, h = rms(lin(L["o"], attn.view(rows, HIDDEN)), L["ln2"], self.eps, residual=h)
+            d = lin(L["down"], K.swiglu_fused(lin(L["gate_up"], xn)))
+            nxt = self.layers[li + 1]["ln1"] if li + 1 < self.n_layers else self.final_norm
+            xn, h = rms(d, nxt, self.eps, residual=h)
+        targets, _ = K.lm_head_argmax(xn, self.embed)
+        path, accepted, following, after = K.tree_commit(cache.kv, tables, lengths, row_start, tree, tokens, targets, most)
+        cache.tok[at] = following.to(torch.int32)
+        cache.pos[at] = after
+        back = torch.cat([accepted, following.to(torch.int32), path.view(-1)]).tolist()
+        out = []
+        for i, s in enumerate(slots):
+            kept = back[i]
+            cache.host_len[s] += kept
+            nodes = back[2 * batch + i * most + 1:2 * batch + i * most + kept]
+            out.append([ids[i][n - 1] for n in nodes] + [back[batch + i]])
+        return out
+
     # ---- prefill -----------------------------------------------------------------
     @torch.inference_mode()
     def prefill(self, cache: SlotCache, slots: list[int], prompts: list[torch.Tensor],
