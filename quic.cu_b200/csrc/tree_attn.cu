@@ -9,9 +9,11 @@
 //
 // This file: the form for few rows (mma.sync), the merge of a request's parts, and the entry point; tree_attn_tc.cu has the form
 // for more rows.
-// A CTA has 16 or 32 rows and a part of the keys, which its four warps walk 32 (16 of 128 dims) at a time, each through a ring of its own
-// (cp.async, no barrier between warps), one pass with a running maximum and sum per row; the warps' results meet in
-// shared memory at the end, those of several CTAs in the merge kernel.  Bound: the bytes of K and V.
+// A CTA has 16 or 32 rows and a part of the keys, which its four warps walk 32 (16 of 128 dims) at a time, each through a ring of
+// its own (cp.async, no barrier between warps), one pass with a running maximum and sum per row; the warps' results meet in
+// shared memory at the end, those of several CTAs in the merge kernel.  Bound: the bytes of K and V (16 x 1 x 8192, fp16, 14:2 heads
+// of 64: 19 us of which the merge takes 4, 3.5 TB/s; 9 x 13 x 7247..14495, 8:8 heads: 44 us, 4.5 TB/s), and launches for small calls
+// (1 x 1 x 300: 5.6 us).
 #include <math.h>
 
 #include "tree_attn.cuh"
@@ -51,15 +53,14 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Keys of a warp's tile (8 KB of K and V) and tiles of its ring: two CTAs an SM with two tiles a warp under way (with tiles of 32
-// keys for 128 dims too, one CTA fitted an SM).
+// Keys of a warp's tile (8 KB of K and V) and tiles of its ring: two CTAs an SM with two tiles a warp under way.  With tiles of 32
+// keys for 128 dims too, one CTA fitted an SM: 48 requests x 2 nodes x 11707 tokens, 16:1 heads, 65 -> 85 us; with rings of two
+// tiles 16 x 1 x 8192, 14:2 heads of 64, 19 -> 21 us, of four (one CTA an SM) 27.  Eight warps a CTA are ahead by 1 us where
+// there are fewer row tiles than SMs, and behind by 3 us where there are more.
 template <int D>
 constexpr int kTileKeys = D == 64 ? 32 : 16;
-#ifndef FEW_STAGES
-#define FEW_STAGES 3
-#endif
-constexpr int kStages = FEW_STAGES;
-constexpr uint32_t kRowsBytes = 32 * 64 * 2;                         // K (or V) of a tile
+constexpr int kStages = 3;
+constexpr uint32_t kRowsBytes = 32 * 64 * 2;  // K (or V) of a tile
 template <int D, int MT>
 constexpr uint32_t kSmem = kWarps * kStages * 2 * kRowsBytes > kWarps * MT * 16 * (D + 4) * 4 ? kWarps * kStages * 2 * kRowsBytes
                                                                                               : kWarps * MT * 16 * (D + 4) * 4;
@@ -466,9 +467,15 @@ Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound
     p.parts = 2 * kTreeTcCtas;
     return p;
   }
+  // Parts by their cost in keys: waves of CTAs, each with 256 keys' worth of beginning and end; the merge of the parts.  (The most
+  // parts of every number of waves are looked at; equal shares of all requests' keys instead, which ragged requests would call
+  // for, cost a CTA two row tiles one after the other: 64 x 8 x 200..1500, 14:2 heads, 25 -> 34 us.)
   const int64_t units = (int64_t)requests * kv_heads * p.tiles, slots = 148 * 2;
+  const int64_t most = bound < 256 ? 1 : (bound < 128 * 256 ? (bound + 255) / 256 : 128);
   int64_t best = 1, least = INT64_MAX;
-  for (int64_t s = 1; s <= 128 && (s == 1 || (s - 1) * 256 < bound); ++s) {
+  for (int64_t waves = 0; waves <= 4; ++waves) {
+    int64_t s = waves == 0 ? 1 : waves * slots / units;
+    s = s < 1 ? 1 : (s > most ? most : s);
     const int64_t part = ((bound + s - 1) / s + 63) / 64 * 64;
     const int64_t cost = (units * s + slots - 1) / slots * (part + 256) + (s > 1 ? 256 + 8 * s : 0);
     if (cost < least) least = cost, best = s;

@@ -8,15 +8,21 @@
 //                  tensor memory, a tile ahead of the softmax;
 //   softmax        a thread owns a row (TMEM lane): P = exp2(..) rounded to the tensors' type, which replaces the scores as
 //                  the A operand of the second product; warps without rows rest;
-//   O += P V       B = the V tile as it lies in the cache (token-major, the transposed form), 64 dims a product.
+//   O += P V       B = the V tile as it lies in the cache (token-major, the transposed form), N = the head dims.
 // The reference point of a row's exponentials moves only when its maximum has grown by more than 2^8 (P and the sums stay far
 // within their types' ranges); O is rescaled in tensor memory then.
 // K and V come by TMA, in boxes of as many tokens as lie together in a block for sure (the largest power of two that divides
 // the block size, 8 to 64); positions without a block are fetched from beyond the planes, as zeros.  (By cp.async, which takes
 // any block size, the loaders had to fence every stage for the tensor cores, and the fence waited for all copies under way:
-// 215 us instead of CHECK at 8 requests x 64 nodes x 16384 tokens, 32:8 heads of 128.)
+// 8 requests x 64 nodes x 12000..16384 tokens, bf16, 32:8 heads of 128, 215 us instead of 193.)
 // Only tiles that reach beyond the cached tokens look at masks.  A V row of a node may hold infinities or NaN that most rows
 // must not see: such values are zeroed in shared memory and added, at the end, to the rows that see them.
+//
+// The CTAs have equal shares of the line of key tiles of all requests (tree_attn.cuh): the same case 193 -> 143 us, with an issuer
+// per stream instead of one for both.  148 us now (3.2 TB/s, 660 TFLOP/s; 172 in a loop of seconds, under the power limit).  Of
+// them K and V alone take 101, with the products 112; tensor pipe 49 %, exponentials 32 %, HBM 46 % busy: the streams' stages wait
+// for one another.  Tried and behind: scores fetched during the last exponentials 153, weights by the old maximum before the new
+// one is known 157, two threads a row 187, two CTAs an SM with a stream each 27 -> 31 us at 4 x 15 x 6146.
 //
 // Roles: warps 0-7 queries, softmax and epilogue, warps 8 and 9 MMA issuers of the two streams, warps 10 and 11
 // TMA of K and V.  Every wait is bounded; a wait that runs out sets word 0 of the tensor path's error words and the CTA leaves with

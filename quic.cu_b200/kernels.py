@@ -808,18 +808,24 @@ def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, table
         _same_device(q, out)
     if rows == 0 or requests == 0:
         return out
-    room = width * block
-    if room < 1 or blocks < 1:
+    most = width * block
+    if most < 1 or blocks < 1:
         raise RuntimeError("tree_attn: no blocks")
     if max_new is None or max_new > rows:
         max_new = rows
-    if max_len is None or max_len > room:
-        max_len = room
+    if max_len is None or max_len > most:
+        max_len = most
     if max_new < 1 or max_len < 0:
         raise RuntimeError("tree_attn: max_new must be positive and max_len not negative")
     need = _tree_scratch_bytes(requests, heads, kv_heads, dim, max_new, max_len)
     stream = _raw_stream(device)
-    scratch = _thread_scratch(("tree", device, stream), need, 1 << 20, 0).data_ptr() if need > 0 else None
+    room = None
+    if need > 0:  # (what a graph uses is its own: replays on any stream meet neither each other nor this thread's calls)
+        if torch.cuda.is_current_stream_capturing():
+            room = torch.empty(need, dtype=torch.uint8, device=q.device)
+        else:
+            room = _thread_scratch(("tree", device, stream), need, 1 << 20, 0)
+    scratch = None if room is None else room.data_ptr()
     call = _TREE_ATTN.pack(q.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), out.data_ptr(), q0, q1, k0, k1, k2, v0, v1, v2,
                            tables.data_ptr(), t0, lengths.data_ptr(), row_start.data_ptr(), mask_ptr, mask_row, words, rows,
                            requests, heads, kv_heads, dim, blocks, block, width, dtype, max_new, max_len, softmax_scale)

@@ -335,6 +335,36 @@ def test_another_stream_and_graphs(form):
             o.zero_()
 
 
+def test_two_graphs_at_once(form):
+    """Captured on a stream that has run the operator before, replayed on two streams at once beside eager calls on the first."""
+    cases = [Case([6000, 9000], [20, 3], 16, seed=s) for s in (1, 2)]
+    want = [c.call().clone() for c in cases]
+    i32 = functools.partial(torch.tensor, dtype=torch.int32, device="cuda")
+    lengths, starts = i32(cases[0].lengths), i32(cases[0].starts)
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(2)], [], []
+
+    def call(c):
+        return K.tree_attn(c.q, c.k, c.v, c.tables, lengths, starts, mask=c.mask, max_new=20, max_len=9000)
+
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[0]):
+        call(cases[0])
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[0]):
+            outs.append(call(c))
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(streams[0]):
+            eager = call(cases[1])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[1])
+
+
 def test_same_result_every_time(form):
     case = Case([2500] * 3, [30, 2, 17], 16, seed=12)
     want = case.call()
