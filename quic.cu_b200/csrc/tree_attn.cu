@@ -435,17 +435,18 @@ int launch_few(const TreeArgs& a, cudaStream_t st) {
 constexpr int64_t kMostTokens = 1 << 29;  // of a request: sums of two counts stay within an int
 // Which form takes a call, by the rows of a request and KV head and by the work of the mma.sync form, in tiles of 32 rows x keys of
 // 64 dims (for all requests, of the longest's keys).  The tcgen05 form has three times its throughput where it has the rows for it,
-// but 8 us more of launch, segments and merge.  us, mma.sync / tcgen05, fp16 or bf16:
-//   heads 14:2, dim 64:  5 requests x 23 nodes x 777 tokens 11.2 / 14.5 (48,000), 1 x 48 x 4096 14.3 / 18.3 (91,000),
-//                        64 x 8 x 1500 25.5 / 26.6 (386,000)
-//   heads 32:8, dim 128: 20 x 28 x 15 19.1 / 24.1 (55,000), 4 x 15 x 6146 54 / 26.5 (790,000), 8 x 64 x 16384 907 / 148
-//   heads 16:1, dim 128: 3 x 46 x 1488 22.4 / 17.1 (210,000)
-// Up to 32 rows it is ahead for long keys of 128 dims alone: 48 x 2 x 11707 (16:1) 65 / 52 (1,100,000); of 64 dims
-// 9 x 13 x 14495 (8:8) 44 / 66, 16 x 1 x 8192 (14:2) 19 / 29.
+// but 8 us more of launch, segments and merge.  requests x nodes x tokens (up to, from half of it), us mma.sync / tcgen05:
+//   heads 14:2, dim 64:  5 x 23 x 777 11.0 / 15.3 (48,000), 1 x 48 x 4096 13.6 / 18.1 (91,000), 2 x 32 x 8192 19.9 / 21.0 (230,000),
+//                        32 x 8 x 2048 24.4 / 20.0 (263,000), 64 x 8 x 1500 26.4 / 28.7 (386,000), 16 x 8 x 8192 36.0 / 26.4 (525,000)
+//   heads 32:8, dim 128: 20 x 28 x 15 19.1 / 24.1 (55,000), 4 x 16 x 1024 20.5 / 17.7 (133,000), 4 x 9 x 4096 41.5 / 24.4 (525,000),
+//                        8 x 64 x 16384 907 / 148
+//   heads 16:1, dim 128: 8 x 4 x 2048 16.4 / 17.0 (66,000), 4 x 8 x 4096 17.2 / 19.4 (131,000), 3 x 46 x 1488 22.4 / 17.1 (210,000)
+// Up to 32 rows it is ahead for long keys of 128 dims alone: 16:1 heads, 32 x 2 x 2048 17.5 / 19.7 (131,000), 32 x 2 x 8192
+// 38.4 / 33.2 (524,000); of 64 dims 9 x 13 x 14495 (8:8) 44 / 66, 16 x 1 x 8192 (14:2) 19 / 29.
 bool tensor_pays(int64_t rows, int64_t units, int64_t bound, int dim) {
   const int64_t work = units * ((rows + 31) / 32) * bound * (dim / 64);
   if (rows > 32) return work > 150000;
-  return rows > 16 && dim == 128 && work > 700000;
+  return rows > 16 && dim == 128 && work > 400000;
 }
 
 struct Plan {
