@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
       for (int i = 0; i < kKeys / kAtOnce; ++i) {
         const uint4 w = *reinterpret_cast<const uint4*>(smem + (v_at - (uint32_t)__cvta_generic_to_shared(smem)) +
                                                         tile_at<D>(i * kAtOnce + lane / kPer, lane % kPer));
-        odd |= tree_not_finite<T>(w.x) || tree_not_finite<T>(w.y) || tree_not_finite<T>(w.z) || tree_not_finite<T>(w.w);
+        odd |= tree_not_finite<T>(w);
       }
       if (__any_sync(0xffffffffu, odd)) {
         unsigned char* v_tile = smem + (v_at - (uint32_t)__cvta_generic_to_shared(smem));

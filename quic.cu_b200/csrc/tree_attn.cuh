@@ -113,7 +113,8 @@ template <>
 __device__ __forceinline__ float2 tree_unpack<__nv_bfloat16>(uint32_t w) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
-// The exponent of an infinity or NaN, and whether one of the two values in a word has it.
+// The exponent of an infinity or NaN, and the sign bits of those of the two values in a word that have it (the sum of exponent and
+// fraction reaches the sign then, and never the next value).
 template <typename T>
 constexpr uint32_t kTreeExponent = 0;
 template <>
@@ -121,17 +122,18 @@ constexpr uint32_t kTreeExponent<half> = 0x7c00u;
 template <>
 constexpr uint32_t kTreeExponent<__nv_bfloat16> = 0x7f80u;
 template <typename T>
-__device__ __forceinline__ bool tree_not_finite(uint32_t w) {
-  constexpr uint32_t e = kTreeExponent<T>;
-  return (w & e) == e || ((w >> 16) & e) == e;
+__device__ __forceinline__ uint32_t tree_not_finite(uint32_t w) {
+  constexpr uint32_t one = 0x8000u - kTreeExponent<T>;
+  return ((w & 0x7fff7fffu) + (one << 16 | one)) & 0x80008000u;
+}
+template <typename T>
+__device__ __forceinline__ bool tree_not_finite(const uint4& w) {
+  return (tree_not_finite<T>(w.x) | tree_not_finite<T>(w.y) | tree_not_finite<T>(w.z) | tree_not_finite<T>(w.w)) != 0u;
 }
 // The word with what is not finite replaced by zero.
 template <typename T>
 __device__ __forceinline__ uint32_t tree_finite(uint32_t w) {
-  constexpr uint32_t e = kTreeExponent<T>;
-  if ((w & e) == e) w &= 0xffff0000u;
-  if (((w >> 16) & e) == e) w &= 0x0000ffffu;
-  return w;
+  return w & ~((tree_not_finite<T>(w) >> 15) * 0xffffu);
 }
 
 // fp16 weights are P = 2^(score - maximum + 8): probabilities down to 2^-22 stay normal.  bf16 has fp32's range.

@@ -370,20 +370,23 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
     const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2);
     int u0 = 0;  // steps of the segments before
     bool ok = true;  // (without it a warp goes on to the end, past all waits, for the barriers of the segments)
+    bool ahead = false;  // the segment's queries are on their way already
+    auto queries = [&](const Segment& q) {
+      if (!q.halves && group != 0) return;
+#pragma unroll 4
+      for (int i = lane; i < 32 * (D / 8); i += 32) {  // (a warp its own rows: in their place it gathers its results)
+        const int row = 32 * quarter + i / (D / 8), chunk = i % (D / 8);
+        const int number = q.r0 + group * kRows + row, mine = min(number, q.rows - 1);
+        const int node = (int)a.group.div(mine), head = q.kvh * (int)a.group.d + mine - node * (int)a.group.d;
+        copy16(base + group * kQ + (chunk >> 3) * kHalfQ + sw128_offset(row, chunk & 7),
+               reinterpret_cast<const T*>(a.q) + (int64_t)(q.r.start + node) * a.q_row + (int64_t)head * a.q_head + 8 * chunk,
+               number < q.rows ? 16u : 0u);
+      }
+    };
     for (int seg = 0; more; s = later, more = more_later, ++seg) {
       const int t_begin = s.begin(), t_end = s.end(), steps = s.steps(group);
       // ---- queries of the stream's rows (the first stream's, where they are the same); rows that are none are zero
-      if (s.halves || group == 0) {
-#pragma unroll 4
-        for (int i = lane; i < 32 * (D / 8); i += 32) {  // (a warp its own rows: in their place it gathers its results)
-          const int row = 32 * quarter + i / (D / 8), chunk = i % (D / 8);
-          const int number = s.r0 + group * kRows + row, mine = min(number, s.rows - 1);
-          const int node = (int)a.group.div(mine), head = s.kvh * (int)a.group.d + mine - node * (int)a.group.d;
-          copy16(base + group * kQ + (chunk >> 3) * kHalfQ + sw128_offset(row, chunk & 7),
-                 reinterpret_cast<const T*>(a.q) + (int64_t)(s.r.start + node) * a.q_row + (int64_t)head * a.q_head + 8 * chunk,
-                 number < s.rows ? 16u : 0u);
-        }
-      }
+      if (!ahead) queries(s);
       // ---- meanwhile: the next segment, and what the row sees of the first tile that reaches beyond the cached tokens
       more_later = walk.next(a, later);
       const bool works = quarter < s.warps(group);
@@ -413,21 +416,22 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
         const bool tree = t + kKeys > s.r.len;
         if (tree) {  // (the same for all the CTA's rows)
           unsigned char* const v_tile = smem + kK + st * kStage + kTile;
-#pragma unroll 2
+          bool stored = s.halves;  // (each stream for itself, changed or not: the other's change may be under way)
+#pragma unroll 4
           for (int c = 32 * quarter + lane; c < (int)kTile / 16; c += 32 * kGroupWarps) {
             uint4 w = reinterpret_cast<const uint4*>(v_tile)[c];
-            bool store = s.halves;  // (each stream for itself, changed or not: the other's change may be under way)
-            if (tree_not_finite<T>(w.x) || tree_not_finite<T>(w.y) || tree_not_finite<T>(w.z) || tree_not_finite<T>(w.w)) {
+            const bool odd = tree_not_finite<T>(w);
+            if (odd) {
               w.x = tree_finite<T>(w.x), w.y = tree_finite<T>(w.y), w.z = tree_finite<T>(w.z), w.w = tree_finite<T>(w.w);
               if (t + (c % (kKeys * 8)) / 8 < t_end) {  // (rows behind the last key may hold anything)
                 atomicMin(&odd_s[seg & 1], i);
                 __threadfence_block();  // known before it is gone
               }
-              store = true;
+              stored = true;
             }
-            if (store) reinterpret_cast<uint4*>(v_tile)[c] = w;
+            if (odd || s.halves) reinterpret_cast<uint4*>(v_tile)[c] = w;
           }
-          fence_proxy_async();
+          if (stored) fence_proxy_async();
           __syncwarp();
         }
         if (!works) {
@@ -525,6 +529,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
         softmax_barrier();
         tc_fence_after();
       }
+      // The next segment's queries, while the results are written, where their place is free: in a segment of two streams of rows the
+      // stream's own, unless its results are gathered there; else the first stream's (the results are gathered in the second's).
+      ahead = more_later && (s.halves ? s.n_tiles != s.key_tiles : group == 0);
+      if (ahead) queries(later);
       if (ok && works) {
         const bool both = s.steps(1) > 0 && !s.halves, alone = s.n_tiles == s.key_tiles;
         const int c_begin = s.halves ? 0 : group * (D / 32), c_end = s.halves ? D / 16 : (group + 1) * (D / 32);
