@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
   __shared__ uint32_t valid_s[kRing];  // which boxes of the stage have a block
   __shared__ int64_t sums_s[kThreads / 32];
   __shared__ Walk walk_s;
+  __shared__ Segment segment_s;
   __shared__ uint32_t tmem_base_s;
   __shared__ int fail_s, odd_s[2];  // odd_s: the first tile of an even, odd segment in which V held what is not finite
 
@@ -244,15 +245,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
     if (before <= start && start < before + mine) {
       int b = b0;
       for (int64_t n; (n = tree_units(a, tree_request(a, b)).all(a)) <= start - before; ++b) before += n;
-      walk_s.b = b;
-      walk_s.at = start - before;
-      walk_s.left = min(share, total - start);
+      Walk first = {b, start - before, min(share, total - start)};
+      first.next(a, segment_s);
+      walk_s = first;
     }
     __syncthreads();
   }
   Walk walk = walk_s;
-  Segment s, later;  // this one and the next, whose numbers are fetched ahead
-  bool more = walk.next(a, s), more_later = false;
+  Segment s = segment_s, later;  // this one and the next, whose numbers are fetched ahead
+  bool more = true, more_later = false;
   int ring = 0;  // tiles of the segments before
   bool issuer = false;
 
@@ -265,7 +266,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
     if (lane == 0) tma_prefetch_desc(map);
     bool ok = true;
     for (; ok && more; s = later, more = more_later) {
-      more_later = walk.next(a, later);
       const int32_t* table = a.tables + (int64_t)s.b * a.table_row;
       const int t_begin = s.begin(), t_end = s.end();
       // the blocks of 32 boxes, n_blocks (beyond the planes) where there is none; those of the next 32 are under way meanwhile
@@ -298,6 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
         const int p = t_begin + i * kKeys + box * args.box;
         if (copies && (ring != args.skip_tile || what))
           tma_load_4d(dst + st * kStage, map, 64 * half, p - (int)a.block.div(p) * (int)a.block.d, s.kvh, id, full);
+        if (i == min(2, s.n_tiles - 1)) more_later = walk.next(a, later);
       }
     }
   } else if (warp >= kSoftmaxWarps) {
@@ -387,19 +388,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
       const int t_begin = s.begin(), t_end = s.end(), steps = s.steps(group);
       // ---- queries of the stream's rows (the first stream's, where they are the same); rows that are none are zero
       if (!ahead) queries(s);
-      // ---- meanwhile: the next segment, and what the row sees of the first tile that reaches beyond the cached tokens
-      more_later = walk.next(a, later);
-      const bool works = quarter < s.warps(group);
-      const int number = s.r0 + (s.halves ? group * kRows : 0) + 32 * quarter + lane, mine = min(number, s.rows - 1);
-      const int node = (int)a.group.div(mine);
-      const int tree_from = max(t_begin, s.r.len & ~(kKeys - 1));
-      const uint32_t first0 = tree_visible32(a, s.r, node, tree_from), first1 = tree_visible32(a, s.r, node, tree_from + 32);
       if (s.halves || group == 0) {
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async();
       }
       __syncwarp();
       if (lane == 0) mbar_arrive_cta(smem_u32(&bar_q));
+      // ---- during the first product: the next segment, and what the row sees of the first tile that reaches beyond the cached tokens
+      more_later = walk.next(a, later);
+      const bool works = quarter < s.warps(group);
+      const int number = s.r0 + (s.halves ? group * kRows : 0) + 32 * quarter + lane, mine = min(number, s.rows - 1);
+      const int node = (int)a.group.div(mine);
+      const int tree_from = max(t_begin, s.r.len & ~(kKeys - 1));
+      const uint32_t first0 = tree_visible32(a, s.r, node, tree_from), first1 = tree_visible32(a, s.r, node, tree_from + 32);
       ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_q), seg & 1, limit));
       if (tid == 0) odd_s[(seg + 1) & 1] = 0x7fffffff;  // (all are through with the segment before, none with this)
 
