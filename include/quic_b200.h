@@ -367,7 +367,6 @@ typedef struct {
   int64_t *slot_map;      /* [max_rows] */
   int32_t *positions;     /* [max_rows] */
   int32_t *mask;          /* [max_rows, mask_words], with parents */
-  void *reserved;         /* NULL */
   int32_t max_blocks, n_blocks, requests, block_size, parent_rows, mask_words, max_rows;
 } quic_block_tables_t;
 

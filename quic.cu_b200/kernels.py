@@ -740,7 +740,7 @@ _TREE_TYPES = {torch.float16: 0, torch.bfloat16: 1}
 # (a struct's bytes cross to C in a third of the time that ctypes takes for as many arguments)
 _TREE_ATTN = struct.Struct("=4Q8qQqQQQq11i4xqf4x")  # quic_tree_attn_t
 _TREE_COMMIT = struct.Struct("=Q5qQq5Q10i4Q")       # quic_tree_commit_t
-_BLOCK_TABLES = struct.Struct("=Qq10Q7i4x")         # quic_block_tables_t
+_BLOCK_TABLES = struct.Struct("=Qq9Q7i4x")          # quic_block_tables_t
 _I32_TYPE = torch.int32
 
 
@@ -761,8 +761,8 @@ def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, table
     whether it sees node j of its request; without it row i sees nodes 0 .. i.  Everybody sees the cached tokens.
 
     ``max_new`` bounds the rows of one request (None: all rows; rows beyond stay unwritten), ``max_len`` the lengths
-    (None: what the tables hold); both only plan the launch, tight bounds make it faster.  Returns [rows, heads, dim]
-    (``out`` if given, contiguous; rows outside row_start[0] .. row_start[-1] - 1 stay as they were): rows that see nothing
+    (None: what the tables hold); both only plan the launch, tight bounds make it faster.  ``softmax_scale`` <= 0: dim ** -0.5.
+    Returns [rows, heads, dim] (``out`` if given, contiguous, or ``q`` itself; rows outside row_start[0] .. row_start[-1] - 1 stay as they were): rows that see nothing
     are zero."""
     kind = q.dtype
     dtype = _TREE_TYPES.get(kind)
@@ -800,6 +800,9 @@ def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, table
             lengths.get_device() != device or row_start.get_device() != device or
             (mask is not None and mask.get_device() != device)):
         _same_device(q, kcache, vcache, tables, lengths, row_start, mask)
+    if torch.cuda.current_device() != device:
+        with torch.cuda.device(device):
+            return tree_attn(q, kcache, vcache, tables, lengths, row_start, mask, softmax_scale, max_new, max_len, out)
     if out is None:
         out = q.new_empty(rows, heads, dim)
     elif out.shape != qs or out.dtype is not kind or not out.is_contiguous():
@@ -829,11 +832,7 @@ def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, table
     call = _TREE_ATTN.pack(q.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), out.data_ptr(), q0, q1, k0, k1, k2, v0, v1, v2,
                            tables.data_ptr(), t0, lengths.data_ptr(), row_start.data_ptr(), mask_ptr, mask_row, words, rows,
                            requests, heads, kv_heads, dim, blocks, block, width, dtype, max_new, max_len, softmax_scale)
-    if torch.cuda.current_device() == device:
-        rc = lib().quic_tree_attn(call, scratch, stream)
-    else:
-        with torch.cuda.device(device):
-            rc = lib().quic_tree_attn(call, scratch, stream)
+    rc = lib().quic_tree_attn(call, scratch, stream)
     if rc != 0:
         check(rc, "tree_attn")
     return out
@@ -904,7 +903,7 @@ def block_tables(tables: torch.Tensor, held: torch.Tensor, pool: torch.Tensor, l
     row_start, positions = held.new_empty(requests + 1), held.new_empty(max_rows)
     call = _BLOCK_TABLES.pack(tables.data_ptr(), tables.stride(0), held.data_ptr(), pool.data_ptr(), lengths.data_ptr(),
                               n_new.data_ptr(), parent_ptr, row_start.data_ptr(), slot_map.data_ptr(), positions.data_ptr(),
-                              mask_ptr, 0, width, pool.shape[0] - 4, requests, block_size, parent_rows, words, max_rows)
+                              mask_ptr, width, pool.shape[0] - 4, requests, block_size, parent_rows, words, max_rows)
     if torch.cuda.current_device() == device:
         rc = lib().quic_block_tables(call, _raw_stream(device))
     else:

@@ -150,7 +150,7 @@ def test_commit_entry_point_refuses():
 
 def test_tables_entry_point_refuses():
     def call(requests=2, block=16, max_rows=4, n_blocks=5, max_blocks=3, parents=0, words=0, tables=4096):
-        values = (tables, 3, 4096, 4096, 4096, 4096, parents, 4096, 4096, 4096, 0, 0, max_blocks, n_blocks, requests, block, 4, words, max_rows)
+        values = (tables, 3, 4096, 4096, 4096, 4096, parents, 4096, 4096, 4096, 0, max_blocks, n_blocks, requests, block, 4, words, max_rows)
         return K.lib().quic_block_tables(K._BLOCK_TABLES.pack(*values), None)
     assert call(tables=0) == -1 and call(parents=4096) == -1 and call(parents=4096, words=1) == -1
     assert call(requests=0) == -2 and call(block=0) == -2 and call(max_blocks=0) == -2 and call(n_blocks=-1) == -2
