@@ -7,13 +7,14 @@
 // chunk of a prompt and a single decode token are trees too.  The R = nodes x (query heads per KV head) rows of a
 // request and KV head share their keys; K and V are read once per tile of those rows.
 //
-// This file: the form for few rows (mma.sync), the merge of a request's parts, and the entry point; tree_attn_tc.cu has the form
+// This file: the form for few rows (mma.sync), the merge of many parts of a request, and the entry point; tree_attn_tc.cu has the form
 // for more rows.
 // A CTA has 16 or 32 rows and a part of the keys, which its four warps walk 32 (16 of 128 dims) at a time, each through a ring of
 // its own (cp.async, no barrier between warps), one pass with a running maximum and sum per row; the warps' results meet in
-// shared memory at the end, those of several CTAs in the merge kernel.  Bound: the bytes of K and V (16 x 1 x 8192, fp16, 14:2 heads
-// of 64: 19 us of which the merge takes 4, 3.5 TB/s; 9 x 13 x 7247..14495, 8:8 heads: 44 us, 4.5 TB/s), and launches for small calls
-// (1 x 1 x 300: 5.6 us).
+// shared memory at the end, those of up to eight CTAs as well, which are a cluster then and each sum a share of the rows' dims (over
+// distributed shared memory), those of more CTAs in the merge kernel.  Bound: the bytes of K and V (16 x 1 x 8192, fp16, 14:2 heads
+// of 64: 18.4 us, 3.7 TB/s; 9 x 13 x 7247..14495, 8:8 heads: 45 us, 4.5 TB/s), and for small calls the launch and what depends on one
+// another: lengths, table, keys, results (1 x 1 x 300: 5.0 us).
 #include <math.h>
 
 #include "tree_attn.cuh"
@@ -21,7 +22,7 @@
 namespace quic {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4, kMostCluster = 8;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {  // zeros beyond `bytes`
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -71,20 +72,50 @@ __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
   return row * (D * 2) + ((chunk ^ (row & 7)) << 4);
 }
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// What CTA `rank` of the cluster has at this CTA's shared-memory address `at`.
+__device__ __forceinline__ uint32_t in_cta(uint32_t at, int rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(rank));
+  return remote;
+}
+__device__ __forceinline__ float2 cluster_ld2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_ld4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+// The result of dims 4 c4 .. of a row of a request and KV head: sum x by 1 / l.
+template <typename T, int D>
+__device__ __forceinline__ void write_out(const TreeArgs& a, const TreeRequest& r, int kvh, int row, int c4, const float4& x, float l) {
+  const int node = (int)a.group.div(row), head = kvh * (int)a.group.d + row - node * (int)a.group.d;
+  const float inv = l != 0.f ? 1.f / l : 0.f;  // (NaN stays)
+  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + ((int64_t)(r.start + node) * a.heads + head) * D + 4 * c4) =
+      make_uint2(tree_pack<T>(x.x * inv, x.y * inv), tree_pack<T>(x.z * inv, x.w * inv));
+}
+
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a) {
   constexpr int kKeys = kTileKeys<D>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint32_t valid_s[kWarps][kStages];
+  __shared__ float2 ml_s[MT * 16];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, kvh = blockIdx.y % a.kv_heads, tile = blockIdx.y / a.kv_heads;
   pdl_wait();
   const TreeRequest r = tree_request(a, blockIdx.z);
   const int all = min(r.n, a.max_new) * (int)a.group.d, r0 = tile * 16 * MT;  // row = node x group + head of the group
-  if (r0 >= all) return;
+  if (r0 >= all) return;  // (a cluster as one)
   int per;
   const int parts = tree_parts(a, r.end, per);
-  if (split >= parts) return;
+  if (split >= parts && !a.cluster) return;
   const int t_begin = split * per, t_end = min(t_begin + per, r.end);
   const int32_t* table = a.tables + (int64_t)blockIdx.z * a.table_row;
 
@@ -338,15 +369,45 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
       }
     }
     if (parts == 1) {
-      const int nd = (int)a.group.div(r0 + row), head = kvh * (int)a.group.d + (r0 + row) - nd * (int)a.group.d;
-      const float inv = l != 0.f ? 1.f / l : 0.f;  // (NaN stays)
-      *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + ((int64_t)(r.start + nd) * a.heads + head) * D + 4 * c4) =
-          make_uint2(tree_pack<T>(x.x * inv, x.y * inv), tree_pack<T>(x.z * inv, x.w * inv));
+      if (split == 0) write_out<T, D>(a, r, kvh, r0 + row, c4, x, l);
+    } else if (a.cluster) {  // (in the place of the first warp's part, which nobody else reads)
+      *reinterpret_cast<float4*>(smem + ((row * kLine) + 4 * c4) * 4) = x;
+      if (c4 == 0) ml_s[row] = make_float2(top, l);
     } else {
       a.part_o[(part * (D / 4) + c4) * a.tile_rows + row] = x;
       if (c4 == 0) a.part_ml[part * a.tile_rows + row] = make_float2(top, l);
     }
   }
+  if (!a.cluster || parts == 1) return;
+
+  // ---- the cluster's parts: every CTA sums its share of the rows' dims
+  __syncwarp();
+  cluster_sync();
+  const int share = (kRows * (D / 4) + a.splits - 1) / a.splits, last = min((split + 1) * share, kRows * (D / 4));
+  for (int i = split * share + tid; i < last; i += kWarps * 32) {
+    const int row = i / (D / 4), c4 = i % (D / 4);
+    if (r0 + row >= all) break;
+    const uint32_t ml_at = (uint32_t)__cvta_generic_to_shared(&ml_s[row]), at = (uint32_t)__cvta_generic_to_shared(smem) + (row * kLine + 4 * c4) * 4;
+    float2 ml[kMostCluster];
+    float4 y[kMostCluster], x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int s = 0; s < kMostCluster; ++s)
+      if (s < parts) ml[s] = cluster_ld2(in_cta(ml_at, s)), y[s] = cluster_ld4(in_cta(at, s));
+#pragma unroll
+    for (int s = 0; s < kMostCluster; ++s)
+      if (s < parts) top = fmaxf(top, ml[s].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int s = 0; s < kMostCluster; ++s)
+      if (s < parts) {
+        const float f = tree_ex2(ml[s].x - ref);
+        if (f != 0.f) l += f * ml[s].y, x.x += f * y[s].x, x.y += f * y[s].y, x.z += f * y[s].z, x.w += f * y[s].w;
+      }
+    write_out<T, D>(a, r, kvh, r0 + row, c4, x, l);
+  }
+  __syncwarp();
+  cluster_sync();  // (nobody leaves while its shared memory is read)
 }
 
 // Rows whose keys several CTAs shared: sum of the parts, each by 2^(its maximum - the largest).  A CTA has 32 rows of a tile
@@ -418,39 +479,56 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a) {
     const float f = tree_ex2(x.x - ref);
     if (f != 0.f) sum += f * x.y, v.x += f * y.x, v.y += f * y.y, v.z += f * y.z, v.w += f * y.w;
   }
-  const float inv = sum != 0.f ? 1.f / sum : 0.f;
-  const int node = (int)a.group.div(number), head = kvh * (int)a.group.d + number - node * (int)a.group.d;
-  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + ((int64_t)(r.start + node) * a.heads + head) * D + 16 * quarter + 4 * warp) =
-      make_uint2(tree_pack<T>(v.x * inv, v.y * inv), tree_pack<T>(v.z * inv, v.w * inv));
+  write_out<T, D>(a, r, kvh, number, 4 * quarter + warp, v, sum);
 }
 
 template <typename T, int D, int MT>
 int launch_few(const TreeArgs& a, cudaStream_t st) {
   QUIC_CUDA((allow_smem<tree_attn_kernel<T, D, MT>>(kSmem<D, MT>)));
-  QUIC_CUDA(launch(tree_attn_kernel<T, D, MT>, dim3(a.splits, a.kv_heads * a.tiles, a.requests), dim3(kWarps * 32), kSmem<D, MT>, st,
-                   true, a));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.splits, a.kv_heads * a.tiles, a.requests);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = kSmem<D, MT>;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  if (a.cluster) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  if (pdl_enabled()) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  cfg.attrs = attr;
+  QUIC_CUDA(cudaLaunchKernelEx(&cfg, tree_attn_kernel<T, D, MT>, a));
   return QUIC_OK;
 }
 
 constexpr int64_t kMostTokens = 1 << 29;  // of a request: sums of two counts stay within an int
 // Which form takes a call, by the rows of a request and KV head and by the work of the mma.sync form, in tiles of 32 rows x keys of
 // 64 dims (for all requests, of the longest's keys).  The tcgen05 form has three times its throughput where it has the rows for it,
-// but 8 us more of launch, segments and merge.  requests x nodes x tokens (up to, from half of it), us mma.sync / tcgen05:
-//   heads 14:2, dim 64:  5 x 23 x 777 11.0 / 15.3 (48,000), 1 x 48 x 4096 13.6 / 18.1 (91,000), 2 x 32 x 8192 19.9 / 21.0 (230,000),
-//                        32 x 8 x 2048 24.4 / 20.0 (263,000), 64 x 8 x 1500 26.4 / 28.7 (386,000), 16 x 8 x 8192 36.0 / 26.4 (525,000)
-//   heads 32:8, dim 128: 20 x 28 x 15 19.1 / 24.1 (55,000), 4 x 16 x 1024 20.5 / 17.7 (133,000), 4 x 9 x 4096 41.5 / 24.4 (525,000),
-//                        8 x 64 x 16384 907 / 148
-//   heads 16:1, dim 128: 8 x 4 x 2048 16.4 / 17.0 (66,000), 4 x 8 x 4096 17.2 / 19.4 (131,000), 3 x 46 x 1488 22.4 / 17.1 (210,000)
-// Up to 32 rows it is ahead for long keys of 128 dims alone: 16:1 heads, 32 x 2 x 2048 17.5 / 19.7 (131,000), 32 x 2 x 8192
-// 38.4 / 33.2 (524,000); of 64 dims 9 x 13 x 14495 (8:8) 44 / 66, 16 x 1 x 8192 (14:2) 19 / 29.
+// but 8 us more of launch and merge, and 3 us for every row tile of a CTA.  requests x nodes x tokens, us mma.sync / tcgen05:
+//   heads 14:2, dim 64:  5 x 23 x 388..777 9.8 / 14.3 (work 48,000), 1 x 48 x 4096 14.3 / 18.1 (91,000), 2 x 32 x 8192 20.1 / 20.2
+//                        (230,000), 64 x 5 x 500..1000 18.9 / 24.0 (257,000), 16 x 16 x 1024..2048 21.0 / 16.9 (264,000),
+//                        64 x 8 x 750..1500 26.1 / 27.5 (386,000), 16 x 8 x 4096..8192 34.4 / 25.5 (525,000)
+//   heads 32:8, dim 128: 20 x 28 x 7..15 18.6 / 22.9 (55,000), 4 x 41 x 182..365 19.3 / 22.1 (156,000), 8 x 9 x 512..1024 24.8 / 21.3
+//                        (264,000), 4 x 9 x 2048..4096 38.6 / 23.8 (525,000), 8 x 64 x 16384 907 / 148
+//   heads 16:1, dim 128: 22 x 58 x 30..150 25.4 / 33.6 (265,000), 60 x 4 x 220..1108 25.6 / 21.0 (267,000), 4 x 8 x 4096 18 / 19 (131,000)
+// Up to 32 rows it is ahead for long keys of 128 dims alone: 16:1 heads, 32 x 2 x 2048 18.5 / 19.2 (131,000), 12 x 2 x 2271..11357
+// 25.5 / 21.9 (273,000); of 64 dims 9 x 13 x 14495 (8:8) 45 / 59, 64 x 3 x 4000 (14:2) 34 / 39.  Of 89 calls drawn over these ranges
+// the rule's form is 0.5 % behind the faster one on average, 12 % at worst (3 x 9 x 2877, 16:1 heads: 19.3 / 17.0).
 bool tensor_pays(int64_t rows, int64_t units, int64_t bound, int dim) {
   const int64_t work = units * ((rows + 31) / 32) * bound * (dim / 64);
-  if (rows > 32) return work > 150000;
-  return rows > 16 && dim == 128 && work > 400000;
+  if (rows > 32) return work > (dim == 64 ? 200000 : 160000) + 1500 * units * ((rows + kTreeTcRows - 1) / kTreeTcRows);
+  return rows > 16 && dim == 128 && work > 250000;
 }
 
+// CTAs of the mma.sync form that run at once, by the size of their clusters (148 SMs of two, as the GPU's groups of SMs allow)
+constexpr int kSlots[kMostCluster] = {296, 296, 279, 284, 280, 270, 259, 264};
 struct Plan {
-  bool tc;
+  bool tc, cluster;
   int64_t tiles;                   // row tiles of a request and KV head
   int tile_rows, splits, chunk;    // rows of one (a multiple of 32); mma.sync form: CTAs that share its keys, the keys of one
   int64_t parts;                   // partial results
@@ -468,24 +546,34 @@ Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound
     p.parts = 2 * kTreeTcCtas;
     return p;
   }
-  // Parts by their cost in keys: waves of CTAs, each with 256 keys' worth of beginning and end; the merge of the parts.  (The most
-  // parts of every number of waves are looked at; equal shares of all requests' keys instead, which ragged requests would call
-  // for, cost a CTA two row tiles one after the other: 64 x 8 x 200..1500, 14:2 heads, 25 -> 34 us.)
-  const int64_t units = (int64_t)requests * kv_heads * p.tiles, slots = 148 * 2;
+  // Parts by their cost in keys: waves of CTAs, each with 256 keys' worth of beginning and end; then the merge, by the cluster (64)
+  // or by a kernel of its own (192 and 4 a part).  us with the most parts that fit, cluster / kernel / one part, 14:2 heads of 64:
+  // 1 x 1 x 300 5.1 / 6.1 / 5.6, 1 x 1 x 4000 8.4 / 8.1 (17 parts) / 31.8, 32 x 1 x 500..1000 7.3 / 8.9 / 10.7, 16 x 1 x 8192 18.4 /
+  // 19.7 / 69, 5 x 23 x 0..777 9.5 / 10.1 / 13.5, 1 x 48 x 4096 15.3 / 14.3 (12 parts) / 45.6, 64 x 8 x 200..1500 30.8 / 28.4 / 25.6;
+  // 32:8 heads of 128: 8 x 3 x 2000..4000 27.3 / 31.9 / 67.  The most parts of every number of waves are looked at.  (Equal shares of
+  // all requests' keys instead, which ragged requests would call for, cost a CTA two row tiles one after the other: 64 x 8 x
+  // 200..1500 34.)
+  const int64_t units = (int64_t)requests * kv_heads * p.tiles, slots = kSlots[0];
   const int64_t most = bound < 256 ? 1 : (bound < 128 * 256 ? (bound + 255) / 256 : 128);
   int64_t best = 1, least = INT64_MAX;
   for (int64_t waves = 0; waves <= 4; ++waves) {
     int64_t s = waves == 0 ? 1 : waves * slots / units;
     s = s < 1 ? 1 : (s > most ? most : s);
     const int64_t part = ((bound + s - 1) / s + 63) / 64 * 64;
-    const int64_t cost = (units * s + slots - 1) / slots * (part + 256) + (s > 1 ? 256 + 8 * s : 0);
+    const int64_t cost = (units * s + slots - 1) / slots * (part + 256) + (s > 1 ? 192 + 4 * s : 0);
     if (cost < least) least = cost, best = s;
+  }
+  for (int64_t s = 2; s <= kMostCluster && 64 * (s - 1) < bound; ++s) {
+    const int64_t part = ((bound + s - 1) / s + 63) / 64 * 64;
+    const int64_t cost = (units * s + kSlots[s - 1] - 1) / kSlots[s - 1] * (part + 256) + 64;
+    if (cost < least) least = cost, best = s, p.cluster = true;
   }
   p.chunk = (int)(((bound + best - 1) / best + 63) / 64 * 64);
   if (p.chunk < 64) p.chunk = 64;
   p.splits = (int)((bound + p.chunk - 1) / p.chunk);
   if (p.splits < 1) p.splits = 1;
-  p.parts = p.splits > 1 ? units * p.splits : 0;
+  if (p.cluster) p.chunk = 64;  // (shorter requests: all CTAs of the cluster are there)
+  p.parts = p.splits > 1 && !p.cluster ? units * p.splits : 0;
   return p;
 }
 int64_t first_bytes(const Plan& p, int requests) { return p.tc ? ((int64_t)requests + 2 + 1) / 2 * 16 : 0; }
@@ -548,7 +636,7 @@ extern "C" int quic_tree_attn(const quic_tree_attn_t* t, void* scratch, void* st
   QUIC_REQUIRE(t->requests <= 65535 && t->kv_heads * p.tiles <= 65535, QUIC_E_LIMIT,
                "tree_attn: more than 65535 requests, or row tiles of one");
   TreeArgs a = {};
-  a.splits = p.splits, a.chunk = p.chunk, a.tiles = (int)p.tiles, a.tile_rows = p.tile_rows;
+  a.splits = p.splits, a.chunk = p.chunk, a.cluster = p.cluster, a.tiles = (int)p.tiles, a.tile_rows = p.tile_rows;
   QUIC_REQUIRE(p.parts == 0 || (scratch != nullptr && (uintptr_t)scratch % 16 == 0), QUIC_E_ARG,
                "tree_attn: scratch missing or not 16-byte aligned");
   a.q = t->q, a.k = t->k, a.v = t->v, a.out = t->out;

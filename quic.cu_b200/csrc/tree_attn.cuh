@@ -20,7 +20,8 @@ struct TreeArgs {
   FastDiv block, group;              // tokens per block, query heads per KV head
   int32_t rows, requests, heads, kv_heads, n_blocks, max_blocks, mask_words, max_new;
   int32_t tiles, tile_rows;          // row tiles of a request and KV head at most, rows of one
-  int32_t splits, chunk;             // mma.sync form: CTAs per request, KV head and row tile at most; the tokens of one
+  int32_t splits, chunk;             // mma.sync form: CTAs per request, KV head and row tile at most; the tokens of one at least
+  int32_t cluster;                   // ... which are a cluster and merge their results themselves
   float scale_log2;
 };
 

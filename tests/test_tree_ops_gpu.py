@@ -297,6 +297,24 @@ def test_scale(form):
     case.check(case.call(softmax_scale=0.31), 0.31)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("longest,nodes", [(70, 1), (200, 3), (460, 1), (511, 2), (2040, 1), (2100, 4)])
+def test_requests_of_any_length_beside_a_long_one(form, dim, longest, nodes):
+    """Parts of a request by those of the longest: none, one, fewer, all."""
+    lengths = [longest, 0, 1, 62, 63, 64, longest // 2, longest - 1]
+    case = Case(lengths, [nodes, 1, 0, 1, nodes, 1, nodes, 2], 16, 4, 2, dim, seed=longest)
+    case.check(case.call())
+
+
+@pytest.mark.parametrize("lengths,new", [([40], [3]), ([900, 20], [4, 9]), ([3000] * 3, [40] * 3)])
+def test_results_in_the_place_of_the_queries(form, lengths, new):
+    case = Case(lengths, new, 16, seed=4)
+    want, q = case.call(), case.q.clone()
+    assert case.call(out=case.q) is case.q and torch.equal(case.q, want)
+    case.q = q
+    case.check(want)
+
+
 def test_offsets_beyond_32_bits(form):
     """Blocks that begin beyond element 2^31 of planes of 4.3 GB each."""
     block, blocks = 4096, 4100
