@@ -13,8 +13,11 @@
 // its own (cp.async, no barrier between warps), one pass with a running maximum and sum per row; the warps' results meet in
 // shared memory at the end, those of up to eight CTAs as well, which are a cluster then and each sum a share of the rows' dims (over
 // distributed shared memory), those of more CTAs in the merge kernel.  Bound: the bytes of K and V (16 x 1 x 8192, fp16, 14:2 heads
-// of 64: 18.4 us, 3.7 TB/s; 9 x 13 x 7247..14495, 8:8 heads: 45 us, 4.5 TB/s), and for small calls the launch and what depends on one
-// another: lengths, table, keys, results (1 x 1 x 300: 5.0 us).
+// of 64: 17.6 us, 3.8 TB/s; 9 x 13 x 7247..14495, 8:8 heads: 42.5 us, 4.7 TB/s); with 32 rows what a warp's steps wait for of their own
+// results, two warps a scheduler (64 x 8 x 200..1500: 22.2 us, tensor pipe a fifth busy); for small calls the launch and what depends
+// on one another: lengths, table, keys, results (1 x 1 x 300: 5.0 us).  Moving the reference point for every larger maximum, sums of
+// the rounded weights and separate exponents cost 64 x 8 x 200..1500 25.5, 16 x 1 x 8192 18.4 us; places of keys computed once a key
+// instead of once a row, and the masks of the rows kept in shared memory, cost more than they saved (+0.2 to +1 us).
 #include <math.h>
 
 #include "tree_attn.cuh"
@@ -22,7 +25,7 @@
 namespace quic {
 namespace {
 
-constexpr int kWarps = 4, kMostCluster = 8;
+constexpr int kWarps = 4, kMostCluster = 8, kByRowsTile = 32 * kWarps;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {  // zeros beyond `bytes`
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -39,19 +42,18 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
                : "r"(at)
                : "memory");
 }
-template <typename T>
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma<half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d += a b (kFirst: d = a b)
+template <typename T, bool kFirst = false>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (kFirst) d[0] = d[1] = d[2] = d[3] = 0.f;
+  if constexpr (kTreeExponent<T> == kTreeExponent<half>)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // Keys of a warp's tile (8 KB of K and V) and tiles of its ring: two CTAs an SM with two tiles a warp under way.  With tiles of 32
@@ -101,7 +103,8 @@ __device__ __forceinline__ void write_out(const TreeArgs& a, const TreeRequest& 
       make_uint2(tree_pack<T>(x.x * inv, x.y * inv), tree_pack<T>(x.z * inv, x.w * inv));
 }
 
-template <typename T, int D, int MT>
+// kByRows: a warp has rows of its own and all keys, else the rows of the CTA and every fourth tile of the keys.
+template <typename T, int D, int MT, bool kByRows>
 __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a) {
   constexpr int kKeys = kTileKeys<D>;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -111,12 +114,13 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
   const int split = blockIdx.x, kvh = blockIdx.y % a.kv_heads, tile = blockIdx.y / a.kv_heads;
   pdl_wait();
   const TreeRequest r = tree_request(a, blockIdx.z);
-  const int all = min(r.n, a.max_new) * (int)a.group.d, r0 = tile * 16 * MT;  // row = node x group + head of the group
-  if (r0 >= all) return;  // (a cluster as one)
+  const int all = min(r.n, a.max_new) * (int)a.group.d;  // row = node x group + head of the group
+  if (tile * 16 * MT * (kByRows ? kWarps : 1) >= all) return;  // (a cluster as one)
+  const int r0 = (kByRows ? tile * kWarps + warp : tile) * 16 * MT;
   int per;
   const int parts = tree_parts(a, r.end, per);
   if (split >= parts && !a.cluster) return;
-  const int t_begin = split * per, t_end = min(t_begin + per, r.end);
+  const int t_begin = split * per, t_end = kByRows && r0 >= all ? 0 : min(t_begin + per, r.end);
   const int32_t* table = a.tables + (int64_t)blockIdx.z * a.table_row;
 
   // ---- queries: A fragments of every 16 rows
@@ -142,7 +146,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
   // ---- the warp's ring
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * kStages * 2 * kRowsBytes;
   constexpr int kPer = D / 8, kAtOnce = 32 / kPer;  // chunks of a row, rows of one instruction
-  const int step = kWarps * kKeys;
+  constexpr int step = (kByRows ? 1 : kWarps) * kKeys;
   constexpr uint32_t kAllKeys = 0xffffffffu >> (32 - kKeys);
   // the block of position t + lane, or -1 where there is none
   auto fetch = [&](int t) {
@@ -170,16 +174,18 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
     }
   };
 
-  float o[MT][D / 8][4], m_run[MT][2], l_run[MT][2];
+  float o[MT][D / 8][4], m_run[MT][2];  // m_run: the reference point
+  uint64_t l_run[MT][2];                // two sums each
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
     m_run[m][0] = m_run[m][1] = -INFINITY;
-    l_run[m][0] = l_run[m][1] = 0.f;
+    l_run[m][0] = l_run[m][1] = 0ull;
   }
 
-  const int t_warp = t_begin + warp * kKeys;
+  const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2);
+  const int t_warp = t_begin + (kByRows ? 0 : warp * kKeys);
   int id = fetch(t_warp);
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
@@ -204,10 +210,6 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
     // S = Q K^T
     float s[MT][kKeys / 8][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int n = 0; n < kKeys / 8; ++n) s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.f;
-#pragma unroll
     for (int kk = 0; kk < D / 32; ++kk)
 #pragma unroll
       for (int n = 0; n < kKeys / 8; ++n) {
@@ -215,7 +217,8 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
         ldsm4(b, k_at + tile_at<D>(n * 8 + (lane & 7), kk * 4 + (lane >> 3)));
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          mma<T>(s[m][n], qf[m][2 * kk], b[0], b[1]);
+          if (kk == 0) mma<T, true>(s[m][n], qf[m][2 * kk], b[0], b[1]);
+          else mma<T>(s[m][n], qf[m][2 * kk], b[0], b[1]);
           mma<T>(s[m][n], qf[m][2 * kk + 1], b[2], b[3]);
         }
       }
@@ -237,37 +240,58 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
         }
     }
 
-    // running maximum and sum
+    // reference points: moved when a score is far above (from -inf: by any)
+    bool grown = false;
+    float top[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float mx = fmaxf(s[m][0][2 * h], s[m][0][2 * h + 1]);
+#pragma unroll
+        for (int n = 1; n < kKeys / 8; ++n) mx = max3(mx, s[m][n][2 * h], s[m][n][2 * h + 1]);
+        top[m][h] = mx * a.scale_log2;  // (the scale is positive)
+        grown |= top[m][h] > m_run[m][h] + kTreeGrowth;
+      }
+    if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = top[m][h];  // of the row: four lanes have eight keys each
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          if (mx > m_run[m][h] + kTreeGrowth) {
+            const float alpha = tree_ex2(m_run[m][h] - mx);
+            m_run[m][h] = mx;
+            float x, y;
+            unpair2(l_run[m][h], x, y);
+            l_run[m][h] = pair2(x * alpha, y * alpha);
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) {
+              o[m][n][2 * h] *= alpha;
+              o[m][n][2 * h + 1] *= alpha;
+            }
+          }
+        }
+    }
+
+    // weights and their sums
     uint32_t p[MT][kKeys / 16][4];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < kKeys / 8; ++n) mx = fmaxf(mx, fmaxf(s[m][n][2 * h], s[m][n][2 * h + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m_run[m][h], mx * a.scale_log2);  // (the scale is positive)
-        const float ref = m_new == -INFINITY ? 0.f : m_new, shifted = kTreeShift<T> - ref;
-        const float alpha = tree_ex2(m_run[m][h] - ref);
-        m_run[m][h] = m_new;
-        float sum = 0.f;
+        const float shifted = kTreeShift<T> - (m_run[m][h] == -INFINITY ? 0.f : m_run[m][h]);
+        const uint64_t shifted2 = pair2(shifted, shifted);
 #pragma unroll
         for (int n = 0; n < kKeys / 8; ++n) {
-          const uint32_t w = tree_pack<T>(tree_ex2(fmaf(s[m][n][2 * h], a.scale_log2, shifted)),
-                                          tree_ex2(fmaf(s[m][n][2 * h + 1], a.scale_log2, shifted)));
-          p[m][n >> 1][2 * (n & 1) + h] = w;
-          const float2 f = tree_unpack<T>(w);  // what the product will see: the weights sum to one
-          sum += f.x + f.y;
-        }
-        l_run[m][h] = l_run[m][h] * alpha + sum;
-        if (alpha != 1.f) {
-#pragma unroll
-          for (int n = 0; n < D / 8; ++n) {
-            o[m][n][2 * h] *= alpha;
-            o[m][n][2 * h + 1] *= alpha;
-          }
+          float x, y;
+          unpair2(fma2(pair2(s[m][n][2 * h], s[m][n][2 * h + 1]), scale2, shifted2), x, y);
+          x = tree_ex2(x);  // 2^-inf = 0 for keys that are not seen
+          y = tree_ex2(y);
+          p[m][n >> 1][2 * (n & 1) + h] = tree_pack<T>(x, y);
+          l_run[m][h] = add2(l_run[m][h], pair2(x, y));
         }
       }
 
@@ -330,7 +354,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   pdl_launch_dependents();
 
-  // ---- the four warps' parts
+  // ---- the four warps' parts, or rows
   constexpr int kRows = MT * 16, kLine = D + 4;  // a row: D values, maximum, sum
   float* const mine = reinterpret_cast<float*>(smem) + warp * kRows * kLine;
   __syncthreads();
@@ -341,11 +365,23 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
       float* line = mine + (16 * m + 8 * h + g) * kLine;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(line + 8 * n + 2 * c) = make_float2(o[m][n][2 * h], o[m][n][2 * h + 1]);
-      float l = l_run[m][h];
+      float l, l1;
+      unpair2(l_run[m][h], l, l1);
+      l += l1;
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
       if (c == 0) line[D] = l != l ? INFINITY : m_run[m][h], line[D + 1] = l;  // (a maximum passes over NaN)
     }
+  if constexpr (kByRows) {
+    __syncwarp();
+#pragma unroll 4
+    for (int i = lane; i < kRows * (D / 4); i += 32) {
+      const int row = i / (D / 4), c4 = i % (D / 4);
+      if (r0 + row >= all) break;
+      write_out<T, D>(a, r, kvh, r0 + row, c4, *reinterpret_cast<const float4*>(mine + row * kLine + 4 * c4), mine[row * kLine + D + 1]);
+    }
+    return;
+  }
   __syncthreads();
   const int64_t part = tree_part(a, blockIdx.z, kvh, tile) + split;
   for (int i = tid; i < kRows * (D / 4); i += kWarps * 32) {
@@ -482,9 +518,9 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a) {
   write_out<T, D>(a, r, kvh, number, 4 * quarter + warp, v, sum);
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D, int MT, bool kByRows>
 int launch_few(const TreeArgs& a, cudaStream_t st) {
-  QUIC_CUDA((allow_smem<tree_attn_kernel<T, D, MT>>(kSmem<D, MT>)));
+  QUIC_CUDA((allow_smem<tree_attn_kernel<T, D, MT, kByRows>>(kSmem<D, MT>)));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.splits, a.kv_heads * a.tiles, a.requests);
   cfg.blockDim = dim3(kWarps * 32);
@@ -502,7 +538,7 @@ int launch_few(const TreeArgs& a, cudaStream_t st) {
     attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
   cfg.attrs = attr;
-  QUIC_CUDA(cudaLaunchKernelEx(&cfg, tree_attn_kernel<T, D, MT>, a));
+  QUIC_CUDA(cudaLaunchKernelEx(&cfg, tree_attn_kernel<T, D, MT, kByRows>, a));
   return QUIC_OK;
 }
 
@@ -510,18 +546,19 @@ constexpr int64_t kMostTokens = 1 << 29;  // of a request: sums of two counts st
 // Which form takes a call, by the rows of a request and KV head and by the work of the mma.sync form, in tiles of 32 rows x keys of
 // 64 dims (for all requests, of the longest's keys).  The tcgen05 form has three times its throughput where it has the rows for it,
 // but 8 us more of launch and merge, and 3 us for every row tile of a CTA.  requests x nodes x tokens, us mma.sync / tcgen05:
-//   heads 14:2, dim 64:  5 x 23 x 388..777 9.8 / 14.3 (work 48,000), 1 x 48 x 4096 14.3 / 18.1 (91,000), 2 x 32 x 8192 20.1 / 20.2
-//                        (230,000), 64 x 5 x 500..1000 18.9 / 24.0 (257,000), 16 x 16 x 1024..2048 21.0 / 16.9 (264,000),
-//                        64 x 8 x 750..1500 26.1 / 27.5 (386,000), 16 x 8 x 4096..8192 34.4 / 25.5 (525,000)
-//   heads 32:8, dim 128: 20 x 28 x 7..15 18.6 / 22.9 (55,000), 4 x 41 x 182..365 19.3 / 22.1 (156,000), 8 x 9 x 512..1024 24.8 / 21.3
-//                        (264,000), 4 x 9 x 2048..4096 38.6 / 23.8 (525,000), 8 x 64 x 16384 907 / 148
-//   heads 16:1, dim 128: 22 x 58 x 30..150 25.4 / 33.6 (265,000), 60 x 4 x 220..1108 25.6 / 21.0 (267,000), 4 x 8 x 4096 18 / 19 (131,000)
-// Up to 32 rows it is ahead for long keys of 128 dims alone: 16:1 heads, 32 x 2 x 2048 18.5 / 19.2 (131,000), 12 x 2 x 2271..11357
-// 25.5 / 21.9 (273,000); of 64 dims 9 x 13 x 14495 (8:8) 45 / 59, 64 x 3 x 4000 (14:2) 34 / 39.  Of 89 calls drawn over these ranges
-// the rule's form is 0.5 % behind the faster one on average, 12 % at worst (3 x 9 x 2877, 16:1 heads: 19.3 / 17.0).
+//   heads 14:2, dim 64:  5 x 23 x 388..777 9.5 / 14.3 (work 48,000), 1 x 48 x 4096 13.6 / 18.1 (91,000), 2 x 32 x 8192 18.5 / 20.2
+//                        (230,000), 64 x 5 x 500..1000 17.0 / 23.9 (257,000), 16 x 16 x 1024..2048 18.8 / 16.8 (264,000),
+//                        64 x 8 x 750..1500 23.0 / 27.5 (386,000), 16 x 8 x 4096..8192 30.2 / 25.6 (525,000)
+//   heads 32:8, dim 128: 20 x 28 x 7..15 15.3 / 22.9 (55,000), 4 x 41 x 182..365 18.2 / 22.1 (156,000), 8 x 9 x 512..1024 22.7 / 21.3
+//                        (264,000), 4 x 9 x 2048..4096 34.8 / 23.7 (525,000), 8 x 64 x 16384 907 / 150
+//   heads 16:1, dim 128: 22 x 58 x 30..150 24.2 / 33.6 (265,000), 60 x 4 x 220..1108 23.7 / 20.8 (267,000), 3 x 46 x 1488 19.0 / 21.5
+//                        (212,000)
+// Up to 32 rows it is ahead for long keys of 128 dims alone: 16:1 heads, 32 x 2 x 1024..2048 17.3 / 19.1 (131,000), x 4096..8192 35.1 /
+// 32.3 (524,000); of 64 dims 9 x 13 x 7247..14495 (8:8) 44 / 59, 64 x 3 x 2000..4000 (14:2) 30 / 39.  Of 89 calls drawn over these
+// ranges the rule's form is 0.2 % behind the faster one on average, 13 % at worst.
 bool tensor_pays(int64_t rows, int64_t units, int64_t bound, int dim) {
   const int64_t work = units * ((rows + 31) / 32) * bound * (dim / 64);
-  if (rows > 32) return work > (dim == 64 ? 200000 : 160000) + 1500 * units * ((rows + kTreeTcRows - 1) / kTreeTcRows);
+  if (rows > 32) return work > 225000 + 1500 * units * ((rows + kTreeTcRows - 1) / kTreeTcRows);
   return rows > 16 && dim == 128 && work > 250000;
 }
 
@@ -546,8 +583,10 @@ Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound
     p.parts = 2 * kTreeTcCtas;
     return p;
   }
+  p.chunk = 64;
   // Parts by their cost in keys: waves of CTAs, each with 256 keys' worth of beginning and end; then the merge, by the cluster (64)
-  // or by a kernel of its own (192 and 4 a part).  us with the most parts that fit, cluster / kernel / one part, 14:2 heads of 64:
+  // or by a kernel of its own (192 and 4 a part).  us with the most parts that fit, cluster / kernel / one part, 14:2 heads of 64 (with
+  // loops that took 5 to 10 % longer):
   // 1 x 1 x 300 5.1 / 6.1 / 5.6, 1 x 1 x 4000 8.4 / 8.1 (17 parts) / 31.8, 32 x 1 x 500..1000 7.3 / 8.9 / 10.7, 16 x 1 x 8192 18.4 /
   // 19.7 / 69, 5 x 23 x 0..777 9.5 / 10.1 / 13.5, 1 x 48 x 4096 15.3 / 14.3 (12 parts) / 45.6, 64 x 8 x 200..1500 30.8 / 28.4 / 25.6;
   // 32:8 heads of 128: 8 x 3 x 2000..4000 27.3 / 31.9 / 67.  The most parts of every number of waves are looked at.  (Equal shares of
@@ -568,6 +607,17 @@ Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound
     const int64_t cost = (units * s + kSlots[s - 1] - 1) / kSlots[s - 1] * (part + 256) + 64;
     if (cost < least) least = cost, best = s, p.cluster = true;
   }
+  // ... or each warp has 32 rows of its own and all keys, with a quarter of the CTAs and no merge: for many rows and few keys, where
+  // the warps have rows.  us keys by warps / rows by warps: 14:2 heads of 64, 64 x 16 x 15..30 12.6 / 9.6, x 50..100 12.9 / 11.8,
+  // x 200..400 19.1 / 23.0; 32:8 of 128, 20 x 28 x 7..15 18.5 / 15.4, x 50..100 21.1 / 23.1, 64 x 16 x 10..20 33.4 / 24.2; 8:8 of 64,
+  // 20 x 40 x 25..50 (40 rows) 7.5 / 10.9.
+  const int64_t wide = (rows + kByRowsTile - 1) / kByRowsTile, wide_units = (int64_t)requests * kv_heads * wide;
+  if (best == 1 && rows > 32 && 2 * rows >= wide * kByRowsTile &&
+      192 + (wide_units + slots - 1) / slots * ((dim == 64 ? 4 : 6) * bound + 96) <
+          256 + (units + slots - 1) / slots * ((bound + 63) / 64 * 64 + 96)) {
+    p.tile_rows = kByRowsTile, p.tiles = wide;
+    return p;
+  }
   p.chunk = (int)(((bound + best - 1) / best + 63) / 64 * 64);
   if (p.chunk < 64) p.chunk = 64;
   p.splits = (int)((bound + p.chunk - 1) / p.chunk);
@@ -580,9 +630,10 @@ int64_t first_bytes(const Plan& p, int requests) { return p.tc ? ((int64_t)reque
 
 template <typename T, int D>
 int launch_typed(const TreeArgs& a, const Plan& p, cudaStream_t st) {
-  const int rc = p.tc              ? tree_attn_tc_launch(a, kTreeExponent<T> == kTreeExponent<__nv_bfloat16>, D, st)
-                 : a.max_new * (int64_t)a.group.d <= 16 ? launch_few<T, D, 1>(a, st)
-                                   : launch_few<T, D, 2>(a, st);
+  const int rc = p.tc                             ? tree_attn_tc_launch(a, kTreeExponent<T> == kTreeExponent<__nv_bfloat16>, D, st)
+                 : p.tile_rows == kByRowsTile     ? launch_few<T, D, 2, true>(a, st)
+                 : a.max_new * (int64_t)a.group.d <= 16 ? launch_few<T, D, 1, false>(a, st)
+                                                        : launch_few<T, D, 2, false>(a, st);
   if (rc != QUIC_OK || p.parts == 0) return rc;
   const dim3 grid((unsigned)(a.tiles * (a.tile_rows / 32) * (D / 16)), a.kv_heads, a.requests);
   QUIC_CUDA(launch(p.tc ? tree_merge_kernel<T, D, true> : tree_merge_kernel<T, D, false>, grid, dim3(256), 0, st, true, a));

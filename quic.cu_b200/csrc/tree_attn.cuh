@@ -91,6 +91,27 @@ __device__ __forceinline__ float tree_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ uint64_t pair2(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ void unpair2(uint64_t d, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(d)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // Two values in a word of the tensors' type.
 template <typename T>
 __device__ __forceinline__ uint32_t tree_pack(float x, float y);
@@ -137,11 +158,15 @@ __device__ __forceinline__ uint32_t tree_finite(uint32_t w) {
   return w & ~((tree_not_finite<T>(w) >> 15) * 0xffffu);
 }
 
-// fp16 weights are P = 2^(score - maximum + 8): probabilities down to 2^-22 stay normal.  bf16 has fp32's range.
+// The reference point of a row's exponentials moves only when its maximum has grown by more than 2^8: P and the sums stay far within
+// their types' ranges.
+constexpr float kTreeGrowth = 8.f;
+// P = 2^(score - reference + shift), the scores to base 2: fp16 weights reach 2^15 and stay normal down to 2^-21 of the reference.  bf16
+// has fp32's range.
 template <typename T>
 constexpr float kTreeShift = 0.f;
 template <>
-constexpr float kTreeShift<half> = 8.f;
+constexpr float kTreeShift<half> = 7.f;
 
 // The throughput form (tree_attn_tc.cu) takes what TMA can fetch.
 bool tree_attn_tc_takes(int block_size, int64_t k_block, int64_t k_head, int64_t k_tok, int64_t v_block, int64_t v_head, int64_t v_tok);

@@ -9,8 +9,7 @@
 //   softmax        a thread owns a row (TMEM lane): P = exp2(..) rounded to the tensors' type, which replaces the scores as
 //                  the A operand of the second product; warps without rows rest;
 //   O += P V       B = the V tile as it lies in the cache (token-major, the transposed form), N = the head dims.
-// The reference point of a row's exponentials moves only when its maximum has grown by more than 2^8 (P and the sums stay far
-// within their types' ranges); O is rescaled in tensor memory then.
+// O is rescaled in tensor memory when a row's reference point moves (kTreeGrowth).
 // K and V come by TMA, in boxes of as many tokens as lie together in a block for sure (the largest power of two that divides
 // the block size, 8 to 64); positions without a block are fetched from beyond the planes, as zeros.  (By cp.async, which takes
 // any block size, the loaders had to fence every stage for the tensor cores, and the fence waited for all copies under way:
@@ -37,11 +36,6 @@ constexpr int kRows = 128, kKeys = 64, kGroupWarps = 4, kSoftmaxWarps = 2 * kGro
 constexpr int kTmaWarp = kSoftmaxWarps + 2, kThreads = (kTmaWarp + 2) * 32;
 constexpr int kLeastShare = 2;  // key tiles of a CTA
 static_assert(2 * kRows == kTreeTcRows && kKeys == kTreeTcKeys, "two streams of rows");
-constexpr float kGrowth = 8.f;    // of a row's maximum (base 2) before its reference point follows
-template <typename T>
-constexpr float kShift = 0.f;     // P = 2^(score - reference + shift)
-template <>
-constexpr float kShift<half> = 7.f;  // up to 2^15, normal down to 2^-21 of the reference
 constexpr uint32_t kHalfQ = kRows * 128, kHalfK = kKeys * 128;  // 64 dims of Q, of a K or V tile
 
 struct TreeTcArgs {
@@ -62,27 +56,6 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
-}
-__device__ __forceinline__ uint64_t pair2(float x, float y) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
-  return d;
-}
-__device__ __forceinline__ void unpair2(uint64_t d, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(d)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
 }
 // D[tmem] (+)= A[tmem] . B, A 16-bit values packed two to a column
 __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -469,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
 #pragma unroll
         for (int j = 0; j < 64; j += 2) mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], x[j], x[j + 1]);
         const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;  // (the scale is positive)
-        const bool grown = mt > m_run + kGrowth;  // (from -inf: by any score)
+        const bool grown = mt > m_run + kTreeGrowth;  // (from -inf: by any score)
         if (k == 0) {
           m_run = mt;
         } else if (__any_sync(0xffffffffu, grown)) {
@@ -489,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
             tmem_st16(at_o + 16u * c, w);
           }
         }
-        const float ref = kShift<T> - (m_run == -INFINITY ? 0.f : m_run);
+        const float ref = kTreeShift<T> - (m_run == -INFINITY ? 0.f : m_run);
         const uint64_t ref2 = pair2(ref, ref);
         uint64_t l2[2] = {0ull, 0ull};
 #pragma unroll
