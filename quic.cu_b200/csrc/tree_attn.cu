@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a) {
   int64_t part0, part, step;  // the parts are part0, then part + step, part + 2 step, ...
   if constexpr (kTc) {  // the CTA where the row tile begins has it as its last segment, the others as their first
     const TreeUnits u = tree_units(a, r);
-    const int64_t share = a.first[a.requests + 1], t0 = a.first[blockIdx.z] + ((int64_t)kvh * u.row_tiles + tile) * u.key_tiles;
+    const int64_t share = a.first[a.requests + 1], t0 = a.first[blockIdx.z] + ((int64_t)kvh * u.row_tiles + tile) * u.line_tiles;
     const int64_t t1 = t0 + u.key_tiles - 1;
     const bool narrow = t1 <= 0xffffffffll;  // (a division of 64 bits takes as long as a round of loads)
     const int64_t c0 = narrow ? (int64_t)((uint32_t)t0 / (uint32_t)share) : t0 / share;
@@ -542,24 +542,27 @@ int launch_few(const TreeArgs& a, cudaStream_t st) {
   return QUIC_OK;
 }
 
+// What the end of a segment and the beginning of the next cost a CTA of the tcgen05 form, in key tiles.  us with 0 / 3 / 5 / 7 / 9: 64 x 8
+// x 200..1500 (14:2) 26.2 / 23.7 / 22.5 / 22.0 / 23.0, 27 x 25 x 5074..10148 (16:1) 74.8 / 72.9 / 71.0 / 71.4 / 72.2, 8 x 64 x 12000..16384
+// 145.6 / 143.8 / 142.7 / 142.6 / 143.0, 10 x 38 x 4..23 (16:1) 22.0 / 14.5 / 14.4 / 14.3 / 14.6.
+constexpr int kLineGap = 6;
 constexpr int64_t kMostTokens = 1 << 29;  // of a request: sums of two counts stay within an int
 // Which form takes a call, by the rows of a request and KV head and by the work of the mma.sync form, in tiles of 32 rows x keys of
 // 64 dims (for all requests, of the longest's keys).  The tcgen05 form has three times its throughput where it has the rows for it,
-// but 8 us more of launch and merge, and 3 us for every row tile of a CTA.  requests x nodes x tokens, us mma.sync / tcgen05:
-//   heads 14:2, dim 64:  5 x 23 x 388..777 9.5 / 14.3 (work 48,000), 1 x 48 x 4096 13.6 / 18.1 (91,000), 2 x 32 x 8192 18.5 / 20.2
-//                        (230,000), 64 x 5 x 500..1000 17.0 / 23.9 (257,000), 16 x 16 x 1024..2048 18.8 / 16.8 (264,000),
-//                        64 x 8 x 750..1500 23.0 / 27.5 (386,000), 16 x 8 x 4096..8192 30.2 / 25.6 (525,000)
-//   heads 32:8, dim 128: 20 x 28 x 7..15 15.3 / 22.9 (55,000), 4 x 41 x 182..365 18.2 / 22.1 (156,000), 8 x 9 x 512..1024 22.7 / 21.3
-//                        (264,000), 4 x 9 x 2048..4096 34.8 / 23.7 (525,000), 8 x 64 x 16384 907 / 150
-//   heads 16:1, dim 128: 22 x 58 x 30..150 24.2 / 33.6 (265,000), 60 x 4 x 220..1108 23.7 / 20.8 (267,000), 3 x 46 x 1488 19.0 / 21.5
-//                        (212,000)
-// Up to 32 rows it is ahead for long keys of 128 dims alone: 16:1 heads, 32 x 2 x 1024..2048 17.3 / 19.1 (131,000), x 4096..8192 35.1 /
-// 32.3 (524,000); of 64 dims 9 x 13 x 7247..14495 (8:8) 44 / 59, 64 x 3 x 2000..4000 (14:2) 30 / 39.  Of 89 calls drawn over these
-// ranges the rule's form is 0.2 % behind the faster one on average, 13 % at worst.
+// but 6 us more of launch and merge, and 3 us for every row tile of a CTA.  requests x nodes x tokens, us mma.sync / tcgen05:
+//   heads 14:2, dim 64:  5 x 23 x 388..777 9.6 / 13.1 (work 48,000), 1 x 48 x 4096 13.6 / 15.9 (91,000), 2 x 32 x 8192 18.5 / 18.9
+//                        (230,000), 64 x 5 x 500..1000 17.0 / 20.3 (257,000), 16 x 16 x 1024..2048 18.8 / 14.5 (264,000),
+//                        64 x 8 x 750..1500 22.9 / 24.2 (386,000), 16 x 8 x 4096..8192 30.2 / 23.5 (525,000)
+//   heads 32:8, dim 128: 20 x 28 x 7..15 15.3 / 23.2 (55,000), 4 x 16 x 512..1024 16.8 / 14.4 (133,000), 8 x 9 x 512..1024 22.7 / 19.3
+//                        (264,000), 16 x 9 x 256..512 21.2 / 22.7 (267,000), 4 x 9 x 2048..4096 34.7 / 21.3 (525,000)
+//   heads 16:1, dim 128: 16 x 2 x 1024..2048 16.4 / 14.5 (66,000), 4 x 8 x 2048..4096 16.8 / 15.5 (131,000), 22 x 58 x 30..150 24.2 /
+//                        27.2 (265,000), 32 x 2 x 4096..8192 34.8 / 30.7 (524,000)
+// Of up to 32 rows and 64 dims 9 x 13 x 7247..14495 (8:8) 44 / 56, 64 x 3 x 2000..4000 (14:2) 30 / 36.  Of 89 calls drawn over these
+// ranges the rule's form is 0.6 % behind the faster one on average, 12 % at worst.
 bool tensor_pays(int64_t rows, int64_t units, int64_t bound, int dim) {
   const int64_t work = units * ((rows + 31) / 32) * bound * (dim / 64);
-  if (rows > 32) return work > 225000 + 1500 * units * ((rows + kTreeTcRows - 1) / kTreeTcRows);
-  return rows > 16 && dim == 128 && work > 250000;
+  return (rows > 32 || (rows > 16 && dim == 128)) &&
+         work > (dim == 64 ? 225000 : 112500) + 1500 * units * ((rows + kTreeTcRows - 1) / kTreeTcRows);
 }
 
 // CTAs of the mma.sync form that run at once, by the size of their clusters (148 SMs of two, as the GPU's groups of SMs allow)
@@ -687,7 +690,7 @@ extern "C" int quic_tree_attn(const quic_tree_attn_t* t, void* scratch, void* st
   QUIC_REQUIRE(t->requests <= 65535 && t->kv_heads * p.tiles <= 65535, QUIC_E_LIMIT,
                "tree_attn: more than 65535 requests, or row tiles of one");
   TreeArgs a = {};
-  a.splits = p.splits, a.chunk = p.chunk, a.cluster = p.cluster, a.tiles = (int)p.tiles, a.tile_rows = p.tile_rows;
+  a.splits = p.splits, a.chunk = p.chunk, a.cluster = p.cluster, a.line_gap = kLineGap, a.tiles = (int)p.tiles, a.tile_rows = p.tile_rows;
   QUIC_REQUIRE(p.parts == 0 || (scratch != nullptr && (uintptr_t)scratch % 16 == 0), QUIC_E_ARG,
                "tree_attn: scratch missing or not 16-byte aligned");
   a.q = t->q, a.k = t->k, a.v = t->v, a.out = t->out;

@@ -16,12 +16,13 @@ struct TreeArgs {
   const uint32_t* mask;              // [rows][mask_words] by mask_row, or nullptr: node i sees nodes 0 .. i
   float4* part_o;                    // partial results [parts][dim / 4][tile_rows]
   float2* part_ml;                   // [parts][tile_rows]: maximum (base 2), sum
-  int64_t* first;                    // tcgen05 form: key tiles of the requests before each and of all, then a CTA's share
+  int64_t* first;                    // tcgen05 form: key tiles (with gaps) of the requests before each and of all, then a CTA's share
   FastDiv block, group;              // tokens per block, query heads per KV head
   int32_t rows, requests, heads, kv_heads, n_blocks, max_blocks, mask_words, max_new;
   int32_t tiles, tile_rows;          // row tiles of a request and KV head at most, rows of one
   int32_t splits, chunk;             // mma.sync form: CTAs per request, KV head and row tile at most; the tokens of one at least
-  int32_t cluster;                   // ... which are a cluster and merge their results themselves
+  int32_t line_gap;                  // tcgen05 form: key tiles' worth of time that a segment costs
+  int32_t cluster;                   // mma.sync form: these CTAs are a cluster and merge their results themselves
   float scale_log2;
 };
 
@@ -53,19 +54,22 @@ __device__ __forceinline__ int64_t tree_part(const TreeArgs& a, int b, int kvh, 
 }
 
 // tcgen05 form: the work is a line of key tiles (64 keys of one row tile), request after request, KV head after KV head, row
-// tile after row tile; every CTA has an equal share of the line.  A row tile's tiles that one CTA has are a segment.
+// tile after row tile; every CTA has an equal share of the line.  A row tile's tiles that one CTA has are a segment.  Behind each row
+// tile's last tile lie some (line_gap) that are no work, for the time that the end of a segment and the beginning of the next take.
 constexpr int kTreeTcRows = 256, kTreeTcKeys = 64, kTreeTcCtas = 148;
 struct TreeUnits {   // of a request
   int rows;          // (node, head) pairs per KV head
   int row_tiles;
   int key_tiles;     // of each row tile; one without keys writes zeros
-  __device__ __forceinline__ int64_t all(const TreeArgs& a) const { return (int64_t)row_tiles * a.kv_heads * key_tiles; }
+  int line_tiles;    // ... and the gap
+  __device__ __forceinline__ int64_t all(const TreeArgs& a) const { return (int64_t)row_tiles * a.kv_heads * line_tiles; }
 };
 __device__ __forceinline__ TreeUnits tree_units(const TreeArgs& a, const TreeRequest& r) {
   TreeUnits u;
   u.rows = min(r.n, a.max_new) * (int)a.group.d;
   u.row_tiles = (u.rows + kTreeTcRows - 1) / kTreeTcRows;
   u.key_tiles = max(1, (r.end + kTreeTcKeys - 1) / kTreeTcKeys);
+  u.line_tiles = u.key_tiles + a.line_gap;
   return u;
 }
 

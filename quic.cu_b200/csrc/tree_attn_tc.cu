@@ -18,10 +18,11 @@
 // must not see: such values are zeroed in shared memory and added, at the end, to the rows that see them.
 //
 // The CTAs have equal shares of the line of key tiles of all requests (tree_attn.cuh): the same case 193 -> 143 us, with an issuer
-// per stream instead of one for both.  148 us now (3.2 TB/s, 660 TFLOP/s; 172 in a loop of seconds, under the power limit).  Of
-// them K and V alone take 101, with the products 112; tensor pipe 49 %, exponentials 32 %, HBM 46 % busy: the streams' stages wait
-// for one another.  Tried and behind: scores fetched during the last exponentials 153, weights by the old maximum before the new
-// one is known 157, two threads a row 187, two CTAs an SM with a stream each 27 -> 31 us at 4 x 15 x 6146.
+// per stream instead of one for both.  142 us now (3.4 TB/s, 690 TFLOP/s).  Of them K and V alone take 101, with the products 112.  A
+// softmax warp takes 1900 clocks a tile (850 for the 64 exponentials a thread, 280 for the maximum, 100 for the load, 500 for barriers
+// and the way round) and is the slowest part; two of them share a scheduler, whose exponentials are 54 % busy; tensor pipe 49 %, HBM
+// 50 %.  Tried and behind: scores fetched during the last exponentials 153, weights by the old maximum before the new one is known
+// 157, two threads a row 187, one lane of a warp waiting for all 170, two CTAs an SM with a stream each 27 -> 31 us at 4 x 15 x 6146.
 //
 // Roles: warps 0-7 queries, softmax and epilogue, warps 8 and 9 MMA issuers of the two streams, warps 10 and 11
 // TMA of K and V.  Every wait is bounded; a wait that runs out sets word 0 of the tensor path's error words and the CTA leaves with
@@ -108,23 +109,25 @@ struct Walk {
     while (left > 0) {
       s.r = tree_request(a, b);
       const TreeUnits u = tree_units(a, s.r);
+      s.b = b;
       if (u.rows == 0) {
         ++b;
         continue;
       }
       // (a division of 64 bits takes longer than a key tile's products)
-      const uint32_t unit = at <= 0xffffffffll ? (uint32_t)at / (uint32_t)u.key_tiles : (uint32_t)(at / u.key_tiles);
-      s.b = b;
+      const uint32_t unit = at <= 0xffffffffll ? (uint32_t)at / (uint32_t)u.line_tiles : (uint32_t)(at / u.line_tiles);
+      s.tile0 = (int)(at - (int64_t)unit * u.line_tiles);
+      s.n_tiles = (int)min(left, (int64_t)(u.key_tiles - s.tile0));
+      const int step = s.tile0 + max(s.n_tiles, 0) >= u.key_tiles ? u.line_tiles - s.tile0 : s.n_tiles;  // with the gap behind the last
+      at += step;
+      left -= step;
+      if (at == u.all(a)) ++b, at = 0;
+      if (s.n_tiles <= 0) continue;  // (began in a gap)
       s.kvh = (int)(unit / (uint32_t)u.row_tiles);
       s.r0 = (int)(unit - (uint32_t)s.kvh * u.row_tiles) * kTreeTcRows;
       s.rows = u.rows;
       s.halves = u.rows - s.r0 > kRows;
       s.key_tiles = u.key_tiles;
-      s.tile0 = (int)(at - (int64_t)unit * u.key_tiles);
-      s.n_tiles = (int)min(left, (int64_t)(u.key_tiles - s.tile0));
-      at += s.n_tiles;
-      left -= s.n_tiles;
-      if (at == u.all(a)) ++b, at = 0;
       return true;
     }
     return false;
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
     }
     for (int g = 0; g < 2; ++g)
       for (int x = 0; x < 2; ++x) {
-        mbar_init(smem_u32(&bar_s[g][x]), 1);
+        mbar_init(smem_u32(&bar_s[g][x]), 2);
         mbar_init(smem_u32(&bar_p[g][x]), kGroupWarps);
         mbar_init(smem_u32(&bar_o[g][x]), 1);
       }
@@ -219,10 +222,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
       int b = b0;
       for (int64_t n; (n = tree_units(a, tree_request(a, b)).all(a)) <= start - before; ++b) before += n;
       Walk first = {b, start - before, min(share, total - start)};
-      first.next(a, segment_s);
+      if (!first.next(a, segment_s)) segment_s.n_tiles = 0;
       walk_s = first;
     }
     __syncthreads();
+    if (segment_s.n_tiles == 0) {  // the share is all gap
+      if (warp == kSoftmaxWarps)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+      return;
+    }
   }
   Walk walk = walk_s;
   Segment s = segment_s, later;  // this one and the next, whose numbers are fetched ahead
@@ -307,6 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
             umma_f16(to, q + (uint64_t)((c >> 2) * (kHalfQ / 16)) + 2 * (c & 3), kt + (uint64_t)((c >> 2) * (kHalfK / 16)) + 2 * (c & 3),
                      idesc, c > 0 ? 1u : 0u);
           umma_commit(bar);
+          mbar_arrive_cta(bar);  // (hands on what it has seen of the stage: which boxes are there)
         }
         __syncwarp();
         return true;
@@ -379,16 +388,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
 
       // ---- softmax
       float m_run = -INFINITY, l_run = 0.f;
-      for (int k = 0; k < steps && ok; ++k) {
-        const int u = u0 + k, i = s.step_tile(group, k), n = ring + i, st = n % kRing, t = t_begin + i * kKeys;
+      const int stride = s.halves ? 1 : 2;  // of the stream's tiles
+      int i = s.step_tile(group, 0), st = (ring + i) % kRing, t = t_begin + i * kKeys, u = u0;
+      for (int k = 0; ok && k < steps; ++k, ++u, i += stride, t += stride * kKeys, st = st + stride < kRing ? st + stride : st + stride - kRing) {
         const uint32_t at_s = tmem + 128u * group + 64u * (u & 1) + lane_addr;
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_s[group][u & 1]), (u >> 1) & 1, limit));
         if (!ok) break;
-        // (complete: for what the TMA warps wrote, which this thread reads itself)
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_full[st]), (n / kRing) & 1, limit));
-        if (!ok) break;
         const bool tree = t + kKeys > s.r.len;
         if (tree) {  // (the same for all the CTA's rows)
+          // (complete: this thread reads itself what the copies brought)
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_full[st]), ((ring + i) / kRing) & 1, limit));
+          if (!ok) break;
           unsigned char* const v_tile = smem + kK + st * kStage + kTile;
           bool stored = s.halves;  // (each stream for itself, changed or not: the other's change may be under way)
 #pragma unroll 4
