@@ -18,11 +18,12 @@
 // must not see: such values are zeroed in shared memory and added, at the end, to the rows that see them.
 //
 // The CTAs have equal shares of the line of key tiles of all requests (tree_attn.cuh): the same case 193 -> 143 us, with an issuer
-// per stream instead of one for both.  142 us now (3.4 TB/s, 690 TFLOP/s).  Of them K and V alone take 101, with the products 112.  A
-// softmax warp takes 1900 clocks a tile (850 for the 64 exponentials a thread, 280 for the maximum, 100 for the load, 500 for barriers
-// and the way round) and is the slowest part; two of them share a scheduler, whose exponentials are 54 % busy; tensor pipe 49 %, HBM
-// 50 %.  Tried and behind: scores fetched during the last exponentials 153, weights by the old maximum before the new one is known
-// 157, two threads a row 187, one lane of a warp waiting for all 170, two CTAs an SM with a stream each 27 -> 31 us at 4 x 15 x 6146.
+// per stream instead of one for both.  134 to 136 us now (3.5 TB/s, 730 TFLOP/s).  Of them K and V alone take 101, with the products 112.  A
+// softmax warp takes 1900 clocks a tile (280 for the maximum, 100 for the load, 500 for barriers and the way round, the rest for the
+// weights) and is the slowest part; two of them share a scheduler.  With all exponentials on their unit (512 clocks a warp and tile, 54 %
+// busy) it was 143; three in eight are polynomials.  Tried and behind: scores fetched during the last exponentials 153, weights by the
+// old maximum before the new one is known 157, two threads a row 187, one lane of a warp waiting for all 170, two CTAs an SM with a
+// stream each 27 -> 31 us at 4 x 15 x 6146.
 //
 // Roles: warps 0-7 queries, softmax and epilogue, warps 8 and 9 MMA issuers of the two streams, warps 10 and 11
 // TMA of K and V.  Every wait is bounded; a wait that runs out sets word 0 of the tensor path's error words and the CTA leaves with
@@ -51,6 +52,24 @@ __device__ __forceinline__ void mbar_arrive_cta(uint32_t bar) {
 }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {  // zeros beyond `bytes`
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// 2^x of two x up to 127, without the unit for exponentials: x = n + f with n the nearest whole number (the low bits of x + 1.5 2^23),
+// 2^f = 1 + f (c1 + c2 f + c3 f^2 + c4 f^3) on [-1/2, 1/2], fitted to the least largest relative error, 2^-18.4, and 2^n put together
+// from its exponent.  Below -127: 0.  NaN stays.
+__device__ __forceinline__ void ex2_fma(uint64_t x2, float& p0, float& p1) {
+  float x, y;
+  unpair2(x2, x, y);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(-127.f));
+  const uint64_t q = pair2(x, y), n = add2(q, pair2(12582912.f, 12582912.f));
+  const uint64_t f = fma2(add2(n, pair2(-12582912.f, -12582912.f)), pair2(-1.f, -1.f), q);
+  uint64_t p = fma2(pair2(0.00958285f, 0.00958285f), f, pair2(0.05590642f, 0.05590642f));
+  p = fma2(p, f, pair2(0.24024099f, 0.24024099f));
+  p = fma2(p, f, pair2(0.69312419f, 0.69312419f));
+  p = fma2(p, f, pair2(1.f, 1.f));
+  unpair2(n, x, y);
+  unpair2(mul2(p, pair2(__int_as_float((__float_as_int(x) << 23) + 0x3f800000), __int_as_float((__float_as_int(y) << 23) + 0x3f800000))),
+          p0, p1);
 }
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
   asm volatile(
@@ -481,9 +500,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             float p0, p1;
-            unpair2(fma2(pair2(x[32 * h + 2 * j], x[32 * h + 2 * j + 1]), scale2, ref2), p0, p1);
-            p0 = tree_ex2(p0);  // 2^-inf = 0 for keys that are not seen
-            p1 = tree_ex2(p1);
+            const uint64_t e = fma2(pair2(x[32 * h + 2 * j], x[32 * h + 2 * j + 1]), scale2, ref2);
+            if (j % 8 == 1 || j % 8 == 4 || j % 8 == 6) {  // three in eight: none 143 us, two 134.8, three 133.9, four 139
+              ex2_fma(e, p0, p1);
+            } else {
+              unpair2(e, p0, p1);
+              p0 = tree_ex2(p0);  // 2^-inf = 0 for keys that are not seen
+              p1 = tree_ex2(p1);
+            }
             w[j] = tree_pack<T>(p0, p1);
             l2[j & 1] = add2(l2[j & 1], pair2(p0, p1));
           }

@@ -214,6 +214,26 @@ def test_a_nan_score_reaches_its_rows(form):
     assert torch.isnan(got[:, :7].float()).all() and torch.isfinite(got[:, 7:].float()).all()
 
 
+@pytest.mark.parametrize("key", range(0, 70, 3))
+def test_a_nan_score_of_any_key_reaches_its_rows(key):
+    """Whichever way the tcgen05 form takes for the key's exponential; unseen keys and scores far below stay without a trace."""
+    K.lib().quic_set_tree_attn_tensor(1)
+    try:
+        case = Case([70], [3], 16, tree=False, seed=key)
+        case.k[case.place(0, key)[0], 0, case.place(0, key)[1], 5] = float("nan")
+        got = case.call()
+        assert torch.isnan(got[:, :7]).all() and not torch.isnan(got[:, 7:]).any()
+        case = Case([70], [3], 16, tree=False, seed=key, dtype=torch.bfloat16)
+        block, at = case.place(0, key)
+        case.q[...] = 1.0
+        case.k[...] = 30.0
+        case.k[block, :, at] = -30.0  # 2^-690 beside the others'
+        case.v[block, :, at] = 3e38
+        assert (case.call().abs() < 8).all()
+    finally:
+        K.lib().quic_set_tree_attn_tensor(-1)
+
+
 def test_scores_of_the_lowest_value(form):
     """Keys that push a score to the type's end in either direction: the softmax stays finite."""
     case = Case([100], [6], 16, seed=2)
