@@ -447,14 +447,15 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
 }
 
 // Rows whose keys several CTAs shared: sum of the parts, each by 2^(its maximum - the largest).  A CTA has 32 rows of a tile
-// (a row a lane, so that parts are read in whole lines) and 16 head dimensions, a warp every eighth part; the warps meet in
-// shared memory.  Bound by two rounds of loads (with four warps that each read all parts of a row, 17 parts took 22 us).
-template <typename T, int D, bool kTc>
+// (a row a lane, so that parts are read in whole lines).  kFewParts: and all head dimensions, an eighth a warp, which reads all parts;
+// else 16 of them and a warp every eighth part, and the warps meet in shared memory.  Bound by two rounds of loads (17 parts a warp
+// 22 us).
+template <typename T, int D, bool kTc, bool kFewParts>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a) {
-  __shared__ float4 o_s[8][4][32];
-  __shared__ float2 ml_s[8][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y, quarter = blockIdx.x % (D / 16);
-  const int per_tile = a.tile_rows / 32, rows32 = blockIdx.x / (D / 16), tile = rows32 / per_tile, row = rows32 % per_tile * 32 + lane;
+  constexpr int kChunks = kFewParts ? D / 32 : 4;  // of four dims, a thread
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y;
+  const int rows32 = kFewParts ? blockIdx.x : blockIdx.x / (D / 16), chunk0 = kFewParts ? kChunks * warp : 4 * (blockIdx.x % (D / 16));
+  const int per_tile = a.tile_rows / 32, tile = rows32 / per_tile, row = rows32 % per_tile * 32 + lane;
   pdl_launch_dependents();
   pdl_wait();
   const TreeRequest r = tree_request(a, blockIdx.z);
@@ -478,44 +479,53 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a) {
   }
   if (parts == 1) return;
   float top = -INFINITY, l = 0.f;
-  float4 o[4] = {};
+  float4 o[kChunks] = {};
 #pragma unroll 4
-  for (int s = warp; s < parts; s += 8) {  // running maximum and sum
+  for (int s = kFewParts ? 0 : warp; s < parts; s += kFewParts ? 1 : 8) {  // running maximum and sum
     const int64_t at = s == 0 ? part0 : part + s * step;
     const float2 x = a.part_ml[at * a.tile_rows + row];
-    float4 y[4];
+    float4 y[kChunks];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) y[c] = a.part_o[(at * (D / 4) + 4 * quarter + c) * a.tile_rows + row];
+    for (int c = 0; c < kChunks; ++c) y[c] = a.part_o[(at * (D / 4) + chunk0 + c) * a.tile_rows + row];
     const float m = fmaxf(top, x.x), ref = m == -INFINITY ? 0.f : m, f = tree_ex2(top - ref), g = tree_ex2(x.x - ref);
     top = m;
     l = (f != 0.f ? f * l : 0.f) + (g != 0.f ? g * x.y : 0.f);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < kChunks; ++c) {
       o[c].x = (f != 0.f ? f * o[c].x : 0.f) + (g != 0.f ? g * y[c].x : 0.f);
       o[c].y = (f != 0.f ? f * o[c].y : 0.f) + (g != 0.f ? g * y[c].y : 0.f);
       o[c].z = (f != 0.f ? f * o[c].z : 0.f) + (g != 0.f ? g * y[c].z : 0.f);
       o[c].w = (f != 0.f ? f * o[c].w : 0.f) + (g != 0.f ? g * y[c].w : 0.f);
     }
   }
+  if constexpr (kFewParts) {
+    if (number < all) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c) o_s[warp][c][lane] = o[c];
-  ml_s[warp][lane] = make_float2(top, l);
-  __syncthreads();
-  if (warp >= 4 || number >= all) return;  // a warp four dims
-  float m = -INFINITY;
+      for (int c = 0; c < kChunks; ++c) write_out<T, D>(a, r, kvh, number, chunk0 + c, o[c], l);
+    }
+  } else {
+    __shared__ float4 o_s[8][4][32];
+    __shared__ float2 ml_s[8][32];
 #pragma unroll
-  for (int w = 0; w < 8; ++w) m = fmaxf(m, ml_s[w][lane].x);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float sum = 0.f;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < 4; ++c) o_s[warp][c][lane] = o[c];
+    ml_s[warp][lane] = make_float2(top, l);
+    __syncthreads();
+    if (warp >= 4 || number >= all) return;  // a warp four dims
+    float m = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const float2 x = ml_s[w][lane];
-    const float4 y = o_s[w][warp][lane];
-    const float f = tree_ex2(x.x - ref);
-    if (f != 0.f) sum += f * x.y, v.x += f * y.x, v.y += f * y.y, v.z += f * y.z, v.w += f * y.w;
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, ml_s[w][lane].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const float2 x = ml_s[w][lane];
+      const float4 y = o_s[w][warp][lane];
+      const float f = tree_ex2(x.x - ref);
+      if (f != 0.f) sum += f * x.y, v.x += f * y.x, v.y += f * y.y, v.z += f * y.z, v.w += f * y.w;
+    }
+    write_out<T, D>(a, r, kvh, number, chunk0 + warp, v, sum);
   }
-  write_out<T, D>(a, r, kvh, number, 4 * quarter + warp, v, sum);
 }
 
 template <typename T, int D, int MT, bool kByRows>
@@ -638,8 +648,15 @@ int launch_typed(const TreeArgs& a, const Plan& p, cudaStream_t st) {
                  : a.max_new * (int64_t)a.group.d <= 16 ? launch_few<T, D, 1, false>(a, st)
                                                         : launch_few<T, D, 2, false>(a, st);
   if (rc != QUIC_OK || p.parts == 0) return rc;
-  const dim3 grid((unsigned)(a.tiles * (a.tile_rows / 32) * (D / 16)), a.kv_heads, a.requests);
-  QUIC_CUDA(launch(p.tc ? tree_merge_kernel<T, D, true> : tree_merge_kernel<T, D, false>, grid, dim3(256), 0, st, true, a));
+  // few parts, and more CTAs of 16 dims than 148 SMs take at four each: us with a part a warp / with all of them, 8 x 64 x 16384 139 / 133
+  // (4096 CTAs), 27 x 25 x 10148 (16:1) 66.7 / 64.9, 64 x 8 x 1500 on tcgen05 21.6 / 21.4 (1024), 16 x 1 x 8192 on it 25.4 / 27.1 (128)
+  const int64_t units = (int64_t)a.requests * a.kv_heads * a.tiles, narrow = units * (a.tile_rows / 32) * (D / 16);
+  const bool few = narrow > 4 * 148 && (p.tc ? kTreeTcCtas / units + 2 : a.splits) <= 8;
+  const dim3 grid((unsigned)(a.tiles * (a.tile_rows / 32) * (few ? 1 : D / 16)), a.kv_heads, a.requests);
+  if (p.tc)
+    QUIC_CUDA(launch(few ? tree_merge_kernel<T, D, true, true> : tree_merge_kernel<T, D, true, false>, grid, dim3(256), 0, st, true, a));
+  else
+    QUIC_CUDA(launch(few ? tree_merge_kernel<T, D, false, true> : tree_merge_kernel<T, D, false, false>, grid, dim3(256), 0, st, true, a));
   return QUIC_OK;
 }
 

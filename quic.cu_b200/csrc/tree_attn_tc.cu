@@ -18,7 +18,7 @@
 // must not see: such values are zeroed in shared memory and added, at the end, to the rows that see them.
 //
 // The CTAs have equal shares of the line of key tiles of all requests (tree_attn.cuh): the same case 193 -> 143 us, with an issuer
-// per stream instead of one for both.  134 to 136 us now (3.5 TB/s, 730 TFLOP/s).  Of them K and V alone take 101, with the products 112.  A
+// per stream instead of one for both.  132 us now (3.6 TB/s, 750 TFLOP/s).  Of them K and V alone take 101, with the products 112.  A
 // softmax warp takes 1900 clocks a tile (280 for the maximum, 100 for the load, 500 for barriers and the way round, the rest for the
 // weights) and is the slowest part; two of them share a scheduler.  With all exponentials on their unit (512 clocks a warp and tile, 54 %
 // busy) it was 143; three in eight are polynomials.  Tried and behind: scores fetched during the last exponentials 153, weights by the
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
           for (int j = 0; j < 16; ++j) {
             float p0, p1;
             const uint64_t e = fma2(pair2(x[32 * h + 2 * j], x[32 * h + 2 * j + 1]), scale2, ref2);
-            if (j % 8 == 1 || j % 8 == 4 || j % 8 == 6) {  // three in eight: none 143 us, two 134.8, three 133.9, four 139
+            if (j % 8 == 1 || j % 8 == 4 || j % 8 == 6) {  // three in eight: none 143 us, two 134.8, three 133.9, four 139 (with a slower merge)
               ex2_fma(e, p0, p1);
             } else {
               unpair2(e, p0, p1);
