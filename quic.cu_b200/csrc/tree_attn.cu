@@ -13,12 +13,14 @@
 // its own (cp.async, no barrier between warps), one pass with a running maximum and sum per row; the warps' results meet in
 // shared memory at the end, those of up to eight CTAs as well, which are a cluster then and each sum a share of the rows' dims (over
 // distributed shared memory), those of more CTAs in the merge kernel.  Bound: the bytes of K and V (16 x 1 x 8192, fp16, 14:2 heads
-// of 64: 17.6 us, 3.8 TB/s; 9 x 13 x 7247..14495, 8:8 heads: 42.5 us, 4.7 TB/s); with 32 rows what a warp's steps wait for of their own
-// results, two warps a scheduler (64 x 8 x 200..1500: 22.2 us, tensor pipe a fifth busy); for small calls the launch and what depends
+// of 64: 16.7 us, 4.0 TB/s; 9 x 13 x 7247..14495, 8:8 heads: 40.6 us, 4.9 TB/s); with 32 rows what a warp's steps wait for of their own
+// results, two warps a scheduler (64 x 8 x 200..1500: 18.8 us); for small calls the launch and what depends
 // on one another: lengths, table, keys, results (1 x 1 x 300: 5.0 us).  Moving the reference point for every larger maximum, sums of
-// the rounded weights and separate exponents cost 64 x 8 x 200..1500 25.5, 16 x 1 x 8192 18.4 us; places of keys computed once a key
-// instead of once a row, and the masks of the rows kept in shared memory, cost more than they saved (+0.2 to +1 us).
+// the rounded weights and separate exponents cost 64 x 8 x 200..1500 25.5 instead of 22.2 us; places of keys computed by the
+// lane of the key, and the masks of the rows kept in shared memory, cost more than they saved (+0.2 to +1 us).
 #include <math.h>
+
+#include <type_traits>
 
 #include "tree_attn.cuh"
 
@@ -154,23 +156,45 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
     const int id = p < t_end ? __ldg(table + a.block.div(p)) : -1;
     return id < a.n_blocks ? id : -1;
   };
+  const T* const k_lane = reinterpret_cast<const T*>(a.k) + kvh * a.k_head + lane % kPer * 8;
+  const T* const v_lane = reinterpret_cast<const T*>(a.v) + kvh * a.v_head + lane % kPer * 8;
+  const int run = a.max_blocks == 1 || a.block.d % 16 == 0 ? 16 : (a.block.d % 8 == 0 ? 8 : 0);
   auto request = [&](int t, int stage, int id) {
     const uint32_t ok = __ballot_sync(0xffffffffu, id >= 0) & kAllKeys;
     if (lane == 0) valid_s[warp][stage] = ok;
-    const int p = t + (lane & (kKeys - 1)), off = p - (int)a.block.div(p) * (int)a.block.d;
     const uint32_t dst = ring + stage * 2 * kRowsBytes;
     const int chunk = lane % kPer;
+    // Keys that lie in one block, one after the other: their place is looked up once (once a row, 64 x 8 x 200..1500 takes 22.2
+    // instead of 18.8 us, 9 x 13 x 14495 in blocks of 24, 42.3 instead of 40.6).
+    auto runs = [&](auto length) {
+      constexpr int kRun = decltype(length)::value;
 #pragma unroll
+      for (int h = 0; h < kKeys / kRun; ++h) {
+        const int64_t at = max(__shfl_sync(0xffffffffu, id, kRun * h), 0);
+        const int p = t + kRun * h, off = p - (int)a.block.div(p) * (int)a.block.d + lane / kPer;
+        const T* kp = k_lane + at * a.k_block + off * a.k_tok;
+        const T* vp = v_lane + at * a.v_block + off * a.v_tok;
+#pragma unroll
+        for (int i = 0; i < kRun / kAtOnce; ++i) {
+          const int row = kRun * h + i * kAtOnce + lane / kPer;
+          const uint32_t bytes = ok >> row & 1u ? 16u : 0u, to = dst + tile_at<D>(row, chunk);
+          cp_async16(to, kp, bytes);
+          cp_async16(to + kRowsBytes, vp, bytes);
+          kp += kAtOnce * a.k_tok, vp += kAtOnce * a.v_tok;
+        }
+      }
+    };
+    if (run == 16) return runs(std::integral_constant<int, 16>{});
+    if (run == 8) return runs(std::integral_constant<int, 8>{});
+    const int p = t + (lane & (kKeys - 1)), off = p - (int)a.block.div(p) * (int)a.block.d;
+#pragma unroll 1
     for (int i = 0; i < kKeys / kAtOnce; ++i) {
       const int row = i * kAtOnce + lane / kPer;
       const int bid = __shfl_sync(0xffffffffu, id, row), boff = __shfl_sync(0xffffffffu, off, row);
-      const int64_t at = max(bid, 0);
-      const int64_t o = bid >= 0 ? boff : 0;
-      const uint32_t bytes = bid >= 0 ? 16u : 0u;
-      cp_async16(dst + tile_at<D>(row, chunk), reinterpret_cast<const T*>(a.k) + at * a.k_block + kvh * a.k_head + o * a.k_tok + chunk * 8,
-                 bytes);
-      cp_async16(dst + kRowsBytes + tile_at<D>(row, chunk),
-                 reinterpret_cast<const T*>(a.v) + at * a.v_block + kvh * a.v_head + o * a.v_tok + chunk * 8, bytes);
+      const int64_t at = max(bid, 0), o = bid >= 0 ? boff : 0;
+      const uint32_t bytes = bid >= 0 ? 16u : 0u, to = dst + tile_at<D>(row, chunk);
+      cp_async16(to, k_lane + at * a.k_block + o * a.k_tok, bytes);
+      cp_async16(to + kRowsBytes, v_lane + at * a.v_block + o * a.v_tok, bytes);
     }
   };
 
@@ -187,7 +211,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attn_kernel(const TreeArgs a
   const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2);
   const int t_warp = t_begin + (kByRows ? 0 : warp * kKeys);
   int id = fetch(t_warp);
-#pragma unroll
+#pragma unroll(D == 64 && MT == 1 ? kStages - 1 : 1)  // (else code that is read once: 57.9 -> 54.3 us at 48 x 2 x 11707, 16:1 heads of 128)
   for (int s = 0; s < kStages - 1; ++s) {
     if (t_warp + s * step < t_end) request(t_warp + s * step, s, id);
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -560,15 +584,15 @@ constexpr int64_t kMostTokens = 1 << 29;  // of a request: sums of two counts st
 // Which form takes a call, by the rows of a request and KV head and by the work of the mma.sync form, in tiles of 32 rows x keys of
 // 64 dims (for all requests, of the longest's keys).  The tcgen05 form has three times its throughput where it has the rows for it,
 // but 6 us more of launch and merge, and 3 us for every row tile of a CTA.  requests x nodes x tokens, us mma.sync / tcgen05:
-//   heads 14:2, dim 64:  5 x 23 x 388..777 9.6 / 13.1 (work 48,000), 1 x 48 x 4096 13.6 / 15.9 (91,000), 2 x 32 x 8192 18.5 / 18.9
-//                        (230,000), 64 x 5 x 500..1000 17.0 / 20.3 (257,000), 16 x 16 x 1024..2048 18.8 / 14.5 (264,000),
-//                        64 x 8 x 750..1500 22.9 / 24.2 (386,000), 16 x 8 x 4096..8192 30.2 / 23.5 (525,000)
-//   heads 32:8, dim 128: 20 x 28 x 7..15 15.3 / 23.2 (55,000), 4 x 16 x 512..1024 16.8 / 14.4 (133,000), 8 x 9 x 512..1024 22.7 / 19.3
-//                        (264,000), 16 x 9 x 256..512 21.2 / 22.7 (267,000), 4 x 9 x 2048..4096 34.7 / 21.3 (525,000)
-//   heads 16:1, dim 128: 16 x 2 x 1024..2048 16.4 / 14.5 (66,000), 4 x 8 x 2048..4096 16.8 / 15.5 (131,000), 22 x 58 x 30..150 24.2 /
-//                        27.2 (265,000), 32 x 2 x 4096..8192 34.8 / 30.7 (524,000)
-// Of up to 32 rows and 64 dims 9 x 13 x 7247..14495 (8:8) 44 / 56, 64 x 3 x 2000..4000 (14:2) 30 / 36.  Of 89 calls drawn over these
-// ranges the rule's form is 0.6 % behind the faster one on average, 12 % at worst.
+//   heads 14:2, dim 64:  5 x 23 x 388..777 9.2 / 12.9 (work 48,000), 1 x 48 x 4096 13.3 / 15.4 (91,000), 2 x 32 x 8192 16.8 / 18.5
+//                        (230,000), 64 x 5 x 500..1000 15.4 / 20.1 (257,000), 16 x 16 x 1024..2048 17.3 / 14.6 (264,000),
+//                        64 x 8 x 750..1500 21.7 / 23.1 (386,000), 16 x 8 x 4096..8192 28.7 / 22.4 (525,000)
+//   heads 32:8, dim 128: 20 x 28 x 7..15 15.5 / 17.3 (55,000), 4 x 16 x 512..1024 16.1 / 14.4 (133,000), 8 x 9 x 512..1024 21.5 / 20.7
+//                        (264,000), 16 x 9 x 256..512 20.3 / 22.2 (267,000), 4 x 9 x 2048..4096 31.5 / 21.0 (525,000)
+//   heads 16:1, dim 128: 16 x 2 x 1024..2048 15.5 / 14.4 (66,000), 4 x 8 x 2048..4096 16.4 / 15.1 (131,000), 32 x 2 x 4096..8192 32.6 /
+//                        30.2 (524,000)
+// Of up to 32 rows and 64 dims 9 x 13 x 7247..14495 (8:8) 41.7 / 53.3, 64 x 3 x 2000..4000 (14:2) 29.9 / 35.0.  Of 89 calls drawn over
+// these ranges the rule's form is 0.6 % behind the faster one on average.
 bool tensor_pays(int64_t rows, int64_t units, int64_t bound, int dim) {
   const int64_t work = units * ((rows + 31) / 32) * bound * (dim / 64);
   return (rows > 32 || (rows > 16 && dim == 128)) &&
@@ -649,9 +673,9 @@ int launch_typed(const TreeArgs& a, const Plan& p, cudaStream_t st) {
                                                         : launch_few<T, D, 2, false>(a, st);
   if (rc != QUIC_OK || p.parts == 0) return rc;
   // few parts, and more CTAs of 16 dims than 148 SMs take at four each: us with a part a warp / with all of them, 8 x 64 x 16384 139 / 133
-  // (4096 CTAs), 27 x 25 x 10148 (16:1) 66.7 / 64.9, 64 x 8 x 1500 on tcgen05 21.6 / 21.4 (1024), 16 x 1 x 8192 on it 25.4 / 27.1 (128)
+  // (4096 CTAs), 27 x 25 x 10148 (16:1) 66.7 / 64.9, 64 x 8 x 1500 on tcgen05 21.6 / 21.4 (1024), 16 x 1 x 8192 on it 25.4 / 27.1 (128), 8 x 48 x 2048 20 / 22 (1024, of six parts)
   const int64_t units = (int64_t)a.requests * a.kv_heads * a.tiles, narrow = units * (a.tile_rows / 32) * (D / 16);
-  const bool few = narrow > 4 * 148 && (p.tc ? kTreeTcCtas / units + 2 : a.splits) <= 8;
+  const bool few = narrow > 4 * 148 && (p.tc ? kTreeTcCtas / units + 2 : a.splits) <= 4;
   const dim3 grid((unsigned)(a.tiles * (a.tile_rows / 32) * (few ? 1 : D / 16)), a.kv_heads, a.requests);
   if (p.tc)
     QUIC_CUDA(launch(few ? tree_merge_kernel<T, D, true, true> : tree_merge_kernel<T, D, true, false>, grid, dim3(256), 0, st, true, a));
