@@ -127,8 +127,13 @@ int quic_w4a16_tensor_status(void);
  * more. */
 int32_t *quic_error_words_new(void);
 void quic_error_words_free(int32_t *words);
+/* What the calling thread launches from here on by stand-alone operators reports
+ * to these two words instead of the device's own (quic_w4a16_tensor_status);
+ * NULL: to the device's own again.  For a model that is driven operator by
+ * operator.  Calls with words of their own are not concerned. */
+int quic_error_words_watch(int32_t *words);
 /* Test hook for the bounded waits of the tcgen05 kernels (linears, lm_head,
- * prefill attention, the decode step's rows chain): in launches that follow a
+ * prefill and tree attention, the decode step's rows chain): in launches that follow a
  * wait lasts `wait_limit_us` microseconds at most (0: the default, two seconds)
  * and the operand tile of k block (attention: key tile) `skip_kblock` never
  * comes (-1: none), so the waits for it run out, every role of the CTA leaves

@@ -664,6 +664,13 @@ void tc_test_hook(uint32_t* wait_limit_us, int32_t* skip_kblock) {
 }
 }  // namespace quic
 
+extern "C" int quic_error_words_watch(int32_t* words) {
+  void* p = nullptr;
+  if (words != nullptr) QUIC_CUDA(cudaHostGetDevicePointer(&p, words, 0));
+  quic::t_status_words = static_cast<int*>(p);
+  return QUIC_OK;
+}
+
 extern "C" int32_t* quic_error_words_new(void) {
   quic::WordPool& pool = quic::word_pool();
   std::lock_guard<std::mutex> hold(pool.mu);

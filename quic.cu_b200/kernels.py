@@ -181,6 +181,7 @@ SIGNATURES = {
     "quic_decode_persist": (C.c_int, [C.POINTER(Model), C.POINTER(Decode), _P, _P, _I32, _P]),
     "quic_decode_persist_watch": (C.c_int, [C.POINTER(Model), C.POINTER(Decode), _P, _P, _I32, _P, _P]),
     "quic_decode_persist_status": (C.c_int, [_P, _P, C.POINTER(_I32)]),
+    "quic_error_words_watch": (C.c_int, [_P]),
     "quic_tree_attn": (C.c_int, [_P, _P, _P]),
     "quic_tree_attn_scratch_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I64]),
     "quic_set_tree_attn_tensor": (None, [C.c_int]),

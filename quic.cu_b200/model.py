@@ -18,6 +18,7 @@ tokenizer_path) -> (QUICForCausalLM, tokenizer)`` (src/model.py:306) and
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import itertools
 import json
@@ -75,6 +76,7 @@ class SlotCache:
         self._error_words = 0                      # address of page-locked words, where bounded waits that gave up report:
         self._step_error = self._prefill_error = C.c_int64(0)  # two words each of captured steps and of prefills, as one number
         self._persist_error = C.c_int32(0)                     # ... and that of the persistent kernel under decode_async()
+        self._verify_error = C.c_int64(0)                      # ... and the two of verify()
 
     def check_slots(self, slots, count: int, what: str) -> None:
         """Every kernel indexes the KV planes and the per-slot state by slot: a slot outside
@@ -108,28 +110,41 @@ class SlotCache:
         return t
 
     def error_words(self) -> int:
-        """Address of this cache's error words: captured steps +0, prefills +8, the persistent kernel +16."""
+        """Address of this cache's error words: captured steps +0, prefills +8, the persistent kernel +16, verify() +24."""
         if not self._error_words:
             at = K.lib().quic_error_words_new()
             if not at:
                 raise RuntimeError(K.lib().quic_last_error().decode("utf-8", "replace"))
             self._step_error, self._prefill_error = C.c_int64.from_address(at), C.c_int64.from_address(at + 8)
             self._persist_error = C.c_int32.from_address(at + 16)
+            self._verify_error = C.c_int64.from_address(at + 24)
             self._error_words = at
         return self._error_words
 
     def raise_errors(self) -> None:
-        """Raises if a bounded wait gave up in a prefill or step of this cache, as far as they have run: a caller who
+        """Raises if a bounded wait gave up in a prefill, step or verify of this cache, as far as they have run: a caller who
         has synchronised hears of all of them.  Reads page-locked memory and costs no synchronisation."""
-        for what, word in (("a prefill", self._prefill_error), ("a step", self._step_error), ("a step", self._persist_error)):
+        for what, word in (("a prefill", self._prefill_error), ("a step", self._step_error), ("a step", self._persist_error),
+                           ("a verify", self._verify_error)):
             if word.value:
                 status = word.value & 0xffffffff or word.value >> 32
                 word.value = 0
                 if word is self._persist_error:  # (its exchange area is as the wait left it)
                     K.check(K.lib().quic_decode_persist_status(K.ptr(self._persist_sync), K.stream_ptr(), C.byref(C.c_int32())),
                             "decode_persist_status")
+                lost = ("nothing of it is kept, the rows are as they were before" if word is self._verify_error else
+                        "its results and the rows' cache entries are invalid")
                 raise RuntimeError(f"quic_b200: a bounded wait of a kernel gave up (status 0x{status & 0xffffffff:x}) in {what} "
-                                   "of this cache: its results and the rows' cache entries are invalid")
+                                   f"of this cache: {lost}")
+
+    @contextlib.contextmanager
+    def watch(self, offset: int):
+        """The operators that this thread calls meanwhile report to this cache's error words at ``offset``."""
+        K.check(K.lib().quic_error_words_watch(self.error_words() + offset), "error_words_watch")
+        try:
+            yield
+        finally:
+            K.lib().quic_error_words_watch(None)
 
     def persist_sync(self) -> torch.Tensor:
         """Exchange area of the persistent decode kernel (zeroed once)."""
@@ -572,6 +587,9 @@ class QUICForCausalLM:
         node 0 of the tree, drafts[i][j] node j + 1.  ``parents[i][j]``: the node before which it is drafted to follow, 0 .. j;
         None: the drafts are a chain.  All rows' nodes must fit behind the cached tokens of their slots.
 
+        Raises if a bounded wait gave up in it, or in a prefill or step before it: nothing is accepted then, the rows' tokens,
+        positions and cached keys are as before the call.
+
         The linears run at the sum of the rows' nodes; attention is ``kernels.tree_attn`` over the slots, whose tables
         ``kernels.block_tables`` builds from the rows' lengths, and ``kernels.tree_commit`` keeps the branch."""
         cache.check_slots(slots, len(drafts), "verify")
@@ -606,23 +624,31 @@ class QUICForCausalLM:
         tables = slot.view(batch, 1).clone()
         row_start, slot_map, positions, mask = K.block_tables(tables, held, pool, lengths, n_new, cache.s_max, rows, parents=tree,
                                                               max_new=most)
-        tokens[row_start[:-1].long()] = cache.tok[at].long()
-        h = self.embed[tokens]
-        rms, lin = K.rmsnorm().forward, K.w4a16_linear
-        xn = rms(h, self.layers[0]["ln1"], self.eps)
-        for li, L in enumerate(self.layers):
-            k, v = cache.kv[li, 0], cache.kv[li, 1]
-            q = K.qkv_rope_append_at(lin(L["qkv"], xn), slot_map, positions, self.rope_cos, self.rope_sin, k, v)
-            attn = K.tree_attn(q.transpose(0, 1), k, v, tables, lengths, row_start, mask=mask, max_new=most, max_len=longest)
-            xn, h = rms(lin(L["o"], attn.view(rows, HIDDEN)), L["ln2"], self.eps, residual=h)
-            d = lin(L["down"], K.swiglu_fused(lin(L["gate_up"], xn)))
-            nxt = self.layers[li + 1]["ln1"] if li + 1 < self.n_layers else self.final_norm
-            xn, h = rms(d, nxt, self.eps, residual=h)
-        targets, _ = K.lm_head_argmax(xn, self.embed)
+        first = cache.tok[at]
+        tokens[row_start[:-1].long()] = first.long()
+        with cache.watch(24):
+            h = self.embed[tokens]
+            rms, lin = K.rmsnorm().forward, K.w4a16_linear
+            xn = rms(h, self.layers[0]["ln1"], self.eps)
+            for li, L in enumerate(self.layers):
+                k, v = cache.kv[li, 0], cache.kv[li, 1]
+                q = K.qkv_rope_append_at(lin(L["qkv"], xn), slot_map, positions, self.rope_cos, self.rope_sin, k, v)
+                attn = K.tree_attn(q.transpose(0, 1), k, v, tables, lengths, row_start, mask=mask, max_new=most, max_len=longest)
+                xn, h = rms(lin(L["o"], attn.view(rows, HIDDEN)), L["ln2"], self.eps, residual=h)
+                d = lin(L["down"], K.swiglu_fused(lin(L["gate_up"], xn)))
+                nxt = self.layers[li + 1]["ln1"] if li + 1 < self.n_layers else self.final_norm
+                xn, h = rms(d, nxt, self.eps, residual=h)
+            targets, _ = K.lm_head_argmax(xn, self.embed)
         path, accepted, following, after = K.tree_commit(cache.kv, tables, lengths, row_start, tree, tokens, targets, most)
         cache.tok[at] = following.to(torch.int32)
         cache.pos[at] = after
         back = torch.cat([accepted, following.to(torch.int32), path.view(-1)]).tolist()
+        try:
+            cache.raise_errors()
+        except RuntimeError:
+            cache.tok[at], cache.pos[at] = first, lengths
+            cache._verify_error.value = 0  # (where the error before it was raised)
+            raise
         out = []
         for i, s in enumerate(slots):
             kept = back[i]

@@ -178,3 +178,68 @@ def test_the_engine_hears_of_a_prefill_that_gave_up(tiny_model):
     with _Hook(), pytest.raises(RuntimeError, match="bounded wait.*in a prefill"):
         engine.run()
     assert K.lib().quic_w4a16_tensor_status() == 0
+
+
+def _verify_rows(net, cache):
+    """Three rows with prompts and drafts for them (the first two chains)."""
+    slots, g = [2, 0, 1], torch.Generator().manual_seed(3)
+    net.prefill(cache, slots, [torch.randint(0, 2048, (n,), generator=g) for n in (33, 130, 70)])
+    drafts = [torch.randint(0, 2048, (n,), generator=g).tolist() for n in (3, 5, 9)]
+    return slots, drafts, [[0, 1, 2], [0, 1, 2, 3, 4], [0, 0, 1, 2, 0, 4, 4, 6, 3]]
+
+
+@pytest.mark.parametrize("kernel", ["w4a16_linear", "tree_attn", "lm_head_argmax"])
+def test_a_verify_that_gave_up_raises_and_keeps_nothing(tiny_model, monkeypatch, kernel):
+    """Operands that come late change nothing.  Where those of one of its kernels never come, the call raises and names its
+    cache's call; tokens, positions, lengths and the K and V of cached tokens are as before, the next call is right, and no other
+    cache and no stand-alone operator hears of it."""
+    net, lib = tiny_model[0], K.lib()
+    inner, hook = getattr(K, kernel), [0, -1]
+
+    def hooked(*args, **more):
+        lib.quic_w4a16_tensor_test_hook(*hook)
+        try:
+            return inner(*args, **more)
+        finally:
+            lib.quic_w4a16_tensor_test_hook(0, -1)
+
+    lib.quic_set_tree_attn_tensor(1)
+    try:
+        plain, cache, other = (net.new_cache(n_slots=3, s_max=256) for _ in range(3))
+        slots, drafts, parents = _verify_rows(net, plain)
+        want = net.verify(plain, slots, drafts, parents)
+        _verify_rows(net, other)
+        _verify_rows(net, cache)
+        before = (list(cache.host_len), cache.tok.clone(), cache.pos.clone(), cache.kv.clone())
+        monkeypatch.setattr(K, kernel, hooked)
+        for skip in (0, 1) if kernel == "w4a16_linear" else (0,):
+            hook[:] = 2000, skip
+            with pytest.raises(RuntimeError, match="bounded wait.*in a verify"):
+                net.verify(cache, slots, drafts, parents)
+            hook[:] = 0, -1
+            cache.raise_errors()  # (heard of once)
+            assert cache.host_len == before[0] and torch.equal(cache.tok, before[1]) and torch.equal(cache.pos, before[2])
+            for s in slots:
+                assert torch.equal(cache.kv[:, :, s, :, :before[0][s]], before[3][:, :, s, :, :before[0][s]])
+            other.raise_errors()
+            assert lib.quic_w4a16_tensor_status() == 0
+        hook[:] = 50000, -300
+        assert net.verify(other, slots, drafts, parents) == want
+        hook[:] = 0, -1
+        assert net.verify(cache, slots, drafts, parents) == want
+        for s in slots:
+            assert torch.equal(cache.kv[:, :, s, :, :cache.host_len[s]], plain.kv[:, :, s, :, :cache.host_len[s]])
+    finally:
+        lib.quic_set_tree_attn_tensor(-1)
+        lib.quic_w4a16_tensor_status()
+
+
+def test_a_verify_hears_of_the_prefill_before_it(tiny_model):
+    net = tiny_model[0]
+    cache = net.new_cache(n_slots=2, s_max=256)
+    with _Hook():
+        net.prefill(cache, [0, 1], _prompts(2, 40))
+    with pytest.raises(RuntimeError, match="bounded wait.*in a prefill"):
+        net.verify(cache, [0, 1], [[1, 2], [3]])
+    cache.raise_errors()
+    assert K.lib().quic_w4a16_tensor_status() == 0
