@@ -395,8 +395,9 @@ void quic_set_tree_attn_tensor(int mode);
  *     (parents NULL: its number), 0 behind the last one;
  *   mask int32 [max_rows, mask_words] (with parents), the node's ancestors and
  *     itself, 0 behind the last one.
- * parents int32 [parent_rows] or NULL, one per row; an entry that is no earlier
- * node counts as -1.  All or nothing: where the pool lacks blocks (status: how
+ * parents int32 [parent_rows], one per row, an entry that is no earlier node counts
+ * as -1; or NULL: no trees.  An empty list has an address too (any that is not
+ * NULL): rows are then more than it has.  All or nothing: where the pool lacks blocks (status: how
  * many), a request needs more than max_blocks (status -1), or there are more rows
  * than max_rows or, with parents, than parent_rows or 32 * mask_words in a request
  * (status -2), no request gets rows or blocks: row_start is all 0.  Ended requests give theirs back all the

@@ -892,7 +892,7 @@ def block_tables(tables: torch.Tensor, held: torch.Tensor, pool: torch.Tensor, l
         words = -(-(max_rows if max_new is None else max_new) // 32) or 1
         if words < 1:
             raise RuntimeError("block_tables: max_new must not be negative")
-        parent_rows, parent_ptr = parents.shape[0], parents.data_ptr()
+        parent_rows = parents.shape[0]
     device = tables.get_device()
     if (device < 0 or held.get_device() != device or pool.get_device() != device or lengths.get_device() != device or
             n_new.get_device() != device or (parents is not None and parents.get_device() != device)):
@@ -902,6 +902,8 @@ def block_tables(tables: torch.Tensor, held: torch.Tensor, pool: torch.Tensor, l
         mask_ptr = mask.data_ptr()
     slot_map = torch.empty(max_rows, dtype=torch.int64, device=tables.device)
     row_start, positions = held.new_empty(requests + 1), held.new_empty(max_rows)
+    if parents is not None:  # (a tensor without elements has no address, which would say that there are no trees)
+        parent_ptr = parents.data_ptr() or row_start.data_ptr()
     call = _BLOCK_TABLES.pack(tables.data_ptr(), tables.stride(0), held.data_ptr(), pool.data_ptr(), lengths.data_ptr(),
                               n_new.data_ptr(), parent_ptr, row_start.data_ptr(), slot_map.data_ptr(), positions.data_ptr(),
                               mask_ptr, width, pool.shape[0] - 4, requests, block_size, parent_rows, words, max_rows)

@@ -579,6 +579,25 @@ def test_tables_in_a_graph_and_without_a_pool():
     assert start.tolist() == [0, 0, 0, 0] and int(pool[3]) == -1 and slots.tolist() == [-1] * 8
 
 
+@pytest.mark.parametrize("requests,block", [(1, 16), (5, 8)])
+def test_no_parents_at_all(requests, block):
+    """An empty list of parents is none for any row, not a chain: rows are refused, and without rows the masks are zero."""
+    i32 = functools.partial(torch.tensor, dtype=torch.int32, device="cuda")
+    tables, held, pool = torch.zeros(requests, 4, dtype=torch.int32, device="cuda"), i32([0] * requests), K.block_pool(9, "cuda")
+    none, lengths = i32([]), i32([0] * requests)
+    for mine in (none, i32([7])[1:]):
+        torch.full((6 * 2,), 0x5a5a5a5a, dtype=torch.int32, device="cuda")  # (what a result without a store may hold)
+        start, slots, positions, mask = K.block_tables(tables, held, pool, lengths, i32([1] * requests), block, 6, parents=mine, max_new=40)
+        assert int(pool[3]) == -2 and start.tolist() == [0] * (requests + 1) and slots.tolist() == [-1] * 6
+        assert positions.tolist() == [0] * 6 and mask.tolist() == [[0, 0]] * 6
+        assert held.tolist() == [0] * requests and int(pool[1]) == 9
+        torch.full((6 * 2,), 0x5a5a5a5a, dtype=torch.int32, device="cuda")
+        start, slots, positions, mask = K.block_tables(tables, held, pool, lengths, i32([0] * requests), block, 6, parents=mine, max_new=40)
+        assert int(pool[3]) == 0 and start.tolist() == [0] * (requests + 1) and slots.tolist() == [-1] * 6
+        assert positions.tolist() == [0] * 6 and mask.tolist() == [[0, 0]] * 6
+        assert K.block_tables(tables, held, pool, lengths, i32([0] * requests), block, 0, parents=mine)[3].shape == (0, 1)
+
+
 # ---- tree_commit -------------------------------------------------------------------------------
 def _walk(parents, tokens, targets):
     path, at = [0], 0
