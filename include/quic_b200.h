@@ -401,7 +401,7 @@ void quic_set_tree_attn_tensor(int mode);
  * many), a request needs more than max_blocks (status -1), or there are more rows
  * than max_rows or, with parents, than parent_rows or 32 * mask_words in a request
  * (status -2), no request gets rows or blocks: row_start is all 0.  Ended requests give theirs back all the
- * same.  Status 0: done.  A pool serves one stream at a time.  At most 4096
+ * same.  Status 0: done.  A pool serves one stream at a time.  1 to 4096
  * requests and 65535 * 256 rows.  Positions reach 2^29 at most. */
 int quic_block_tables(const quic_block_tables_t *t, void *stream);
 

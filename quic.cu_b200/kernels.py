@@ -858,7 +858,7 @@ def block_tables(tables: torch.Tensor, held: torch.Tensor, pool: torch.Tensor, l
     request, the first entries of its table row) and ``pool`` (``block_pool``) are updated in place: requests get the blocks
     that their rows need from the pool, ended ones give theirs back.  Returns
 
-    * ``row_start`` int32 [requests + 1], where each request's rows begin;
+    * ``row_start`` int32 [requests + 1] (there may be none), where each request's rows begin;
     * ``slot_map`` int64 [max_rows], block * block_size + offset per row, -1 behind the last;
     * ``positions`` int32 [max_rows], lengths + the depth of the row's node (without ``parents``: its number);
     * ``mask`` int32 [max_rows, words] with ``parents`` (int32, one per row: an earlier node of the request's tree or -1):
@@ -904,6 +904,10 @@ def block_tables(tables: torch.Tensor, held: torch.Tensor, pool: torch.Tensor, l
     row_start, positions = held.new_empty(requests + 1), held.new_empty(max_rows)
     if parents is not None:  # (a tensor without elements has no address, which would say that there are no trees)
         parent_ptr = parents.data_ptr() or row_start.data_ptr()
+    if requests == 0:  # (nothing to launch over: no rows, whatever the pool holds)
+        for t, value in ((row_start, 0), (slot_map, -1), (positions, 0), (pool[3], 0)):
+            t.fill_(value)
+        return row_start, slot_map, positions, mask if mask is None else mask.zero_()
     call = _BLOCK_TABLES.pack(tables.data_ptr(), tables.stride(0), held.data_ptr(), pool.data_ptr(), lengths.data_ptr(),
                               n_new.data_ptr(), parent_ptr, row_start.data_ptr(), slot_map.data_ptr(), positions.data_ptr(),
                               mask_ptr, width, pool.shape[0] - 4, requests, block_size, parent_rows, words, max_rows)

@@ -598,6 +598,27 @@ def test_no_parents_at_all(requests, block):
         assert K.block_tables(tables, held, pool, lengths, i32([0] * requests), block, 0, parents=mine)[3].shape == (0, 1)
 
 
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("max_rows", [0, 5])
+def test_tables_of_no_requests(max_rows, tree):
+    """A step without requests has no rows; tree_attn and tree_commit take what comes back."""
+    i32 = functools.partial(torch.tensor, dtype=torch.int32, device="cuda")
+    pool = K.block_pool(3, "cuda")
+    pool[3] = -2  # (of the call before)
+    tables, none = torch.zeros(0, 4, dtype=torch.int32, device="cuda"), i32([])
+    parents = i32([0] * max_rows) if tree else None
+    start, slots, positions, mask = K.block_tables(tables, i32([]), pool, none, none, 16, max_rows, parents=parents, max_new=40)
+    assert start.tolist() == [0] and start.dtype is torch.int32 and slots.tolist() == [-1] * max_rows and slots.dtype is torch.int64
+    assert positions.tolist() == [0] * max_rows and positions.dtype is torch.int32
+    assert mask is None if not tree else mask.tolist() == [[0, 0]] * max_rows and mask.dtype is torch.int32
+    assert pool.tolist() == [0, 3, 0, 0, 0, 1, 2]
+    kv = torch.zeros(1, 2, 3, 2, 16, 64, device="cuda").half()
+    q = torch.ones(max_rows, 14, 64, device="cuda").half()
+    assert torch.equal(K.tree_attn(q, kv[0, 0], kv[0, 1], tables, none, start, mask=mask, out=q), torch.ones_like(q))
+    path, accepted, following, after = K.tree_commit(kv, tables, none, start, i32([0] * max_rows), slots, slots, 4)
+    assert path.shape == (0, 4) and accepted.shape == following.shape == after.shape == (0,)
+
+
 # ---- tree_commit -------------------------------------------------------------------------------
 def _walk(parents, tokens, targets):
     path, at = [0], 0
