@@ -44,7 +44,7 @@ struct TreeTcArgs {
   TreeArgs t;
   int32_t box, log_boxes; // tokens of a TMA box, log2 of the boxes of a tile
   uint32_t wait_limit_us;
-  int32_t skip_tile;      // test hook: this key tile never comes; below -1, all come late (-1: none)
+  int32_t skip_tile;      // test hook: this key tile never comes; below -1, all come late, and issuers without a step (-1: none)
 };
 
 __device__ __forceinline__ void mbar_arrive_cta(uint32_t bar) {
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
         mbar_init(smem_u32(&bar_p[g][x]), kGroupWarps);
         mbar_init(smem_u32(&bar_o[g][x]), 1);
       }
-    mbar_init(smem_u32(&bar_q), kSoftmaxWarps);
+    mbar_init(smem_u32(&bar_q), kSoftmaxWarps + 2);
     mbar_init(smem_u32(&bar_drain), 2);
     fail_s = 0;
     odd_s[0] = odd_s[1] = 0x7fffffff;
@@ -319,6 +319,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_tc_kernel(const __grid_
     bool ok = true;
     for (int seg = 0; ok && more; s = later, more = more_later, ++seg) {
       const int steps = s.steps(g);
+      // Through with the segment before.  In a segment without a step for its stream nothing else waits for an issuer, which waits for a
+      // parity: two segments behind the others it would wait for a phase that has passed.
+      if (lane == 0) mbar_arrive_cta(smem_u32(&bar_q));
+      if (args.skip_tile < -1 && steps == 0) pause_us(min(-2 * args.skip_tile, (int)(args.wait_limit_us / 2)));
       const uint64_t q = q0 + (uint64_t)((s.halves ? g : 0) * (kQ / 16));
       auto scores = [&](int k) {
         const int n = ring + s.step_tile(g, k), st = n % kRing, x = (u + k) & 1;

@@ -470,6 +470,29 @@ def test_waits_that_give_up(layout):
         lib.quic_set_tree_attn_tensor(-1)
 
 
+@pytest.mark.parametrize("layout", [(14, 2, 64), (32, 8, 128)])
+def test_an_issuer_that_is_late_where_it_has_no_step(layout):
+    """Requests of one key tile each, several to a CTA of the tcgen05 form: the second stream has nothing to do, and its issuer comes
+    two tiles' time late to every one of them."""
+    lib = K.lib()
+    heads, kv_heads, dim = layout
+    requests = 1200 // kv_heads
+    case = Case([(7 * b) % 60 for b in range(requests)], [1 + b % 3 for b in range(requests)], 16, heads, kv_heads, dim, seed=dim)
+    lib.quic_set_tree_attn_tensor(1)
+    try:
+        want = case.call().clone()
+        for late in (-200, -40):
+            lib.quic_w4a16_tensor_test_hook(50000, late)
+            try:
+                got = case.call().clone()
+            finally:
+                lib.quic_w4a16_tensor_test_hook(0, -1)
+            assert lib.quic_w4a16_tensor_status() == 0 and torch.equal(got, want)
+        case.check(want)
+    finally:
+        lib.quic_set_tree_attn_tensor(-1)
+
+
 # ---- block_tables ----------------------------------------------------------------------------
 class Pool:
     """block_tables in Python integers."""
