@@ -3,6 +3,7 @@
 
 import functools
 import math
+import threading
 
 import pytest
 import torch
@@ -207,6 +208,32 @@ def test_what_a_row_does_not_see_does_not_reach_it(form, layout, nodes, value):
         assert torch.isnan(got[last].float()).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", LAYOUTS[:2])
+@pytest.mark.parametrize("block", [5, 8, 24, 64])
+@pytest.mark.parametrize("nodes,tree", [(3, True), (3, False), (40, True), (40, False)])
+def test_a_node_that_is_not_finite_reaches_the_rows_that_see_it(form, dtype, layout, block, nodes, tree):
+    """One value of one node's V is an infinity or NaN: the results of the rows that see the node show it there, and nothing else
+    changes; so it is for the last node, which without masks only its own row sees."""
+    heads, kv_heads, dim = layout
+    case = Case([70, 0, 301], [nodes, 2, nodes - 1], block, heads, kv_heads, dim, dtype, tree, seed=nodes + block)
+    clean, group = case.call().clone(), heads // kv_heads
+    for value, node in ((float("nan"), 1), (float("inf"), nodes // 2), (float("-inf"), nodes - 1)):
+        v = case.v.clone()
+        places, odd = [], torch.zeros_like(clean, dtype=torch.bool)
+        for b in range(3):
+            at = min(node, case.new[b] - 1)
+            place, off = case.place(b, case.lengths[b] + at)
+            case.v[place, 1, off, dim - 3] = value
+            for i, sees in enumerate(case.sees[b]):
+                if at in sees:
+                    odd[case.starts[b] + i, group:2 * group, dim - 3] = True
+        got = case.call()
+        assert torch.equal(got[~odd], clean[~odd]) and odd.any() and not odd.all(0).any()
+        assert torch.isnan(got[odd]).all() if math.isnan(value) else (got[odd] == value).all()
+        case.v = v
+
+
 def test_a_nan_score_reaches_its_rows(form):
     case = Case([3], [2], 16, seed=1)
     case.k[case.place(0, 1)[0], 0, 1] = float("nan")
@@ -311,6 +338,23 @@ def test_tables_shorter_than_the_lengths(form):
 def test_bounds_only_plan(form, bounds):
     case = Case([700, 5], [9, 1], 16, seed=6)
     case.check(case.call(**bounds))
+
+
+@pytest.mark.parametrize("tree", [True, False])
+@pytest.mark.parametrize("most", [1, 5, 33])
+@pytest.mark.parametrize("dtype,layout", [(torch.float16, (14, 2, 64)), (torch.bfloat16, (32, 8, 128))])
+def test_rows_beyond_the_bound_stay_unwritten(form, tree, most, dtype, layout):
+    """max_new below the rows of some requests: the rows up to it are right, the others of the request as they were."""
+    case = Case([300, 0, 41, 2000], [40, 3, 6, 34], 16, *layout, dtype=dtype, tree=tree, seed=most)
+    case.clear_unused()
+    out = torch.full_like(case.q, 7.0)
+    assert case.call(out=out, max_new=most) is out
+    want, size = case.want()
+    limit = 3.2 * HALF[dtype] * size + 2.0 ** -24 + (2040 * 2.0 ** -32 * 8 if dtype is torch.float16 else 0.0)  # (as in Case.check)
+    for b, n in enumerate(case.new):
+        s, e = case.starts[b], case.starts[b] + min(n, most)
+        assert ((out[s:e].double() - want[s:e]).abs() <= limit[s:e]).all()
+        assert (out[e:case.starts[b + 1]] == 7).all()
 
 
 def test_scale(form):
@@ -491,6 +535,31 @@ def test_an_issuer_that_is_late_where_it_has_no_step(layout):
         case.check(want)
     finally:
         lib.quic_set_tree_attn_tensor(-1)
+
+
+@pytest.mark.parametrize("lengths,new", [([3000, 900], [40, 9]), ([8000], [3])])
+def test_two_threads_on_one_stream(form, lengths, new):
+    """A call is several launches, and those of three threads interleave: each has scratch memory of its own."""
+    cases = [Case(lengths, new, 16, seed=s) for s in range(3)]
+    i32 = functools.partial(torch.tensor, dtype=torch.int32, device="cuda")
+    more = [(i32(c.lengths), i32(c.starts)) for c in cases]
+    want, got, start = [c.call() for c in cases], [[] for _ in cases], threading.Barrier(3)
+
+    def work(i):
+        c = cases[i]
+        start.wait()
+        for _ in range(200):
+            got[i].append(K.tree_attn(c.q, c.k, c.v, c.tables, *more[i], mask=c.mask, max_new=max(new), max_len=max(lengths)))
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert len(outs) == 200 and all(torch.equal(o, w) for o in outs)
 
 
 # ---- block_tables ----------------------------------------------------------------------------
@@ -721,6 +790,42 @@ def test_commit_leaves_bad_requests_alone():
     assert got[1].tolist() == [0, 2] and got[3].tolist() == [3, 16] and got[0].tolist() == [[-1] * 4, [0, 2, -1, -1]]
     assert got[2].tolist() == [-1, 1]
     assert torch.equal(kv, before)
+
+
+def test_two_threads_of_tables_and_commits():
+    """Steps of two threads with a pool and a cache each, on one stream: blocks, rows and masks, then the commit."""
+    i32 = functools.partial(torch.tensor, dtype=torch.int32, device="cuda")
+
+    def steps(seed, out, start=None):
+        kv = torch.randn(2, 2, 20, 2, 16, 64, device="cuda", generator=_gen(seed)).half()
+        tables, held, lengths = torch.zeros(4, 5, dtype=torch.int32, device="cuda"), i32([0] * 4), i32([0] * 4)
+        pool, new = K.block_pool(20, "cuda"), i32([3, 1, 0, 6])
+        parents, tokens = i32([-1, 0, 0, -1, -1, 0, 0, 1, 2, 2]), i32([0, seed, 1, 0, 0, 1 - seed, seed, 1, 1, 0])
+        targets = i32([1] * 10)
+        torch.cuda.synchronize()
+        if start is not None:
+            start.wait()
+        for _ in range(60):
+            row_start, slots, positions, mask = K.block_tables(tables, held, pool, lengths, new, 16, 10, parents=parents, max_new=6)
+            more = K.tree_commit(kv, tables, lengths, row_start, parents, tokens, targets, 6)
+            out.append([row_start, slots, positions, mask, *more])
+            lengths = more[3] % 60
+        out.append([tables, held, pool, lengths, kv])
+
+    want, got = [[], []], [[], []]
+    for seed in range(2):
+        steps(seed, want[seed])
+    start = threading.Barrier(2)
+    threads = [threading.Thread(target=steps, args=(seed, got[seed], start)) for seed in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert len(a) == len(b) == 61
+        for x, y in zip(a, b):
+            assert all(torch.equal(p, q) for p, q in zip(x, y))
 
 
 # ---- together ------------------------------------------------------------------------------------

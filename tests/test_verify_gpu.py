@@ -135,6 +135,45 @@ def test_un_quantised_weights():
     assert ((a - b).norm(dim=-1) <= 2 * (34 / 3) ** 0.5 * 2 ** -11 * b.norm(dim=-1)).all()
 
 
+def test_the_right_branch_is_accepted_whole(tiny_model):
+    """Every call keeps all of the branch that greedy decoding takes, and the token after it (linears at a quarter of the scale: no
+    near ties)."""
+    _, _, state, config = tiny_model
+    net = qmodel.from_state_dict({k: v * 0.25 if k.endswith("weight_scale") else v for k, v in state.items()}, config)
+    g = torch.Generator().manual_seed(8)
+    prompts = [torch.randint(0, 2048, (n,), generator=g) for n in (33, 130, 70, 5)]
+    slots = [3, 0, 2, 1]
+    cache, plain = (net.new_cache(n_slots=4, s_max=256) for _ in range(2))
+    net.prefill(cache, slots, prompts)
+    net.prefill(plain, slots, prompts)
+    steps = net.decode(plain, slots, 40)
+    done = [0] * 4
+    for turn in range(4):
+        rights = [int(torch.randint(0, 7, (1,), generator=g)) for _ in slots]
+        drafts, parents = zip(*[_draft(s[n:n + right], g, 2048) for s, n, right in zip(steps, done, rights)])
+        for i, new in enumerate(net.verify(cache, slots, list(drafts), list(parents))):
+            # (the last node is drafted at random and may be right by chance)
+            assert rights[i] + 1 <= len(new) <= rights[i] + 2
+            assert new == steps[i][done[i]:done[i] + len(new)]
+            done[i] += len(new)
+
+
+def test_a_chain_is_accepted_by_un_quantised_weights():
+    """All of it, or up to a near tie of the logits that a prefill of the same text gives."""
+    from quic_cu_b200.checkpoint import qwen_config_dict, synthetic_dense_checkpoint
+
+    net = qmodel.from_state_dict(synthetic_dense_checkpoint(n_layers=2, vocab=2048, seed=5), qwen_config_dict(2, 2048))
+    for start in (0, 500):
+        prompt = torch.arange(start, start + 40)
+        caches = [net.new_cache(n_slots=1, s_max=128) for _ in range(3)]
+        first = [net.prefill(c, [0], [prompt])[0] for c in caches[:2]][0].cpu()
+        steps = net.decode(caches[0], [0], 6)[0]
+        got = net.verify(caches[1], [0], [steps[:5]])[0]
+        _, logits = net.prefill(caches[2], [0], [torch.cat([prompt, first, torch.tensor(steps[:5])])], all_logits=True)
+        compared = _near(got, steps, logits[40:].cpu())
+        assert len(got) == (6 if compared == 6 else compared + 1)
+
+
 def test_refusals(tiny_model):
     net, _, _, _ = tiny_model
     cache = net.new_cache(n_slots=3, s_max=32)
