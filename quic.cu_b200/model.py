@@ -584,8 +584,8 @@ class QUICForCausalLM:
         after them, at least one.
 
         ``drafts[i]``: token ids drafted for slots[i], any number (a list or a 1-D tensor on the host); the row's next token is
-        node 0 of the tree, drafts[i][j] node j + 1.  ``parents[i][j]``: the node before which it is drafted to follow, 0 .. j;
-        None: the drafts are a chain.  All rows' nodes must fit behind the cached tokens of their slots.
+        node 0 of the tree, drafts[i][j] node j + 1.  ``parents[i][j]``, 0 .. j: the node that drafts[i][j] directly follows, 0 the
+        row's next token, k > 0 drafts[i][k - 1]; None: the drafts are a chain.  All rows' nodes must fit behind the cached tokens of their slots.
 
         Raises if a bounded wait gave up in it, or in a prefill or step before it: nothing is accepted then, the rows' tokens,
         positions and cached keys are as before the call.
