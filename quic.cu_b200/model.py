@@ -694,24 +694,25 @@ class QUICForCausalLM:
                                           torch.tensor(lens)).to(dev, non_blocking=True)
         table = torch.tensor([bounds[:-1], lens, slots, offs], dtype=torch.int32).to(dev, non_blocking=True)
         seq_start, seq_len, seq_slot, seq_off = table[0], table[1], table[2], table[3]
-        h = self.embed[ids]
-        rms, lin = K.rmsnorm().forward, K.w4a16_linear
-        xn = rms(h, self.layers[0]["ln1"], self.eps)
-        for li, L in enumerate(self.layers):
-            qkv = lin(L["qkv"], xn)
-            # heads split, RoPE applied and K/V written into their slots by one kernel
-            q = K.qkv_rope_append(qkv, slot_of, pos, self.rope_cos, self.rope_sin, cache.kv[li, 0], cache.kv[li, 1])
-            attn = K.attn_prefill(q, cache.kv[li, 0], cache.kv[li, 1], seq_start, seq_len, seq_slot, max(lens),
-                                  seq_off=seq_off)
-            o = lin(L["o"], attn)
-            xn, h = rms(o, L["ln2"], self.eps, residual=h)
-            gu = lin(L["gate_up"], xn)
-            act = K.swiglu_fused(gu)
-            d = lin(L["down"], act)
-            nxt = self.layers[li + 1]["ln1"] if li + 1 < self.n_layers else self.final_norm
-            xn, h = rms(d, nxt, self.eps, residual=h)
-        last = torch.tensor([b - 1 for b in bounds[1:]], device=dev)
-        logits = K.gemm().forward(xn, self.embed)
+        with cache.watch(8):
+            h = self.embed[ids]
+            rms, lin = K.rmsnorm().forward, K.w4a16_linear
+            xn = rms(h, self.layers[0]["ln1"], self.eps)
+            for li, L in enumerate(self.layers):
+                qkv = lin(L["qkv"], xn)
+                # heads split, RoPE applied and K/V written into their slots by one kernel
+                q = K.qkv_rope_append(qkv, slot_of, pos, self.rope_cos, self.rope_sin, cache.kv[li, 0], cache.kv[li, 1])
+                attn = K.attn_prefill(q, cache.kv[li, 0], cache.kv[li, 1], seq_start, seq_len, seq_slot, max(lens),
+                                      seq_off=seq_off)
+                o = lin(L["o"], attn)
+                xn, h = rms(o, L["ln2"], self.eps, residual=h)
+                gu = lin(L["gate_up"], xn)
+                act = K.swiglu_fused(gu)
+                d = lin(L["down"], act)
+                nxt = self.layers[li + 1]["ln1"] if li + 1 < self.n_layers else self.final_norm
+                xn, h = rms(d, nxt, self.eps, residual=h)
+            last = torch.tensor([b - 1 for b in bounds[1:]], device=dev)
+            logits = K.gemm().forward(xn, self.embed)
         first = K.sampler().forward(logits[last].unsqueeze(1)).view(-1)
         st = torch.tensor(slots, device=dev, dtype=torch.long)
         cache.tok[st] = first.to(torch.int32)

@@ -148,6 +148,21 @@ def test_a_prefill_that_gave_up_is_heard_of_by_its_own_cache(tiny_model, length)
     assert K.lib().quic_w4a16_tensor_status() == 0
 
 
+def test_a_prefill_of_all_logits_that_gave_up_is_heard_of_too(tiny_model):
+    """It runs operator by operator; its cache hears of it all the same, and only it."""
+    net, slots = tiny_model[0], [0, 1]
+    good, bad = (net.new_cache(n_slots=2, s_max=256) for _ in range(2))
+    net.prefill(good, slots, _prompts(2, 40))
+    with _Hook():
+        net.prefill(bad, slots, _prompts(2, 40), all_logits=True)
+    assert K.lib().quic_w4a16_tensor_status() == 0
+    net.decode(good, slots, 2)
+    good.raise_errors()
+    with pytest.raises(RuntimeError, match="bounded wait.*in a prefill"):
+        net.decode(bad, slots, 2)
+    bad.raise_errors()
+
+
 def test_a_forward_step_that_gave_up_is_heard_of_by_the_next(tiny_model):
     """forward() does not wait for its step: the next one raises, or raise_errors() after a synchronisation."""
     net, rows = tiny_model[0], 20
