@@ -359,6 +359,10 @@ int quic_tree_attn(const quic_tree_attn_t *t, void *scratch, void *stream);
 int64_t quic_tree_attn_scratch_bytes(int32_t requests, int32_t heads,
                                      int32_t kv_heads, int32_t dim,
                                      int32_t max_new, int64_t max_len);
+/* Which of its two forms quic_tree_attn runs: -1 (default) whichever is faster
+ * by the sizes, 0 the mma.sync form, 1 the tcgen05 form where blocks (a multiple
+ * of 8 tokens) and strides (positive) allow it.  For A/B timing and tests. */
+void quic_set_tree_attn_tensor(int mode);
 
 typedef struct {
   int32_t *tables; /* [requests, max_blocks], rows table_row apart */
@@ -374,11 +378,6 @@ typedef struct {
   int32_t *mask;          /* [max_rows, mask_words], with parents */
   int32_t max_blocks, n_blocks, requests, block_size, parent_rows, mask_words, max_rows;
 } quic_block_tables_t;
-
-/* Which of its two forms quic_tree_attn runs: -1 (default) whichever is faster
- * by the sizes, 0 the mma.sync form, 1 the tcgen05 form where blocks (a multiple
- * of 8 tokens) and strides (positive) allow it.  For A/B timing and tests. */
-void quic_set_tree_attn_tensor(int mode);
 
 /* What a step needs to know of its requests, built on the device from their
  * lengths.  n_new[b] > 0: request b gets that many rows behind lengths[b] cached

@@ -243,7 +243,8 @@ __global__ void embed_rows_kernel(const half* __restrict__ embed, const int32_t*
 // already added) of a prefill: every row brings its own slot and position, q is written
 // head-major.  One thread per (row, head, 8 of the 64 dims), which reads the 8 stored pairs
 // its dims come from (32 bytes) with their cos / sin (16 bytes each) and writes 16 bytes.
-// kAt: row b goes to place at[b] of the cache, slot x s_max + position, instead of (slots[b], row_pos[b]).
+// kAt: row b goes to place at[b] of the cache, slot x s_max + position, instead of (slots[b], row_pos[b]); us with and without, at 1, 48
+// and 512 rows: 2.1 / 1.9, 2.6 / 2.4, 2.6 / 2.6 (a launch; 2.4 MB at 512 rows).
 template <bool kAt>
 __global__ void __launch_bounds__(256) qkv_rope_rows_kernel(
     const half* __restrict__ qkv, const int32_t* __restrict__ slots, const int32_t* __restrict__ row_pos,

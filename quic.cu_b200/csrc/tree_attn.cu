@@ -5,7 +5,8 @@
 // for node i of a request's tree over the request's cached positions 0 .. len - 1 and those of the nodes (position
 // len + a for node a) that it sees: its ancestors and itself by bit mask, or without masks nodes 0 .. i.  A chain, the next
 // chunk of a prompt and a single decode token are trees too.  The R = nodes x (query heads per KV head) rows of a
-// request and KV head share their keys; K and V are read once per tile of those rows.
+// request and KV head share their keys; K and V are read once per tile of those rows.  (A tile walks the keys to the end of its
+// request, those behind its last node as well: a prompt's chunk without cached tokens costs twice what it must.)
 //
 // This file: the form for few rows (mma.sync), the merge of many parts of a request, and the entry point; tree_attn_tc.cu has the form
 // for more rows.
@@ -576,23 +577,25 @@ int launch_few(const TreeArgs& a, cudaStream_t st) {
   return QUIC_OK;
 }
 
-// What the end of a segment and the beginning of the next cost a CTA of the tcgen05 form, in key tiles.  us with 0 / 3 / 5 / 7 / 9: 64 x 8
-// x 200..1500 (14:2) 26.2 / 23.7 / 22.5 / 22.0 / 23.0, 27 x 25 x 5074..10148 (16:1) 74.8 / 72.9 / 71.0 / 71.4 / 72.2, 8 x 64 x 12000..16384
-// 145.6 / 143.8 / 142.7 / 142.6 / 143.0, 10 x 38 x 4..23 (16:1) 22.0 / 14.5 / 14.4 / 14.3 / 14.6.
+// What the end of a segment and the beginning of the next cost a CTA of the tcgen05 form, in key tiles.  us with 0 / 3 / 5 / 6 / 7 / 9:
+// 64 x 8 x 200..1500 (14:2) 25.4 / 22.8 / 21.7 / 21.3 / 20.9 / 21.7, 27 x 25 x 5074..10148 (16:1) 67.4 / 66.9 / 65.2 / 65.0 / 64.8 / 65.2,
+// 8 x 64 x 12000..16384 132.5 / 131.4 / 131.1 / 130.9 / 131.1 / 131.3, 10 x 38 x 4..23 (16:1) 21.8 / 14.6 / 14.4 / 14.5 / 14.3 / 14.3.
 constexpr int kLineGap = 6;
 constexpr int64_t kMostTokens = 1 << 29;  // of a request: sums of two counts stay within an int
 // Which form takes a call, by the rows of a request and KV head and by the work of the mma.sync form, in tiles of 32 rows x keys of
 // 64 dims (for all requests, of the longest's keys).  The tcgen05 form has three times its throughput where it has the rows for it,
 // but 6 us more of launch and merge, and 3 us for every row tile of a CTA.  requests x nodes x tokens, us mma.sync / tcgen05:
-//   heads 14:2, dim 64:  5 x 23 x 388..777 9.2 / 12.9 (work 48,000), 1 x 48 x 4096 13.3 / 15.4 (91,000), 2 x 32 x 8192 16.8 / 18.5
-//                        (230,000), 64 x 5 x 500..1000 15.4 / 20.1 (257,000), 16 x 16 x 1024..2048 17.3 / 14.6 (264,000),
-//                        64 x 8 x 750..1500 21.7 / 23.1 (386,000), 16 x 8 x 4096..8192 28.7 / 22.4 (525,000)
-//   heads 32:8, dim 128: 20 x 28 x 7..15 15.5 / 17.3 (55,000), 4 x 16 x 512..1024 16.1 / 14.4 (133,000), 8 x 9 x 512..1024 21.5 / 20.7
-//                        (264,000), 16 x 9 x 256..512 20.3 / 22.2 (267,000), 4 x 9 x 2048..4096 31.5 / 21.0 (525,000)
-//   heads 16:1, dim 128: 16 x 2 x 1024..2048 15.5 / 14.4 (66,000), 4 x 8 x 2048..4096 16.4 / 15.1 (131,000), 32 x 2 x 4096..8192 32.6 /
-//                        30.2 (524,000)
-// Of up to 32 rows and 64 dims 9 x 13 x 7247..14495 (8:8) 41.7 / 53.3, 64 x 3 x 2000..4000 (14:2) 29.9 / 35.0.  Of 89 calls drawn over
-// these ranges the rule's form is 0.6 % behind the faster one on average.
+//   heads 14:2, dim 64:  5 x 23 x 388..777 9.2 / 12.8 (work 48,000), 1 x 48 x 4096 13.1 / 15.3 (91,000), 2 x 32 x 8192 17.4 / 18.0
+//                        (230,000), 64 x 5 x 500..1000 15.3 / 19.8 (257,000), 16 x 16 x 1024..2048 17.1 / 14.5 (264,000),
+//                        64 x 8 x 750..1500 21.8 / 23.0 (386,000), 16 x 8 x 4096..8192 28.4 / 22.3 (525,000)
+//   heads 32:8, dim 128: 20 x 28 x 7..15 15.3 / 17.2 (55,000), 4 x 16 x 512..1024 15.9 / 14.3 (133,000), 8 x 9 x 512..1024 21.6 / 20.6
+//                        (264,000), 16 x 9 x 256..512 20.0 / 22.0 (267,000), 4 x 9 x 2048..4096 31.4 / 21.0 (525,000)
+//   heads 16:1, dim 128: 16 x 2 x 1024..2048 15.4 / 14.3 (66,000), 4 x 8 x 2048..4096 16.4 / 14.8 (131,000), 32 x 2 x 4096..8192 32.4 /
+//                        30.0 (524,000)
+// Of up to 32 rows and 64 dims 9 x 13 x 7247..14495 (8:8) 41.9 / 53.1, 64 x 3 x 2000..4000 (14:2) 29.9 / 35.0.  Of 89 calls drawn over
+// these ranges the rule's form is 1.2 % behind the faster one on average: even with it for 84, and behind near the line by 46 % (51 x 20 x
+// 107, 32:8: 41.6 / 28.5), 33 % (1 x 13 x 17767, 16:1: 23.5 / 31.2), 17 % (22 x 33 x 7..14, 16:1: 14.4 / 12.3) and 7 %; of the calls above by
+// 18 % at 16 x 16 x 1024..2048, 11 % at 4 x 16 x 512..1024, 8 % at 16 x 2 x 1024..2048.
 bool tensor_pays(int64_t rows, int64_t units, int64_t bound, int dim) {
   const int64_t work = units * ((rows + 31) / 32) * bound * (dim / 64);
   return (rows > 32 || (rows > 16 && dim == 128)) &&
@@ -622,13 +625,13 @@ Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound
   }
   p.chunk = 64;
   // Parts by their cost in keys: waves of CTAs, each with 256 keys' worth of beginning and end; then the merge, by the cluster (64)
-  // or by a kernel of its own (192 and 4 a part).  us with the most parts that fit, cluster / kernel / one part, 14:2 heads of 64 (with
-  // loops that took 5 to 10 % longer):
-  // 1 x 1 x 300 5.1 / 6.1 / 5.6, 1 x 1 x 4000 8.4 / 8.1 (17 parts) / 31.8, 32 x 1 x 500..1000 7.3 / 8.9 / 10.7, 16 x 1 x 8192 18.4 /
-  // 19.7 / 69, 5 x 23 x 0..777 9.5 / 10.1 / 13.5, 1 x 48 x 4096 15.3 / 14.3 (12 parts) / 45.6, 64 x 8 x 200..1500 30.8 / 28.4 / 25.6;
-  // 32:8 heads of 128: 8 x 3 x 2000..4000 27.3 / 31.9 / 67.  The most parts of every number of waves are looked at.  (Equal shares of
-  // all requests' keys instead, which ragged requests would call for, cost a CTA two row tiles one after the other: 64 x 8 x
-  // 200..1500 34.)
+  // or by a kernel of its own (192 and 4 a part).  us with the best number of parts, cluster / kernel / one part, 14:2 heads of 64:
+  // 1 x 1 x 300 4.8 / 5.8 / 4.6, 1 x 1 x 4000 7.6 / 7.8 (17 parts) / 24.7, 32 x 1 x 500..1000 6.8 / 8.4 / 8.9, 16 x 1 x 8192 16.7 /
+  // 18.2 / 60, 5 x 23 x 0..777 8.7 / 10.0 / 11.1, 1 x 48 x 4096 12.5 (6) / 13.2 (12) / 39, 64 x 8 x 200..1500 25.1 / 22.1 / 18.6;
+  // 32:8 heads of 128: 8 x 3 x 2000..4000 23.3 / 27.5 / 52; 8:8 of 64: 9 x 13 x 7247..14495 41.3 / 40.7 / 94.  The costs, fitted to loops
+  // that took up to a third longer, take the best within 0.1 us but at 1 x 1 x 300 (4.9) and 1 x 48 x 4096 (13.1).  The most parts of
+  // every number of waves are looked at.  (Equal shares of all requests' keys instead, which ragged requests would call for, cost a CTA two
+  // row tiles one after the other: 64 x 8 x 200..1500 34 where the loop of that time took 25.6.)
   const int64_t units = (int64_t)requests * kv_heads * p.tiles, slots = kSlots[0];
   const int64_t most = bound < 256 ? 1 : (bound < 128 * 256 ? (bound + 255) / 256 : 128);
   int64_t best = 1, least = INT64_MAX;
@@ -645,9 +648,9 @@ Plan make_plan(int requests, int kv_heads, int heads, int max_new, int64_t bound
     if (cost < least) least = cost, best = s, p.cluster = true;
   }
   // ... or each warp has 32 rows of its own and all keys, with a quarter of the CTAs and no merge: for many rows and few keys, where
-  // the warps have rows.  us keys by warps / rows by warps: 14:2 heads of 64, 64 x 16 x 15..30 12.6 / 9.6, x 50..100 12.9 / 11.8,
-  // x 200..400 19.1 / 23.0; 32:8 of 128, 20 x 28 x 7..15 18.5 / 15.4, x 50..100 21.1 / 23.1, 64 x 16 x 10..20 33.4 / 24.2; 8:8 of 64,
-  // 20 x 40 x 25..50 (40 rows) 7.5 / 10.9.
+  // the warps have rows.  us keys by warps / rows by warps: 14:2 heads of 64, 64 x 16 x 15..30 12.4 / 9.0, x 50..100 12.6 / 10.6 (the
+  // rule takes the former), x 200..400 17.8 / 19.2; 32:8 of 128, 20 x 28 x 7..15 19.6 / 15.4, x 50..100 21.9 / 21.5, 64 x 16 x 10..20 35.3 /
+  // 24.0; 8:8 of 64, 20 x 40 x 25..50 (40 rows) 7.5 / 9.8.
   const int64_t wide = (rows + kByRowsTile - 1) / kByRowsTile, wide_units = (int64_t)requests * kv_heads * wide;
   if (best == 1 && rows > 32 && 2 * rows >= wide * kByRowsTile &&
       192 + (wide_units + slots - 1) / slots * ((dim == 64 ? 4 : 6) * bound + 96) <

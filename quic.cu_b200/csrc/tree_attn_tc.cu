@@ -18,10 +18,11 @@
 // must not see: such values are zeroed in shared memory and added, at the end, to the rows that see them.
 //
 // The CTAs have equal shares of the line of key tiles of all requests (tree_attn.cuh): the same case 193 -> 143 us, with an issuer
-// per stream instead of one for both.  132 us now (3.6 TB/s, 750 TFLOP/s).  Of them K and V alone take 101, with the products 112.  A
-// softmax warp takes 1900 clocks a tile (280 for the maximum, 100 for the load, 500 for barriers and the way round, the rest for the
-// weights) and is the slowest part; two of them share a scheduler.  With all exponentials on their unit (512 clocks a warp and tile, 54 %
-// busy) it was 143; three in eight are polynomials.  Tried and behind: scores fetched during the last exponentials 153, weights by the
+// per stream instead of one for both.  126 to 132 us now (3.6 to 3.8 TB/s, 750 to 780 TFLOP/s) at the 1.8 GHz that it has after a rest, 152 to
+// 156 at the 1.53 GHz that calls one after the other settle at (power limit): 2170 clocks a tile by stamps in both.  Of the 143, K and V alone
+// took 101, with the products 112.  A softmax warp's clocks: 1150 to 1550 from complete scores to stored weights (1550 the slowest of a
+// stream's four, which sets the pace), 150 to 500 until the scores are complete, 450 for the way round; two of them share a scheduler.  With all exponentials on their unit (512 clocks a warp
+// and tile, 54 % busy) it was 143; three in eight are polynomials.  Tried and behind: scores fetched during the last exponentials 153, weights by the
 // old maximum before the new one is known 157, two threads a row 187, one lane of a warp waiting for all 170, two CTAs an SM with a
 // stream each 27 -> 31 us at 4 x 15 x 6146.
 //

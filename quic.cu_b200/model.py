@@ -591,7 +591,9 @@ class QUICForCausalLM:
         positions and cached keys are as before the call.
 
         The linears run at the sum of the rows' nodes; attention is ``kernels.tree_attn`` over the slots, whose tables
-        ``kernels.block_tables`` builds from the rows' lengths, and ``kernels.tree_commit`` keeps the branch."""
+        ``kernels.block_tables`` builds from the rows' lengths, and ``kernels.tree_commit`` keeps the branch.  They are called one by
+        one: 3 ms of host time a call with 24 layers, whatever the rows up to 64 (eight steps of ``decode`` for one row, six for
+        eight)."""
         cache.check_slots(slots, len(drafts), "verify")
         if not slots:
             raise RuntimeError("verify: empty batch")
